@@ -1,0 +1,684 @@
+// The row-wise steps of a DiT block for training: LayerNorm with adaLN modulation and RMSNorm with rotary embedding,
+// forward (keeping the row statistics) and backward (with the column sums that are the gradients of the per-channel
+// vectors).  Rows are x[b, s, :] of a [B, S, D] tensor; n is the normalised row.
+//
+//   LayerNorm   n = (x - mean) rstd      y = (n w + c) (1 + scale_b) + shift_b
+//               g = dy (1 + scale_b) w   dx = rstd (g - mean(g) - n mean(g n))
+//               A_b = sum_s dy, N_b = sum_s dy n:   dshift_b = A_b, dscale_b = w N_b + c A_b,
+//               dw = sum_b (1 + scale_b) N_b, dc = sum_b (1 + scale_b) A_b
+//   RMSNorm     n = x rstd               y = R_s (n w)   (R_s rotates channel pairs by the angles of table row s)
+//               h = R_s^T dy, g = h w    dx = rstd (g - n mean(g n)),   dw = sum_{b, s} h n
+//
+// Bound by HBM: the forward pass reads x and writes y, the backward pass reads x and dy and writes dx, each once.  One
+// CTA owns a row at a time and walks over the rows of one sample; a thread owns the same 16-byte pieces of every row, so
+//  - the rows travel through a ring in shared memory that each thread fills (cp.async) and reads back for itself: the
+//    bytes in flight cost neither registers nor barriers;
+//  - the column sums over the CTA's rows stay in the thread's registers (fp32, rows in a fixed order) and reach memory
+//    once per CTA; a second kernel adds the CTAs' partial sums in a fixed order, so results do not depend on timing.
+// Statistics, coefficients and sums are fp32; y and dx are rounded once, when they are stored.
+#include <algorithm>
+
+#include "quant_common.cuh"
+
+namespace dax {
+namespace {
+
+constexpr int kStages = 3;          // rows in the ring: one in use, two in flight
+constexpr int64_t kMaxWidth = 8192;
+
+struct NormArgs {
+  const uint8_t* x;       // input rows
+  const uint8_t* dy;      // backward: gradient rows
+  uint8_t* out;           // y (forward) or dx (backward)
+  int64_t x_sb, x_ss, dy_sb, dy_ss, out_sb, out_ss;  // byte strides: sample, token
+  const float* weight;    // [D] or null (1)
+  const float* bias;      // [D] or null (0)
+  const float* shift;     // [B, D] or null (0)
+  const float* scale;     // [B, D] or null (0)
+  const float* cos;       // [S, 64] or null (no rotation)
+  const float* sin;
+  float* mean;            // [B, S] statistics: written forward, read backward (LayerNorm)
+  float* rstd;            // [B, S]
+  float* part;            // backward: [B, gridDim.x, SUMS, D] column sums
+  int64_t S;
+  int D;
+  float eps;
+};
+
+__device__ __forceinline__ void cp_async16(void* smem_dst, const void* gmem_src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(smem_dst))),
+               "l"(gmem_src) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// ---- 16-byte pieces: eight 16-bit or four fp32 elements ------------------------------------------------------------
+template <int DT> struct Piece { static constexpr int value = DT == DAX_F32 ? 4 : 8; };
+
+template <int DT>
+__device__ __forceinline__ void unpack(const uint4& r, float (&f)[Piece<DT>::value]) {
+  if constexpr (DT == DAX_F32) {
+    f[0] = __uint_as_float(r.x); f[1] = __uint_as_float(r.y); f[2] = __uint_as_float(r.z); f[3] = __uint_as_float(r.w);
+  } else {
+    unpack2<DT == DAX_BF16>(r.x, f[0], f[1]);
+    unpack2<DT == DAX_BF16>(r.y, f[2], f[3]);
+    unpack2<DT == DAX_BF16>(r.z, f[4], f[5]);
+    unpack2<DT == DAX_BF16>(r.w, f[6], f[7]);
+  }
+}
+template <int DT>
+__device__ __forceinline__ uint4 pack(const float (&f)[Piece<DT>::value]) {
+  if constexpr (DT == DAX_F32) {
+    return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+  } else {
+    return make_uint4(pack2_rn<DT == DAX_BF16>(f[0], f[1]), pack2_rn<DT == DAX_BF16>(f[2], f[3]),
+                      pack2_rn<DT == DAX_BF16>(f[4], f[5]), pack2_rn<DT == DAX_BF16>(f[6], f[7]));
+  }
+}
+template <int N>
+__device__ __forceinline__ void load_f32(const float* p, float (&f)[N]) {
+#pragma unroll
+  for (int k = 0; k < N; k += 4) *reinterpret_cast<float4*>(&f[k]) = *reinterpret_cast<const float4*>(p + k);
+}
+template <int N>
+__device__ __forceinline__ void store_f32(float* p, const float (&f)[N]) {
+#pragma unroll
+  for (int k = 0; k < N; k += 4) *reinterpret_cast<float4*>(p + k) = *reinterpret_cast<const float4*>(&f[k]);
+}
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+// Sums of a pair of values over the CTA, the same number in every thread.  The caller alternates between two slots, so
+// one barrier per reduction is enough: a slot is written again only after the barrier of the reduction in between.
+__device__ __forceinline__ void cta_sum2(float& a, float& c, float2* slot) {
+  a = warp_sum(a);
+  c = warp_sum(c);
+  const int warps = blockDim.x >> 5;
+  if (warps == 1) return;
+  if ((threadIdx.x & 31) == 0) slot[threadIdx.x >> 5] = make_float2(a, c);
+  __syncthreads();
+  a = slot[0].x;
+  c = slot[0].y;
+  for (int k = 1; k < warps; ++k) {
+    a += slot[k].x;
+    c += slot[k].y;
+  }
+}
+
+// The rotary factors of this thread's pairs: a head has 128 channels and blockDim.x pieces are a whole number of heads,
+// so all pieces of a thread sit at the same channels of their heads and share the factors.
+template <int DT> struct Rotary { float c[Piece<DT>::value / 2], s[Piece<DT>::value / 2]; };
+template <int DT>
+__device__ __forceinline__ void load_rotary(const NormArgs& p, int64_t row, Rotary<DT>& r) {
+  constexpr int E = Piece<DT>::value;
+  const int pair = (threadIdx.x * E % 128) / 2;
+#pragma unroll
+  for (int k = 0; k < E / 2; k += 2) {
+    *reinterpret_cast<float2*>(&r.c[k]) = *reinterpret_cast<const float2*>(p.cos + row * 64 + pair + k);
+    *reinterpret_cast<float2*>(&r.s[k]) = *reinterpret_cast<const float2*>(p.sin + row * 64 + pair + k);
+  }
+}
+
+// ---- forward ---------------------------------------------------------------------------------------------------------
+template <int DT, int NV, bool LN>
+__global__ void __launch_bounds__(512) norm_forward_kernel(const NormArgs p) {
+  constexpr int E = Piece<DT>::value;
+  extern __shared__ uint4 ring[];  // [kStages][NV][blockDim.x], then the coefficients
+  __shared__ float2 red[2][16];
+  const int T = blockDim.x, tid = threadIdx.x, b = blockIdx.y;
+  const int pieces = p.D / E;
+  const uint8_t* x = p.x + b * p.x_sb;
+  uint8_t* y = p.out + b * p.out_sb;
+
+  // y = n mul + add per channel, folded once per CTA; a thread reads back only what it wrote: no barrier
+  const bool coef = p.weight != nullptr || p.scale != nullptr;
+  float4* mul_s = reinterpret_cast<float4*>(ring + kStages * NV * T);
+  float4* add_s = mul_s + NV * (E / 4) * T;
+  if (coef) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int v = tid + i * T;
+      if (v >= pieces) continue;
+      float m[E], a[E], t[E];
+#pragma unroll
+      for (int k = 0; k < E; ++k) { m[k] = 1.f; a[k] = 0.f; }
+      if (p.weight != nullptr) load_f32<E>(p.weight + v * E, m);
+      if (LN && p.bias != nullptr) load_f32<E>(p.bias + v * E, a);
+      if (LN && p.scale != nullptr) {
+        load_f32<E>(p.scale + static_cast<int64_t>(b) * p.D + v * E, t);
+#pragma unroll
+        for (int k = 0; k < E; ++k) { m[k] *= 1.f + t[k]; a[k] *= 1.f + t[k]; }
+        load_f32<E>(p.shift + static_cast<int64_t>(b) * p.D + v * E, t);
+#pragma unroll
+        for (int k = 0; k < E; ++k) a[k] += t[k];
+      }
+#pragma unroll
+      for (int q = 0; q < E / 4; ++q) {
+        mul_s[(i * (E / 4) + q) * T + tid] = *reinterpret_cast<float4*>(&m[4 * q]);
+        if (LN) add_s[(i * (E / 4) + q) * T + tid] = *reinterpret_cast<float4*>(&a[4 * q]);
+      }
+    }
+  }
+
+  auto fetch = [&](int64_t row, int stage) {
+    if (row < p.S) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int v = tid + i * T;
+        if (v < pieces) cp_async16(&ring[(stage * NV + i) * T + tid], x + row * p.x_ss + v * 16);
+      }
+    }
+    cp_async_commit();  // one group per row, empty past the end: the group count stays uniform
+  };
+  const int64_t step = gridDim.x;
+  int64_t row = blockIdx.x;
+#pragma unroll
+  for (int k = 0; k < kStages - 1; ++k) fetch(row + k * step, k);
+  const float inv_d = 1.f / static_cast<float>(p.D);
+  int stage = 0;
+  for (; row < p.S; row += step) {
+    fetch(row + (kStages - 1) * step, stage == 0 ? kStages - 1 : stage - 1);
+    Rotary<DT> rot;
+    if (!LN && p.cos != nullptr) load_rotary<DT>(p, row, rot);
+    cp_async_wait<kStages - 1>();  // this thread's pieces of the row have landed
+    float f[NV][E];
+    float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      if (tid + i * T < pieces) {
+        unpack<DT>(ring[(stage * NV + i) * T + tid], f[i]);
+#pragma unroll
+        for (int k = 0; k < E; ++k) {
+          if (LN) s0 += f[i][k];
+          else s0 = fmaf(f[i][k], f[i][k], s0);
+        }
+      }
+    }
+    cta_sum2(s0, s1, red[0]);
+    float mean = 0.f, var;
+    if (LN) {
+      // second pass around the first estimate of the mean: exact enough for rows whose mean dwarfs their spread, and
+      // it takes the rounding of that estimate out again (a constant row normalises to zero)
+      const float m0 = s0 * inv_d;
+      s0 = s1 = 0.f;
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        if (tid + i * T < pieces) {
+#pragma unroll
+          for (int k = 0; k < E; ++k) {
+            const float d = f[i][k] - m0;
+            s0 += d;
+            s1 = fmaf(d, d, s1);
+          }
+        }
+      cta_sum2(s0, s1, red[1]);
+      const float dm = s0 * inv_d;
+      mean = m0 + dm;
+      var = fmaxf(fmaf(-dm, dm, s1 * inv_d), 0.f);
+    } else {
+      var = s0 * inv_d;
+      __syncthreads();  // the one slot in use is written again by the next row
+    }
+    const float rstd = rsqrtf(var + p.eps);
+    if (tid == 0) {
+      if (LN) p.mean[static_cast<int64_t>(b) * p.S + row] = mean;
+      p.rstd[static_cast<int64_t>(b) * p.S + row] = rstd;
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      if (tid + i * T >= pieces) continue;
+#pragma unroll
+      for (int k = 0; k < E; ++k) f[i][k] = (f[i][k] - mean) * rstd;
+      if (coef) {
+#pragma unroll
+        for (int q = 0; q < E / 4; ++q) {
+          const float4 m = mul_s[(i * (E / 4) + q) * T + tid];
+          float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (LN) a = add_s[(i * (E / 4) + q) * T + tid];
+          f[i][4 * q] = fmaf(f[i][4 * q], m.x, a.x);
+          f[i][4 * q + 1] = fmaf(f[i][4 * q + 1], m.y, a.y);
+          f[i][4 * q + 2] = fmaf(f[i][4 * q + 2], m.z, a.z);
+          f[i][4 * q + 3] = fmaf(f[i][4 * q + 3], m.w, a.w);
+        }
+      }
+      if (!LN && p.cos != nullptr) {
+#pragma unroll
+        for (int k = 0; k < E / 2; ++k) {
+          const float u = f[i][2 * k], w = f[i][2 * k + 1];
+          f[i][2 * k] = u * rot.c[k] - w * rot.s[k];
+          f[i][2 * k + 1] = fmaf(u, rot.s[k], w * rot.c[k]);
+        }
+      }
+      *reinterpret_cast<uint4*>(y + row * p.out_ss + (tid + i * T) * 16) = pack<DT>(f[i]);
+    }
+    stage = stage == kStages - 1 ? 0 : stage + 1;
+  }
+}
+
+// ---- backward --------------------------------------------------------------------------------------------------------
+// SUMS: column sums kept (0: none wanted; LayerNorm 2: A and N; RMSNorm 1: N).
+template <int DT, int NV, bool LN, int SUMS>
+__global__ void __launch_bounds__(512) norm_backward_kernel(const NormArgs p) {
+  constexpr int E = Piece<DT>::value;
+  extern __shared__ uint4 ring[];  // [kStages][2][NV][blockDim.x], then the coefficients
+  __shared__ float2 red[2][16];
+  const int T = blockDim.x, tid = threadIdx.x, b = blockIdx.y;
+  const int pieces = p.D / E;
+  const uint8_t* x = p.x + b * p.x_sb;
+  const uint8_t* dy = p.dy + b * p.dy_sb;
+  uint8_t* dx = p.out + b * p.out_sb;
+  const float* mean_b = LN ? p.mean + static_cast<int64_t>(b) * p.S : nullptr;
+  const float* rstd_b = p.rstd + static_cast<int64_t>(b) * p.S;
+
+  const bool coef = p.weight != nullptr || p.scale != nullptr;  // g = dy mul
+  float4* mul_s = reinterpret_cast<float4*>(ring + kStages * 2 * NV * T);
+  if (coef) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int v = tid + i * T;
+      if (v >= pieces) continue;
+      float m[E], t[E];
+#pragma unroll
+      for (int k = 0; k < E; ++k) m[k] = 1.f;
+      if (p.weight != nullptr) load_f32<E>(p.weight + v * E, m);
+      if (LN && p.scale != nullptr) {
+        load_f32<E>(p.scale + static_cast<int64_t>(b) * p.D + v * E, t);
+#pragma unroll
+        for (int k = 0; k < E; ++k) m[k] *= 1.f + t[k];
+      }
+#pragma unroll
+      for (int q = 0; q < E / 4; ++q) mul_s[(i * (E / 4) + q) * T + tid] = *reinterpret_cast<float4*>(&m[4 * q]);
+    }
+  }
+
+  auto fetch = [&](int64_t row, int stage) {
+    if (row < p.S) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int v = tid + i * T;
+        if (v < pieces) {
+          cp_async16(&ring[(stage * 2 * NV + i) * T + tid], x + row * p.x_ss + v * 16);
+          cp_async16(&ring[((stage * 2 + 1) * NV + i) * T + tid], dy + row * p.dy_ss + v * 16);
+        }
+      }
+    }
+    cp_async_commit();
+  };
+  float sum_n[SUMS > 0 ? NV : 1][E], sum_a[SUMS > 1 ? NV : 1][E];
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int k = 0; k < E; ++k) {
+      if (SUMS > 0) sum_n[SUMS > 0 ? i : 0][k] = 0.f;
+      if (SUMS > 1) sum_a[SUMS > 1 ? i : 0][k] = 0.f;
+    }
+
+  const int64_t step = gridDim.x;
+  int64_t row = blockIdx.x;
+#pragma unroll
+  for (int k = 0; k < kStages - 1; ++k) fetch(row + k * step, k);
+  const float inv_d = 1.f / static_cast<float>(p.D);
+  int stage = 0, parity = 0;
+  // the statistics of a row are read one row ahead
+  float mean_next = 0.f, rstd_next = 0.f;
+  if (row < p.S) {
+    if (LN) mean_next = mean_b[row];
+    rstd_next = rstd_b[row];
+  }
+  for (; row < p.S; row += step) {
+    fetch(row + (kStages - 1) * step, stage == 0 ? kStages - 1 : stage - 1);
+    const float mean = mean_next, rstd = rstd_next;
+    if (row + step < p.S) {
+      if (LN) mean_next = mean_b[row + step];
+      rstd_next = rstd_b[row + step];
+    }
+    Rotary<DT> rot;
+    if (!LN && p.cos != nullptr) load_rotary<DT>(p, row, rot);
+    cp_async_wait<kStages - 1>();
+    float n[NV][E], g[NV][E];
+    float s_g = 0.f, s_gn = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      if (tid + i * T >= pieces) continue;
+      unpack<DT>(ring[(stage * 2 * NV + i) * T + tid], n[i]);
+      unpack<DT>(ring[((stage * 2 + 1) * NV + i) * T + tid], g[i]);
+      if (!LN && p.cos != nullptr) {  // rotate the gradient back
+#pragma unroll
+        for (int k = 0; k < E / 2; ++k) {
+          const float u = g[i][2 * k], w = g[i][2 * k + 1];
+          g[i][2 * k] = fmaf(u, rot.c[k], w * rot.s[k]);
+          g[i][2 * k + 1] = w * rot.c[k] - u * rot.s[k];
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < E; ++k) {
+        n[i][k] = (n[i][k] - mean) * rstd;
+        if (SUMS > 0) sum_n[SUMS > 0 ? i : 0][k] = fmaf(g[i][k], n[i][k], sum_n[SUMS > 0 ? i : 0][k]);
+        if (SUMS > 1) sum_a[SUMS > 1 ? i : 0][k] += g[i][k];
+      }
+      if (coef) {
+#pragma unroll
+        for (int q = 0; q < E / 4; ++q) {
+          const float4 m = mul_s[(i * (E / 4) + q) * T + tid];
+          g[i][4 * q] *= m.x;
+          g[i][4 * q + 1] *= m.y;
+          g[i][4 * q + 2] *= m.z;
+          g[i][4 * q + 3] *= m.w;
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < E; ++k) {
+        if (LN) s_g += g[i][k];
+        s_gn = fmaf(g[i][k], n[i][k], s_gn);
+      }
+    }
+    cta_sum2(s_g, s_gn, red[parity]);
+    const float m_g = s_g * inv_d, m_gn = s_gn * inv_d;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      if (tid + i * T >= pieces) continue;
+      float o[E];
+#pragma unroll
+      for (int k = 0; k < E; ++k) o[k] = (fmaf(-n[i][k], m_gn, g[i][k]) - (LN ? m_g : 0.f)) * rstd;
+      *reinterpret_cast<uint4*>(dx + row * p.out_ss + (tid + i * T) * 16) = pack<DT>(o);
+    }
+    stage = stage == kStages - 1 ? 0 : stage + 1;
+    parity ^= 1;
+  }
+  if constexpr (SUMS > 0) {
+    float* part = p.part + (static_cast<int64_t>(b) * gridDim.x + blockIdx.x) * SUMS * p.D;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int v = tid + i * T;
+      if (v >= pieces) continue;
+      store_f32<E>(part + v * E, sum_n[SUMS > 0 ? i : 0]);
+      if (SUMS > 1) store_f32<E>(part + p.D + v * E, sum_a[SUMS > 1 ? i : 0]);
+    }
+  }
+}
+
+// ---- column sums over the CTAs ---------------------------------------------------------------------------------------
+// A block owns 32 channels: 16 thread rows add every 16th partial sum, then one row adds the 16 results, always in the
+// same order.
+struct JoinArgs {
+  const float* part;  // [B, ctas, SUMS, D]
+  const float* weight;
+  const float* bias;
+  const float* scale;
+  float* dweight;
+  float* dbias;
+  float* dshift;
+  float* dscale;
+  int B, ctas, D;
+};
+template <int SUMS>
+__global__ void __launch_bounds__(512) norm_join_kernel(const JoinArgs p) {
+  __shared__ float sm[2][16][33];
+  const int tx = threadIdx.x, ty = threadIdx.y;
+  const int n = blockIdx.x * 32 + tx;
+  const bool in = n < p.D;
+  float dw = 0.f, dc = 0.f;
+  for (int b = 0; b < p.B; ++b) {
+    float s_n = 0.f, s_a = 0.f;
+    if (in) {
+      const float* q = p.part + static_cast<int64_t>(b) * p.ctas * SUMS * p.D + n;
+      for (int c = ty; c < p.ctas; c += 16) {
+        s_n += q[static_cast<int64_t>(c) * SUMS * p.D];
+        if (SUMS > 1) s_a += q[static_cast<int64_t>(c) * SUMS * p.D + p.D];
+      }
+    }
+    __syncthreads();
+    sm[0][ty][tx] = s_n;
+    sm[1][ty][tx] = s_a;
+    __syncthreads();
+    if (ty == 0 && in) {
+      s_n = s_a = 0.f;
+      for (int k = 0; k < 16; ++k) {
+        s_n += sm[0][k][tx];
+        s_a += sm[1][k][tx];
+      }
+      const int64_t at = static_cast<int64_t>(b) * p.D + n;
+      const float m = p.scale != nullptr ? 1.f + p.scale[at] : 1.f;
+      if (p.dshift != nullptr) p.dshift[at] = s_a;
+      if (p.dscale != nullptr) {
+        const float w = p.weight != nullptr ? p.weight[n] : 1.f, c = p.bias != nullptr ? p.bias[n] : 0.f;
+        p.dscale[at] = fmaf(w, s_n, c * s_a);
+      }
+      dw = fmaf(m, s_n, dw);
+      dc = fmaf(m, s_a, dc);
+    }
+  }
+  if (ty == 0 && in) {
+    if (p.dweight != nullptr) p.dweight[n] = dw;
+    if (p.dbias != nullptr) p.dbias[n] = dc;
+  }
+}
+
+// ---- launch shapes -----------------------------------------------------------------------------------------------------
+// Pieces per thread: one up to 256 pieces per row (threads beyond that add barrier time), two up to 640, else four.
+struct RowShape { int nv, threads; };
+inline RowShape row_shape(int64_t D, int dtype) {
+  const int64_t pieces = D * dtype_bytes(dtype) / 16;
+  const int nv = pieces <= 256 ? 1 : (pieces <= 640 ? 2 : 4);
+  const int64_t threads = ((pieces + nv - 1) / nv + 31) / 32 * 32;
+  return {nv, static_cast<int>(threads)};
+}
+// CTAs that stay resident and stride over the rows, over all samples: what fits on the GPU at once, and no more than 1024
+// threads or 16 CTAs per SM (more adds nothing to the bytes in flight, but partial sums to join).
+inline int64_t max_ctas(int64_t B, int64_t S, int threads) {
+  const int64_t per_sm = std::min<int64_t>(16, std::max<int64_t>(1, 1024 / threads));
+  return std::min(S, std::max<int64_t>(1, per_sm * sm_count() / B));
+}
+
+template <typename K>
+int launch_rows(K kernel, const NormArgs& p, int64_t B, int threads, size_t smem, int64_t* ctas, cudaStream_t st) {
+  if (smem > 40 * 1024) DAX_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+  int per_sm = 0;
+  DAX_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, threads, smem));
+  *ctas = std::min(max_ctas(B, p.S, threads), std::max<int64_t>(1, static_cast<int64_t>(per_sm) * sm_count() / B));
+  kernel<<<dim3(static_cast<unsigned>(*ctas), static_cast<unsigned>(B)), threads, smem, st>>>(p);
+  DAX_CUDA(cudaGetLastError());
+  return DAX_OK;
+}
+
+template <int DT, int NV, bool LN>
+int run_nv(const NormArgs& p, int64_t B, int threads, int64_t* ctas, int sums, bool backward, cudaStream_t st) {
+  constexpr size_t coef = static_cast<size_t>(Piece<DT>::value) * 4;  // bytes of one fp32 vector for a piece
+  const bool has_coef = p.weight != nullptr || p.scale != nullptr;
+  const size_t slots = static_cast<size_t>(NV) * threads;
+  if (!backward) {
+    const size_t smem = slots * (kStages * 16 + (has_coef ? (LN ? 2 : 1) * coef : 0));
+    return launch_rows(norm_forward_kernel<DT, NV, LN>, p, B, threads, smem, ctas, st);
+  }
+  const size_t smem = slots * (kStages * 32 + (has_coef ? coef : 0));
+  if (sums == 0) return launch_rows(norm_backward_kernel<DT, NV, LN, 0>, p, B, threads, smem, ctas, st);
+  return launch_rows(norm_backward_kernel<DT, NV, LN, LN ? 2 : 1>, p, B, threads, smem, ctas, st);
+}
+
+template <bool LN>
+int run_rows(const NormArgs& p, int dtype, int64_t B, int64_t* ctas, int sums, bool backward, cudaStream_t st) {
+  const RowShape s = row_shape(p.D, dtype);
+#define DAX_ROWS(DT, N) \
+  if (dtype == DT && s.nv == N) return run_nv<DT, N, LN>(p, B, s.threads, ctas, sums, backward, st)
+  DAX_ROWS(DAX_BF16, 1); DAX_ROWS(DAX_BF16, 2); DAX_ROWS(DAX_BF16, 4);
+  DAX_ROWS(DAX_F16, 1); DAX_ROWS(DAX_F16, 2); DAX_ROWS(DAX_F16, 4);
+  DAX_ROWS(DAX_F32, 1); DAX_ROWS(DAX_F32, 2); DAX_ROWS(DAX_F32, 4);
+#undef DAX_ROWS
+  return fail(DAX_ERR_UNSUPPORTED, "norm: dtype %d is not BF16/F16/F32", dtype);
+}
+
+int check_rows(const char* what, int dtype, int64_t B, int64_t S, int64_t D) {
+  DAX_REQUIRE(B >= 0 && S >= 0 && D > 0, DAX_ERR_INVALID, "%s: bad shape B=%lld S=%lld D=%lld", what, (long long)B, (long long)S, (long long)D);
+  DAX_REQUIRE(dtype == DAX_BF16 || dtype == DAX_F16 || dtype == DAX_F32, DAX_ERR_UNSUPPORTED, "%s: dtype %d is not BF16/F16/F32", what, dtype);
+  DAX_REQUIRE(D % 8 == 0 && D <= kMaxWidth, DAX_ERR_UNSUPPORTED, "%s: D=%lld must be a multiple of 8 and at most %lld", what,
+              (long long)D, (long long)kMaxWidth);
+  DAX_REQUIRE(B <= 65535, DAX_ERR_UNSUPPORTED, "%s: batch %lld exceeds 65535", what, (long long)B);
+  return DAX_OK;
+}
+int check_tensor(const char* what, const char* name, const void* t, int64_t sb, int64_t ss, int dtype) {
+  DAX_REQUIRE(t != nullptr, DAX_ERR_INVALID, "%s: %s is null", what, name);
+  const int64_t e = dtype_bytes(dtype);
+  DAX_REQUIRE(aligned16(t) && sb * e % 16 == 0 && ss * e % 16 == 0, DAX_ERR_ALIGN,
+              "%s: %s must be 16-byte aligned, with sample and token strides of whole 16 bytes", what, name);
+  return DAX_OK;
+}
+int check_vectors(const char* what, std::initializer_list<const void*> vs) {
+  for (const void* v : vs) DAX_REQUIRE(aligned16(v), DAX_ERR_ALIGN, "%s: the per-channel vectors must be 16-byte aligned", what);
+  return DAX_OK;
+}
+#define DAX_TRY(expr)              \
+  do {                             \
+    const int rc__ = (expr);       \
+    if (rc__ != DAX_OK) return rc__; \
+  } while (0)
+
+template <bool LN>
+int forward(NormArgs p, int dtype, int64_t B, int64_t D, cudaStream_t st) {
+  if (B == 0 || p.S == 0) return DAX_OK;
+  const int64_t e = dtype_bytes(dtype);
+  p.D = static_cast<int>(D);
+  p.x_sb *= e; p.x_ss *= e; p.out_sb *= e; p.out_ss *= e;
+  int64_t ctas = 0;
+  return run_rows<LN>(p, dtype, B, &ctas, 0, false, st);
+}
+
+template <bool LN>
+int backward(const char* what, NormArgs p, JoinArgs j, int dtype, int64_t B, int64_t D, void* workspace, size_t bytes, cudaStream_t st) {
+  const bool want = j.dweight != nullptr || j.dbias != nullptr || j.dshift != nullptr || j.dscale != nullptr;
+  const int sums = want ? (LN ? 2 : 1) : 0;
+  int64_t ctas = B > 0 ? max_ctas(B, p.S, row_shape(D, dtype).threads) : 0;
+  if (want) {
+    const size_t need = static_cast<size_t>(B) * ctas * sums * D * 4;
+    DAX_REQUIRE(bytes >= need && (need == 0 || workspace != nullptr), DAX_ERR_INVALID,
+                "%s: workspace of %zu bytes is smaller than the %zu required", what, bytes, need);
+    DAX_REQUIRE(aligned16(workspace), DAX_ERR_ALIGN, "%s: workspace must be 16-byte aligned", what);
+  }
+  const int64_t e = dtype_bytes(dtype);
+  p.D = static_cast<int>(D);
+  p.x_sb *= e; p.x_ss *= e; p.dy_sb *= e; p.dy_ss *= e; p.out_sb *= e; p.out_ss *= e;
+  p.part = static_cast<float*>(workspace);
+  if (B > 0 && p.S > 0) DAX_TRY(run_rows<LN>(p, dtype, B, &ctas, sums, true, st));
+  if (want) {
+    j.part = p.part;
+    j.B = static_cast<int>(B);
+    j.ctas = static_cast<int>(ctas);
+    j.D = p.D;
+    norm_join_kernel<LN ? 2 : 1><<<static_cast<unsigned>((D + 31) / 32), dim3(32, 16), 0, st>>>(j);
+    DAX_CUDA(cudaGetLastError());
+  }
+  return DAX_OK;
+}
+
+}  // namespace
+}  // namespace dax
+
+extern "C" {
+
+size_t dax_norm_backward_workspace_bytes(int64_t B, int64_t S, int64_t D, int dtype) {
+  if (B <= 0 || S <= 0 || D <= 0 || D > dax::kMaxWidth || dax::dtype_bytes(dtype) < 2) return 0;
+  return static_cast<size_t>(B) * dax::max_ctas(B, S, dax::row_shape(D, dtype).threads) * 2 * D * 4;
+}
+
+int dax_layernorm_modulate(const void* x, int dtype, int64_t B, int64_t S, int64_t D, int64_t x_sb, int64_t x_ss,
+                           const float* ln_weight, const float* ln_bias, const float* shift, const float* scale, float eps,
+                           void* y, int64_t y_sb, int64_t y_ss, float* mean, float* rstd, void* stream) {
+  using namespace dax;
+  const char* what = "layernorm_modulate";
+  DAX_TRY(check_rows(what, dtype, B, S, D));
+  if (B == 0 || S == 0) return DAX_OK;
+  DAX_TRY(check_tensor(what, "x", x, x_sb, x_ss, dtype));
+  DAX_TRY(check_tensor(what, "y", y, y_sb, y_ss, dtype));
+  DAX_REQUIRE(mean != nullptr && rstd != nullptr, DAX_ERR_INVALID, "%s: mean and rstd are needed", what);
+  DAX_REQUIRE((shift == nullptr) == (scale == nullptr), DAX_ERR_INVALID, "%s: shift and scale come together", what);
+  DAX_REQUIRE(ln_bias == nullptr || ln_weight != nullptr, DAX_ERR_INVALID, "%s: bias needs weight", what);
+  DAX_TRY(check_vectors(what, {ln_weight, ln_bias, shift, scale}));
+  NormArgs p{};
+  p.x = static_cast<const uint8_t*>(x); p.x_sb = x_sb; p.x_ss = x_ss;
+  p.out = static_cast<uint8_t*>(y); p.out_sb = y_sb; p.out_ss = y_ss;
+  p.weight = ln_weight; p.bias = ln_bias; p.shift = shift; p.scale = scale;
+  p.mean = mean; p.rstd = rstd; p.S = S; p.eps = eps;
+  return forward<true>(p, dtype, B, D, static_cast<cudaStream_t>(stream));
+}
+
+int dax_layernorm_modulate_backward(const void* dy, const void* x, int dtype, int64_t B, int64_t S, int64_t D, int64_t dy_sb,
+                                    int64_t dy_ss, int64_t x_sb, int64_t x_ss, const float* mean, const float* rstd,
+                                    const float* ln_weight, const float* ln_bias, const float* scale, void* dx, int64_t dx_sb,
+                                    int64_t dx_ss, float* dweight, float* dbias, float* dshift, float* dscale, void* workspace,
+                                    size_t workspace_bytes, void* stream) {
+  using namespace dax;
+  const char* what = "layernorm_modulate_backward";
+  DAX_TRY(check_rows(what, dtype, B, S, D));
+  if (B > 0 && S > 0) {
+    DAX_TRY(check_tensor(what, "x", x, x_sb, x_ss, dtype));
+    DAX_TRY(check_tensor(what, "dy", dy, dy_sb, dy_ss, dtype));
+    DAX_TRY(check_tensor(what, "dx", dx, dx_sb, dx_ss, dtype));
+    DAX_REQUIRE(mean != nullptr && rstd != nullptr, DAX_ERR_INVALID, "%s: mean and rstd are needed", what);
+  }
+  DAX_REQUIRE(ln_bias == nullptr || ln_weight != nullptr, DAX_ERR_INVALID, "%s: bias needs weight", what);
+  DAX_TRY(check_vectors(what, {ln_weight, ln_bias, scale}));
+  NormArgs p{};
+  p.x = static_cast<const uint8_t*>(x); p.x_sb = x_sb; p.x_ss = x_ss;
+  p.dy = static_cast<const uint8_t*>(dy); p.dy_sb = dy_sb; p.dy_ss = dy_ss;
+  p.out = static_cast<uint8_t*>(dx); p.out_sb = dx_sb; p.out_ss = dx_ss;
+  p.weight = ln_weight; p.scale = scale;
+  p.mean = const_cast<float*>(mean); p.rstd = const_cast<float*>(rstd); p.S = S;
+  JoinArgs j{};
+  j.weight = ln_weight; j.bias = ln_bias; j.scale = scale;
+  j.dweight = dweight; j.dbias = dbias; j.dshift = dshift; j.dscale = dscale;
+  return backward<true>(what, p, j, dtype, B, D, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
+}
+
+int dax_rmsnorm_rope(const void* x, int dtype, int64_t B, int64_t S, int64_t D, int64_t x_sb, int64_t x_ss,
+                     const float* norm_weight, const float* rope_cos, const float* rope_sin, float eps, void* y, int64_t y_sb,
+                     int64_t y_ss, float* rstd, void* stream) {
+  using namespace dax;
+  const char* what = "rmsnorm_rope";
+  DAX_TRY(check_rows(what, dtype, B, S, D));
+  if (B == 0 || S == 0) return DAX_OK;
+  DAX_TRY(check_tensor(what, "x", x, x_sb, x_ss, dtype));
+  DAX_TRY(check_tensor(what, "y", y, y_sb, y_ss, dtype));
+  DAX_REQUIRE(rstd != nullptr, DAX_ERR_INVALID, "%s: rstd is needed", what);
+  DAX_REQUIRE((rope_cos == nullptr) == (rope_sin == nullptr), DAX_ERR_INVALID, "%s: rope_cos and rope_sin come together", what);
+  DAX_REQUIRE(rope_cos == nullptr || D % 128 == 0, DAX_ERR_INVALID, "%s: a rotation needs D=%lld to be whole heads of 128", what, (long long)D);
+  DAX_TRY(check_vectors(what, {norm_weight, rope_cos, rope_sin}));
+  NormArgs p{};
+  p.x = static_cast<const uint8_t*>(x); p.x_sb = x_sb; p.x_ss = x_ss;
+  p.out = static_cast<uint8_t*>(y); p.out_sb = y_sb; p.out_ss = y_ss;
+  p.weight = norm_weight; p.cos = rope_cos; p.sin = rope_sin;
+  p.rstd = rstd; p.S = S; p.eps = eps;
+  return forward<false>(p, dtype, B, D, static_cast<cudaStream_t>(stream));
+}
+
+int dax_rmsnorm_rope_backward(const void* dy, const void* x, int dtype, int64_t B, int64_t S, int64_t D, int64_t dy_sb,
+                              int64_t dy_ss, int64_t x_sb, int64_t x_ss, const float* rstd, const float* norm_weight,
+                              const float* rope_cos, const float* rope_sin, void* dx, int64_t dx_sb, int64_t dx_ss,
+                              float* dweight, void* workspace, size_t workspace_bytes, void* stream) {
+  using namespace dax;
+  const char* what = "rmsnorm_rope_backward";
+  DAX_TRY(check_rows(what, dtype, B, S, D));
+  if (B > 0 && S > 0) {
+    DAX_TRY(check_tensor(what, "x", x, x_sb, x_ss, dtype));
+    DAX_TRY(check_tensor(what, "dy", dy, dy_sb, dy_ss, dtype));
+    DAX_TRY(check_tensor(what, "dx", dx, dx_sb, dx_ss, dtype));
+    DAX_REQUIRE(rstd != nullptr, DAX_ERR_INVALID, "%s: rstd is needed", what);
+  }
+  DAX_REQUIRE((rope_cos == nullptr) == (rope_sin == nullptr), DAX_ERR_INVALID, "%s: rope_cos and rope_sin come together", what);
+  DAX_REQUIRE(rope_cos == nullptr || D % 128 == 0, DAX_ERR_INVALID, "%s: a rotation needs D=%lld to be whole heads of 128", what, (long long)D);
+  DAX_TRY(check_vectors(what, {norm_weight, rope_cos, rope_sin}));
+  NormArgs p{};
+  p.x = static_cast<const uint8_t*>(x); p.x_sb = x_sb; p.x_ss = x_ss;
+  p.dy = static_cast<const uint8_t*>(dy); p.dy_sb = dy_sb; p.dy_ss = dy_ss;
+  p.out = static_cast<uint8_t*>(dx); p.out_sb = dx_sb; p.out_ss = dx_ss;
+  p.weight = norm_weight; p.cos = rope_cos; p.sin = rope_sin;
+  p.rstd = const_cast<float*>(rstd); p.S = S;
+  JoinArgs j{};
+  j.weight = norm_weight;
+  j.dweight = dweight;
+  return backward<false>(what, p, j, dtype, B, D, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
+}
+
+}  // extern "C"

@@ -28,7 +28,8 @@ class _Trace:
     """Optional launch accounting: number of library kernels launched and, when timing is on, CUDA
     events around each wrapper on the stream it launches on (used by the benchmark's roofline leg)."""
 
-    KERNELS_PER_CALL = {"layernorm_modulate_quant": 1, "linear_dynamic": 2, "quant_rowwise": 1, "gemm_dequant": 1, "rmsnorm_rope_pack": 1, "attn_prepare": 5, "attn_forward": 1}
+    KERNELS_PER_CALL = {"layernorm_modulate_quant": 1, "linear_dynamic": 2, "quant_rowwise": 1, "gemm_dequant": 1, "rmsnorm_rope_pack": 1, "attn_prepare": 5, "attn_forward": 1,
+                        "layernorm_modulate": 1, "layernorm_modulate_backward": 2, "rmsnorm_rope": 1, "rmsnorm_rope_backward": 2}
 
     def __init__(self):
         self.launches = 0
@@ -403,3 +404,171 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mode: str = "bf
     if out is None:
         out = torch.empty((B, Sq, heads, d), dtype=q.dtype, device=q.device).transpose(1, 2)
     return attn_forward(plan, out)
+
+
+# ---- training: operators with a gradient ---------------------------------------------------------------------------------
+# The backward passes recompute what they need from the inputs and the row statistics that the forward passes return.
+# Workspaces come from torch for every call (nothing is shared between calls, streams or captured graphs).
+def _on_one_device(what: str, *ts) -> torch.device:
+    """The device all tensors live on (the call goes to that device's current stream)."""
+    _need_cuda(*ts)
+    devs = {t.device for t in ts if t is not None}
+    if len(devs) != 1:
+        raise ValueError(f"{what}: tensors are on different devices: {sorted(map(str, devs))}")
+    return devs.pop()
+
+
+def _rows3(t: torch.Tensor) -> torch.Tensor:
+    """``[B, S, D]`` or ``[S, D]`` as ``[B, S, D]`` that the row kernels can read: channels contiguous, everything else in
+    whole 16 bytes.  A tensor that is not laid out like that is copied."""
+    t = t if t.dim() == 3 else t.unsqueeze(0)
+    e = t.element_size()
+    if t.stride(2) != 1 or t.data_ptr() % 16 or (t.shape[0] > 1 and t.stride(0) * e % 16) or (t.shape[1] > 1 and t.stride(1) * e % 16):
+        t = t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
+def _row_strides(t: torch.Tensor) -> Tuple[int, int]:
+    """Sample and token stride; those of a dimension of one are never used and torch may report anything for them."""
+    B, S, D = t.shape
+    return t.stride(0) if B > 1 else 0, t.stride(1) if S > 1 else 0
+
+
+def _vector(what: str, name: str, v: Optional[torch.Tensor], *shape: int) -> None:
+    if v is not None and (v.dtype != torch.float32 or tuple(v.shape) != shape or not v.is_contiguous()):
+        raise ValueError(f"{what}: {name} must be a contiguous fp32 {list(shape)} tensor, got {v.dtype} {list(v.shape)}")
+
+
+def _row_input(what: str, x: torch.Tensor) -> Tuple[int, int, int]:
+    if x.dim() not in (2, 3):
+        raise ValueError(f"{what}: x must be [B, S, D] or [S, D], got {list(x.shape)}")
+    if x.dtype not in (torch.bfloat16, torch.float16, torch.float32):
+        raise NotImplementedError(f"{what}: x must be bf16, fp16 or fp32, got {x.dtype}")
+    return (1, *x.shape) if x.dim() == 2 else tuple(x.shape)
+
+
+def _modulation(what: str, name: str, v: Optional[torch.Tensor], x: torch.Tensor) -> None:
+    _vector(what, name, v, *((x.shape[0], x.shape[2]) if x.dim() == 3 else (x.shape[1],)))
+
+
+def _grad_like(what: str, dy: torch.Tensor, x: torch.Tensor) -> None:
+    if dy.shape != x.shape or dy.dtype != x.dtype:
+        raise ValueError(f"{what}: dy must be {list(x.shape)} of {x.dtype}, got {list(dy.shape)} of {dy.dtype}")
+
+
+def layernorm_modulate(x: torch.Tensor, *, eps: float = 1e-6, ln_weight: Optional[torch.Tensor] = None,
+                       ln_bias: Optional[torch.Tensor] = None, shift: Optional[torch.Tensor] = None,
+                       scale: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """``y = (n [* ln_weight + ln_bias]) [* (1 + scale) + shift]`` with ``n`` the LayerNorm of every token row of ``x [B, S, D]``
+    (bf16, fp16 or fp32); ``ln_weight, ln_bias [D]`` and ``shift, scale [B, D]`` (one row for each sample) fp32.  ``x [S, D]``
+    is one sample with ``shift, scale [D]``.  Returns ``(y, mean, rstd)``; the statistics (fp32, one for each row) are what
+    ``layernorm_modulate_backward`` needs.  The inference step, which quantises ``y``, is ``layernorm_modulate_quant``."""
+    what = "layernorm_modulate"
+    B, S, D = _row_input(what, x)
+    _vector(what, "ln_weight", ln_weight, D)
+    _vector(what, "ln_bias", ln_bias, D)
+    _modulation(what, "shift", shift, x)
+    _modulation(what, "scale", scale, x)
+    dev = _on_one_device(what, x, ln_weight, ln_bias, shift, scale)
+    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    mean, rstd = torch.empty((2, *x.shape[:-1]), dtype=torch.float32, device=dev).unbind(0)
+    x3 = _rows3(x)
+    with torch.cuda.device(dev):
+        tok = TRACE.begin(what)
+        check(load().dax_layernorm_modulate(x3.data_ptr(), _dt(x.dtype), B, S, D, *_row_strides(x3), _ptr(ln_weight),
+                                            _ptr(ln_bias), _ptr(shift), _ptr(scale), float(eps), y.data_ptr(), S * D, D,
+                                            mean.data_ptr(), rstd.data_ptr(), _stream()))
+        TRACE.end(tok, (B, S, D))
+    return y, mean, rstd
+
+
+def layernorm_modulate_backward(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor, *,
+                                ln_weight: Optional[torch.Tensor] = None, ln_bias: Optional[torch.Tensor] = None,
+                                scale: Optional[torch.Tensor] = None, need_params: bool = True):
+    """Gradients of ``layernorm_modulate`` for the output gradient ``dy`` (shape and dtype of ``x``): ``(dx, dweight, dbias,
+    dshift, dscale)``.  The parameter gradients are fp32 sums over the rows, in a fixed order (equal inputs give equal
+    bits); those of vectors that were not given, and all of them with ``need_params=False``, are None."""
+    what = "layernorm_modulate_backward"
+    B, S, D = _row_input(what, x)
+    _grad_like(what, dy, x)
+    _vector(what, "mean", mean, *x.shape[:-1])
+    _vector(what, "rstd", rstd, *x.shape[:-1])
+    _vector(what, "ln_weight", ln_weight, D)
+    _vector(what, "ln_bias", ln_bias, D)
+    _modulation(what, "scale", scale, x)
+    dev = _on_one_device(what, dy, x, mean, rstd, ln_weight, ln_bias, scale)
+    dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    dweight = torch.empty_like(ln_weight) if need_params and ln_weight is not None else None
+    dbias = torch.empty_like(ln_bias) if need_params and ln_bias is not None else None
+    dshift, dscale = torch.empty((2, *scale.shape), dtype=torch.float32, device=dev).unbind(0) if need_params and scale is not None else (None, None)
+    x3, dy3 = _rows3(x), _rows3(dy)
+    with torch.cuda.device(dev):
+        lib, dt = load(), _dt(x.dtype)
+        n = lib.dax_norm_backward_workspace_bytes(B, S, D, dt) if dweight is not None or dscale is not None else 0
+        ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
+        tok = TRACE.begin(what)
+        check(lib.dax_layernorm_modulate_backward(dy3.data_ptr(), x3.data_ptr(), dt, B, S, D, *_row_strides(dy3), *_row_strides(x3),
+                                                  mean.data_ptr(), rstd.data_ptr(), _ptr(ln_weight), _ptr(ln_bias), _ptr(scale),
+                                                  dx.data_ptr(), S * D, D, _ptr(dweight), _ptr(dbias), _ptr(dshift), _ptr(dscale),
+                                                  _ptr(ws), n, _stream()))
+        TRACE.end(tok, (B, S, D))
+    return dx, dweight, dbias, dshift, dscale
+
+
+def _rope_check(what: str, x: torch.Tensor, S: int, D: int, cos: Optional[torch.Tensor], sin: Optional[torch.Tensor]) -> None:
+    if (cos is None) != (sin is None):
+        raise ValueError(f"{what}: rope_cos and rope_sin come together")
+    for name, t in (("rope_cos", cos), ("rope_sin", sin)):
+        if t is not None and (t.dtype != torch.float32 or t.dim() != 2 or t.shape[0] < S or t.shape[1] != 64 or not t.is_contiguous()):
+            raise ValueError(f"{what}: {name} must be a contiguous fp32 [>= {S}, 64] table, got {t.dtype} {list(t.shape)}")
+    if cos is not None and D % 128:
+        raise ValueError(f"{what}: a rotation needs D={D} to be whole heads of 128 channels")
+
+
+def rmsnorm_rope(x: torch.Tensor, norm_weight: Optional[torch.Tensor] = None, *, eps: float = 1e-6,
+                 rope_cos: Optional[torch.Tensor] = None, rope_sin: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """RMSNorm over the whole row of ``x [B, S, D]`` (or ``[S, D]``; bf16, fp16 or fp32), times ``norm_weight [D]`` (fp32), then
+    the rotation of every head's channel pairs by the angles of row ``s`` of the tables (fp32 ``[>= S, 64]``, the same for
+    every sample).  Returns ``(y, rstd)``; ``rstd`` is what ``rmsnorm_rope_backward`` needs.  The inference step, which writes
+    the exchange layout, is ``rmsnorm_rope_pack``."""
+    what = "rmsnorm_rope"
+    B, S, D = _row_input(what, x)
+    _vector(what, "norm_weight", norm_weight, D)
+    _rope_check(what, x, S, D, rope_cos, rope_sin)
+    dev = _on_one_device(what, x, norm_weight, rope_cos, rope_sin)
+    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    rstd = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev)
+    x3 = _rows3(x)
+    with torch.cuda.device(dev):
+        tok = TRACE.begin(what)
+        check(load().dax_rmsnorm_rope(x3.data_ptr(), _dt(x.dtype), B, S, D, *_row_strides(x3), _ptr(norm_weight), _ptr(rope_cos),
+                                      _ptr(rope_sin), float(eps), y.data_ptr(), S * D, D, rstd.data_ptr(), _stream()))
+        TRACE.end(tok, (B, S, D))
+    return y, rstd
+
+
+def rmsnorm_rope_backward(dy: torch.Tensor, x: torch.Tensor, rstd: torch.Tensor, norm_weight: Optional[torch.Tensor] = None, *,
+                          rope_cos: Optional[torch.Tensor] = None, rope_sin: Optional[torch.Tensor] = None,
+                          need_params: bool = True) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """Gradients of ``rmsnorm_rope``: ``(dx, dweight)``, ``dweight`` (fp32, summed in a fixed order) None without a weight
+    or with ``need_params=False``."""
+    what = "rmsnorm_rope_backward"
+    B, S, D = _row_input(what, x)
+    _grad_like(what, dy, x)
+    _vector(what, "rstd", rstd, *x.shape[:-1])
+    _vector(what, "norm_weight", norm_weight, D)
+    _rope_check(what, x, S, D, rope_cos, rope_sin)
+    dev = _on_one_device(what, dy, x, rstd, norm_weight, rope_cos, rope_sin)
+    dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    dweight = torch.empty_like(norm_weight) if need_params and norm_weight is not None else None
+    x3, dy3 = _rows3(x), _rows3(dy)
+    with torch.cuda.device(dev):
+        lib, dt = load(), _dt(x.dtype)
+        n = lib.dax_norm_backward_workspace_bytes(B, S, D, dt) if dweight is not None else 0
+        ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
+        tok = TRACE.begin(what)
+        check(lib.dax_rmsnorm_rope_backward(dy3.data_ptr(), x3.data_ptr(), dt, B, S, D, *_row_strides(dy3), *_row_strides(x3),
+                                            rstd.data_ptr(), _ptr(norm_weight), _ptr(rope_cos), _ptr(rope_sin), dx.data_ptr(), S * D, D,
+                                            _ptr(dweight), _ptr(ws), n, _stream()))
+        TRACE.end(tok, (B, S, D))
+    return dx, dweight

@@ -272,6 +272,49 @@ int dax_attn_forward_direct(const void* q, const void* k, const void* v, int dty
                             int64_t rows_per_dest, int64_t q_begin, int64_t q_end, int64_t n_ranges,
                             int64_t range_stride, void* stream);
 
+/* ---------------------------------------------------------------------------------------------
+ * Training: the row-wise steps of a DiT block with their gradients.  The reference has no counterpart (its path is
+ * inference); the forward formulas are those of the inference steps above (the block's norm / modulate,
+ * dax/adapters/wan/transformer_adapter.py:148-150, and norm_q / norm_k + rotary embedding,
+ * dax/adapters/wan/attn_adapter.py:82-85,164-173).
+ *
+ * x, y, dy, dx are [B, S, D] of one dtype (BF16 / F16 / F32), the channels contiguous; *_sb / *_ss are the strides of a
+ * sample and of a token in elements, in bytes multiples of 16.  D is a multiple of 8, at most 8192.  All vectors, the
+ * statistics and the parameter gradients are contiguous fp32, 16-byte aligned.  n is the normalised row.
+ *
+ * dax_layernorm_modulate:   y = (n w + c) (1 + scale_b) + shift_b, n = (x - mean) rstd; ln_weight, ln_bias [D] or NULL (bias
+ *   needs weight); shift, scale [B, D], both or neither; mean, rstd [B, S] are written.
+ * dax_layernorm_modulate_backward:   dx always; dweight, dbias [D], dshift, dscale [B, D]: those that are not NULL.  ln_bias
+ *   is read for dscale only.
+ * dax_rmsnorm_rope:   y = R_s (n w), n = x rstd, rstd over the whole row; norm_weight [D] or NULL; R_s rotates the channel
+ *   pairs (2i, 2i+1) of every head of 128 by the angles of row s of rope_cos / rope_sin [S, 64] (NULL: no rotation).  One
+ *   rounding, at the end (dax_rmsnorm_rope_pack also rounds before it rotates).
+ * dax_rmsnorm_rope_backward:   dx, and dweight [D] unless NULL.
+ *
+ * The parameter gradients are sums over all rows in a fixed order: equal inputs give equal bits.  `workspace` (16-byte
+ * aligned, dax_norm_backward_workspace_bytes) holds partial sums; it may be NULL when no parameter gradient is wanted.
+ * ------------------------------------------------------------------------------------------- */
+size_t dax_norm_backward_workspace_bytes(int64_t B, int64_t S, int64_t D, int dtype);
+
+int dax_layernorm_modulate(const void* x, int dtype, int64_t B, int64_t S, int64_t D, int64_t x_sb, int64_t x_ss,
+                           const float* ln_weight, const float* ln_bias, const float* shift, const float* scale, float eps,
+                           void* y, int64_t y_sb, int64_t y_ss, float* mean, float* rstd, void* stream);
+
+int dax_layernorm_modulate_backward(const void* dy, const void* x, int dtype, int64_t B, int64_t S, int64_t D, int64_t dy_sb,
+                                    int64_t dy_ss, int64_t x_sb, int64_t x_ss, const float* mean, const float* rstd,
+                                    const float* ln_weight, const float* ln_bias, const float* scale, void* dx, int64_t dx_sb,
+                                    int64_t dx_ss, float* dweight, float* dbias, float* dshift, float* dscale, void* workspace,
+                                    size_t workspace_bytes, void* stream);
+
+int dax_rmsnorm_rope(const void* x, int dtype, int64_t B, int64_t S, int64_t D, int64_t x_sb, int64_t x_ss,
+                     const float* norm_weight, const float* rope_cos, const float* rope_sin, float eps, void* y, int64_t y_sb,
+                     int64_t y_ss, float* rstd, void* stream);
+
+int dax_rmsnorm_rope_backward(const void* dy, const void* x, int dtype, int64_t B, int64_t S, int64_t D, int64_t dy_sb,
+                              int64_t dy_ss, int64_t x_sb, int64_t x_ss, const float* rstd, const float* norm_weight,
+                              const float* rope_cos, const float* rope_sin, void* dx, int64_t dx_sb, int64_t dx_ss,
+                              float* dweight, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
