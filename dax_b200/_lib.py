@@ -64,6 +64,10 @@ SIGNATURES = {
     "dax_layernorm_modulate_backward": (c_int, [c_void_p, c_void_p, c_int, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
     "dax_rmsnorm_rope": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_float, c_void_p, c_int64, c_int64, c_void_p, c_void_p]),
     "dax_rmsnorm_rope_backward": (c_int, [c_void_p, c_void_p, c_int, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "dax_attn_lse_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int64, c_int64]),
+    "dax_attn_forward_lse": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int64, c_int64, c_int64, c_int64, I64x3, I64x3, I64x3, c_float, c_void_p, c_void_p, c_void_p, I64x3, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "dax_attn_backward_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int64, c_int64]),
+    "dax_attn_backward": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int64, c_int64, c_int64, c_int64, I64x3, I64x3, I64x3, I64x3, I64x3, c_float, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, I64x3, I64x3, I64x3, c_void_p, c_size_t, c_void_p]),
 }
 
 _LIB = None

@@ -46,27 +46,6 @@ constexpr int SMEM_TOTAL = OFF_BAR + 256 + 1024 /*alignment slack*/;
 __device__ __forceinline__ void reg_alloc_216() { asm volatile("setmaxnreg.inc.sync.aligned.u32 216;"); }
 __device__ __forceinline__ void reg_dealloc_72() { asm volatile("setmaxnreg.dec.sync.aligned.u32 72;"); }
 
-// D[tmem] (+)= A[tmem] * B[smem]^T, kind::f16, issued by ONE thread.  A: 128 lanes x (K/2) columns, two 16-bit
-// elements of consecutive K per 32-bit cell.
-__device__ __forceinline__ void umma_ts_f16(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc,
-                                            uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(tmem_d),
-      "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
-      : "memory");
-}
-
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ float fmax3(float a, float b, float c) {
-  float d;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-  return d;
-}
 // Two fp32 values -> bf16x2 by keeping the upper halves (one byte-permute for two elements; the rounding
 // conversions run on the unit the exponentials already saturate).  Truncation lowers every P by 2^-9 on average;
 // the epilogue multiplies O by (1 + 2^-9) to centre it.

@@ -29,7 +29,8 @@ class _Trace:
     events around each wrapper on the stream it launches on (used by the benchmark's roofline leg)."""
 
     KERNELS_PER_CALL = {"layernorm_modulate_quant": 1, "linear_dynamic": 2, "quant_rowwise": 1, "gemm_dequant": 1, "rmsnorm_rope_pack": 1, "attn_prepare": 5, "attn_forward": 1,
-                        "layernorm_modulate": 1, "layernorm_modulate_backward": 2, "rmsnorm_rope": 1, "rmsnorm_rope_backward": 2}
+                        "layernorm_modulate": 1, "layernorm_modulate_backward": 2, "rmsnorm_rope": 1, "rmsnorm_rope_backward": 2,
+                        "attention_lse": 1, "attention_backward": 2}
 
     def __init__(self):
         self.launches = 0
@@ -572,3 +573,91 @@ def rmsnorm_rope_backward(dy: torch.Tensor, x: torch.Tensor, rstd: torch.Tensor,
                                             _ptr(dweight), _ptr(ws), n, _stream()))
         TRACE.end(tok, (B, S, D))
     return dx, dweight
+
+
+def _heads_view(t: torch.Tensor) -> Tuple[torch.Tensor, I64x3]:
+    """``t [B, heads, S, 128]`` and its strides for the kernels; a tensor they cannot address (channels not contiguous,
+    broadcast dimensions, misaligned) is copied into token-major memory."""
+    if t.stride(3) != 1 or t.data_ptr() % 16 or any(n > 1 and (st <= 0 or st % 8) for n, st in zip(t.shape, t.stride()[:3])):
+        t = _token_major(t).copy_(t)
+    return t, I64x3(*(st if n > 1 else 128 for n, st in zip(t.shape, t.stride()[:3])))  # a dimension of one: any valid stride
+
+
+def _attention_inputs(what: str, q, k, v, q_lens, k_lens, sm_scale, *more) -> Tuple[int, int, int, int, float, torch.device]:
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        if t.dim() != 4 or t.shape[3] != 128:
+            raise ValueError(f"{what}: {name} must be [B, heads, S, 128], got {list(t.shape)}")
+    if k.shape != v.shape or k.shape[:2] != q.shape[:2]:
+        raise ValueError(f"{what}: q {list(q.shape)}, k {list(k.shape)} and v {list(v.shape)} do not belong together")
+    if q.dtype not in (torch.bfloat16, torch.float16) or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise NotImplementedError(f"{what}: q, k and v must all be bf16 or all fp16, got {q.dtype}, {k.dtype}, {v.dtype}")
+    B, heads, Sq, _ = q.shape
+    for name, t in (("q_lens", q_lens), ("k_lens", k_lens)):
+        if t is not None and (t.dtype != torch.int32 or tuple(t.shape) != (B,) or not t.is_contiguous()):
+            raise ValueError(f"{what}: {name} must be a contiguous int32 [{B}] tensor, got {t.dtype} {list(t.shape)}")
+    if sm_scale is None:
+        sm_scale = 1.0 / math.sqrt(128)
+    if not 0.0 < sm_scale < math.inf:
+        raise ValueError(f"{what}: sm_scale must be positive and finite, got {sm_scale}")
+    return B, heads, Sq, k.shape[2], float(sm_scale), _on_one_device(what, q, k, v, q_lens, k_lens, *more)
+
+
+def _token_major(t: torch.Tensor) -> torch.Tensor:
+    B, heads, S, d = t.shape
+    return torch.empty((B, S, heads, d), dtype=t.dtype, device=t.device).transpose(1, 2)
+
+
+def attention_lse(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, q_lens: Optional[torch.Tensor] = None,
+                  k_lens: Optional[torch.Tensor] = None, sm_scale: Optional[float] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Non-causal attention over ``[B, heads, S, 128]`` (bf16 or fp16, any strides) that keeps what its gradient needs:
+    ``(out, lse)``, ``out`` token-major like the result of ``attention``, ``lse [B, heads, Sq]`` fp32 (natural logarithm).
+    ``q_lens`` / ``k_lens`` (int32 ``[B]`` on the device): the tokens of each sample of a padded batch that exist; the
+    others may hold anything.  Queries that do not exist or see no key get ``out = 0``, ``lse = -inf``."""
+    what = "attention_lse"
+    B, heads, Sq, Sk, sm_scale, dev = _attention_inputs(what, q, k, v, q_lens, k_lens, sm_scale)
+    out = _token_major(q)
+    lse = torch.empty((B, heads, Sq), dtype=torch.float32, device=dev)
+    if lse.numel() == 0:
+        return out, lse
+    if Sk == 0:
+        return out.zero_(), lse.fill_(-math.inf)
+    (q, qs), (k, ks), (v, vs) = _heads_view(q), _heads_view(k), _heads_view(v)
+    with torch.cuda.device(dev):
+        lib = load()
+        n = lib.dax_attn_lse_workspace_bytes(B, heads, Sq, Sk)
+        ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
+        tok = TRACE.begin(what)
+        check(lib.dax_attn_forward_lse(q.data_ptr(), k.data_ptr(), v.data_ptr(), _dt(q.dtype), B, heads, Sq, Sk, qs, ks, vs, sm_scale,
+                                       _ptr(q_lens), _ptr(k_lens), out.data_ptr(), _heads_view(out)[1], lse.data_ptr(),
+                                       _ptr(ws), n, _stream()))
+        TRACE.end(tok, (B, heads, Sq, Sk))
+    return out, lse
+
+
+def attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor, lse: torch.Tensor, *,
+                       q_lens: Optional[torch.Tensor] = None, k_lens: Optional[torch.Tensor] = None,
+                       sm_scale: Optional[float] = None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Gradients ``(dq, dk, dv)`` (token-major) of ``attention_lse`` for the output gradient ``dout``, from the same inputs
+    and what it returned.  The probabilities are recomputed; sums are fp32 in a fixed order, so equal inputs give equal
+    bits.  Tokens that do not exist get zero gradients and contribute to none."""
+    what = "attention_backward"
+    B, heads, Sq, Sk, sm_scale, dev = _attention_inputs(what, q, k, v, q_lens, k_lens, sm_scale, dout, out, lse)
+    for name, t in (("dout", dout), ("out", out)):
+        if t.shape != q.shape or t.dtype != q.dtype:
+            raise ValueError(f"{what}: {name} must be {list(q.shape)} of {q.dtype}, got {list(t.shape)} of {t.dtype}")
+    _vector(what, "lse", lse, B, heads, Sq)
+    dq, dk, dv = _token_major(q), _token_major(k), _token_major(v)
+    if lse.numel() == 0 or Sk == 0:
+        return dq.zero_(), dk.zero_(), dv.zero_()
+    (dout, dos), (q, qs), (k, ks), (v, vs), (out, os_) = map(_heads_view, (dout, q, k, v, out))
+    with torch.cuda.device(dev):
+        lib = load()
+        n = lib.dax_attn_backward_workspace_bytes(B, heads, Sq, Sk)
+        ws = torch.empty(n, dtype=torch.uint8, device=dev)
+        tok = TRACE.begin(what)
+        check(lib.dax_attn_backward(dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), _dt(q.dtype),
+                                    B, heads, Sq, Sk, dos, qs, ks, vs, os_, sm_scale, _ptr(q_lens), _ptr(k_lens), dq.data_ptr(),
+                                    dk.data_ptr(), dv.data_ptr(), _heads_view(dq)[1], _heads_view(dk)[1],
+                                    _heads_view(dv)[1], ws.data_ptr(), n, _stream()))
+        TRACE.end(tok, (B, heads, Sq, Sk))
+    return dq, dk, dv

@@ -315,6 +315,36 @@ int dax_rmsnorm_rope_backward(const void* dy, const void* x, int dtype, int64_t 
                               const float* rope_cos, const float* rope_sin, void* dx, int64_t dx_sb, int64_t dx_ss,
                               float* dweight, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---------------------------------------------------------------------------------------------
+ * Training: attention with a gradient (non-causal, head_dim 128, BF16 / F16).  The reference has no counterpart (its
+ * attention dispatch, dax/adapters/wan/attn_adapter.py:198-229, is inference only).
+ *
+ * q, o, dout, dq [B, heads, Sq, 128], k, v, dk, dv [B, heads, Sk, 128]: element strides (sample, head, token), multiples of
+ * 8, channels contiguous, 16-byte aligned; inputs may not be broadcast (stride 0 over more than one element).
+ * sm_scale > 0.  lse [B, heads, Sq] fp32: natural logarithm of the sum of exp(sm_scale q.k).
+ * q_lens, k_lens: int32 [B] on the device or NULL (all tokens): tokens from a sample's length on do not exist, whatever they
+ * hold (values below 0 and above S count as 0 and S).  Outputs of queries that do not exist or see no key: o = 0,
+ * lse = -inf, dq = 0; of keys that do not exist: dk = dv = 0.
+ * dax_attn_backward needs o and lse as dax_attn_forward_lse wrote them for the same inputs.  Results do not depend on
+ * timing (no atomics): equal inputs give equal bits.
+ * Workspaces (16-byte aligned): dax_attn_lse_workspace_bytes may be 0 (then NULL will do).  With few query or key rows the
+ * other axis is split over several CTAs, whose fp32 parts it holds; the split depends on the sizes alone.
+ * ------------------------------------------------------------------------------------------- */
+size_t dax_attn_lse_workspace_bytes(int64_t B, int64_t heads, int64_t Sq, int64_t Sk);
+
+int dax_attn_forward_lse(const void* q, const void* k, const void* v, int dtype, int64_t B, int64_t heads, int64_t Sq, int64_t Sk,
+                         int64_t q_strides[3], int64_t k_strides[3], int64_t v_strides[3], float sm_scale, const int32_t* q_lens,
+                         const int32_t* k_lens, void* o, int64_t o_strides[3], float* lse, void* workspace, size_t workspace_bytes,
+                         void* stream);
+
+size_t dax_attn_backward_workspace_bytes(int64_t B, int64_t heads, int64_t Sq, int64_t Sk);
+
+int dax_attn_backward(const void* dout, const void* q, const void* k, const void* v, const void* o, const float* lse, int dtype,
+                      int64_t B, int64_t heads, int64_t Sq, int64_t Sk, int64_t do_strides[3], int64_t q_strides[3],
+                      int64_t k_strides[3], int64_t v_strides[3], int64_t o_strides[3], float sm_scale, const int32_t* q_lens,
+                      const int32_t* k_lens, void* dq, void* dk, void* dv, int64_t dq_strides[3], int64_t dk_strides[3],
+                      int64_t dv_strides[3], void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
