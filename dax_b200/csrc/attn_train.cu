@@ -20,7 +20,7 @@
 #include <algorithm>
 #include <cmath>
 
-#include "common.cuh"
+#include "quant_common.cuh"
 #include "sm100_ptx.cuh"
 
 namespace dax {
@@ -28,8 +28,11 @@ namespace {
 
 constexpr int BOX_BYTES = 128 * 128;       // one [128 rows x 64 channels] box
 constexpr int TILE_BYTES = 2 * BOX_BYTES;  // a [128 x 128] tile of 16-bit elements
-constexpr int THREADS = 384;
-constexpr int PRODUCER_WARP = 8, ISSUER_WARP0 = 9, ISSUER_WARP1 = 10, TMEM_WARP = 11;
+// Warps: N row warps (all arithmetic on scores), then a TMA producer, two issuers of products, the owner of tensor memory.
+constexpr int ROW_WARPS_F = 8, ROW_WARPS_B = 16;
+template <int N> struct Warps {
+  static constexpr int threads = (N + 4) * 32, producer = N, issuer0 = N + 1, issuer1 = N + 2, tmem = N + 3;
+};
 constexpr float TAU = 8.f;                 // forward: lazy rescale, p <= 2^8
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr int kMaxSplits = 16;
@@ -37,39 +40,61 @@ constexpr int kMaxSplits = 16;
 struct Rows { const void* p; int64_t sb, sh, st; };  // a [B, heads, S, 128] view: element strides of sample, head, token
 
 struct TrainParams {
-  Rows q, k, v, o, dout, dq, dk, dv;
+  Rows o, dq, dk, dv;
   float* lse;          // [BH, Sq]
   const int* q_lens;   // [B] or null
   const int* k_lens;
-  float* row_stats;    // backward: [BH, Sq_pad, ...] as [2][BH * Sq_pad]: lse * log2(e) (+inf: no such row), then D
+  float* row_stats;    // backward: [2][BH * Sq_pad]: -lse * log2(e) (-inf: no such row), then -D
   float* part;         // split runs: fp32 partial sums
-  float* part_lse;     // split forward runs: [splits, BH, Sq] row maxima-free log2 sums
+  float* part_lse;     // split forward runs: [splits, BH, Sq] log2 of each part's sum of exponentials
   int* status;
   int B, heads, Sq, Sk, Sq_pad, splits;
   float sm_scale;
 };
 
-__device__ __forceinline__ void reg_alloc_216() { asm volatile("setmaxnreg.inc.sync.aligned.u32 216;"); }
-__device__ __forceinline__ void reg_dealloc_72() { asm volatile("setmaxnreg.dec.sync.aligned.u32 72;"); }
+// Register split: row warps and the others, together what the block was launched with (12 warps x 168, 20 warps x 96)
+template <int N> __device__ __forceinline__ void row_warp_registers() {
+  if constexpr (N == ROW_WARPS_F) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+  else asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
+}
+template <int N> __device__ __forceinline__ void other_warp_registers() {
+  if constexpr (N == ROW_WARPS_F) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+  else asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+}
 
-template <bool BF16>
-__device__ __forceinline__ uint32_t pack_rn(float lo, float hi) {
+// ---- rounding to the operands' type ------------------------------------------------------------------------------------
+// The conversion instructions run on the unit of the exponentials, which the kernels need for those.  bf16 is the upper
+// half of fp32, so rounding can be done on the other pipes and two results taken together with one byte permute.
+__device__ __forceinline__ uint32_t upper_halves(uint32_t a, uint32_t b) {
   uint32_t r;
-  if constexpr (BF16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  asm("prmt.b32 %0, %1, %2, 0x7632;" : "=r"(r) : "r"(a), "r"(b));
   return r;
 }
+// Probabilities, never negative: add half a step of the kept part, in the integer pipe (a tie goes up).  The minimum, part
+// of the same instruction, keeps NaN (0x7fffffff) a NaN.
 template <bool BF16>
-__device__ __forceinline__ void unpack(uint32_t w, float& lo, float& hi) {
+__device__ __forceinline__ uint32_t pack_prob(float lo, float hi) {
+  if constexpr (BF16)
+    return upper_halves(__viaddmin_u32(__float_as_uint(lo), 0x8000u, 0x7fffffffu), __viaddmin_u32(__float_as_uint(hi), 0x8000u, 0x7fffffffu));
+  else return pack2_rn<false>(lo, hi);
+}
+// Signed values, as a pair: with g = RN(65537 x), g + RN(x - g) is x rounded to its leading 8 bits (Veltkamp's splitting),
+// three fused-multiply-add-pipe instructions for two elements.  `hi` returns the rounded pair.
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack_signed(uint64_t x, uint64_t& hi) {
   if constexpr (BF16) {
-    lo = __uint_as_float(w << 16);
-    hi = __uint_as_float(w & 0xffff0000u);
+    const uint64_t g = f2_mul(x, f2_splat(65537.f));
+    hi = f2_add(g, f2_fma(g, f2_splat(-1.f), x));
+    float a, b;
+    f2_unpack(hi, a, b);
+    return upper_halves(__float_as_uint(a), __float_as_uint(b));
   } else {
-    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
-    lo = f.x;
-    hi = f.y;
+    const uint32_t w = f2_to16_rn<false>(x);
+    hi = f2_from16<false>(w);
+    return w;
   }
 }
+__device__ __forceinline__ uint64_t f2_bits(uint32_t lo, uint32_t hi) { return f2_pack(__uint_as_float(lo), __uint_as_float(hi)); }
 __device__ __forceinline__ int valid_len(const int* lens, int b, int S) { return lens != nullptr ? min(max(lens[b], 0), S) : S; }
 
 __device__ __forceinline__ const uint16_t* row_ptr(const Rows& t, int b, int h, int64_t s) {
@@ -77,19 +102,54 @@ __device__ __forceinline__ const uint16_t* row_ptr(const Rows& t, int b, int h, 
 }
 __device__ __forceinline__ uint16_t* out_ptr(const Rows& t, int b, int h, int64_t s) { return const_cast<uint16_t*>(row_ptr(t, b, h, s)); }
 
-// 32 fp32 values -> 64 bytes of 16-bit results
-template <bool BF16>
-__device__ __forceinline__ void store_row32(uint16_t* dst, const uint32_t (&v)[32], float mul) {
+// ---- results to memory ----------------------------------------------------------------------------------------------
+// A thread holds a row, memory wants whole lines: a warp's 32 rows x ROWB bytes (64 or 128) go through its own piece of shared
+// memory, 16-byte chunks permuted so that neither side has bank conflicts.
+template <int ROWB>
+__device__ __forceinline__ uint4* stage_at(uint8_t* st, int row, int chunk) {
+  const int swz = ROWB == 128 ? chunk ^ (row & 7) : chunk ^ ((row >> 1) & 3);
+  return reinterpret_cast<uint4*>(st + row * ROWB + swz * 16);
+}
+template <int ROWB>
+__device__ __forceinline__ void stage_flush(uint8_t* st, uint8_t* dst, int64_t row_bytes, int rows) {
+  constexpr int L = ROWB / 16;
+  const int lane = threadIdx.x & 31;
+  __syncwarp();
 #pragma unroll
-  for (int i = 0; i < 32; i += 8) {
+  for (int i = 0; i < L; ++i) {
+    const int row = (i * 32 + lane) / L, chunk = lane % L;
+    if (row < rows) *reinterpret_cast<uint4*>(dst + row * row_bytes + chunk * 16) = *stage_at<ROWB>(st, row, chunk);
+  }
+  __syncwarp();
+}
+// 32 columns of the warp's rows, times `mul`, rounded (64 bytes per row) ...
+template <bool BF16>
+__device__ __forceinline__ void store_cols32(uint8_t* st, const uint32_t (&v)[32], float mul, bool live, uint16_t* dst, int64_t row_elements, int rows) {
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
     uint32_t w[4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) w[k] = pack_rn<BF16>(__uint_as_float(v[i + 2 * k]) * mul, __uint_as_float(v[i + 2 * k + 1]) * mul);
-    *reinterpret_cast<uint4*>(dst + i) = make_uint4(w[0], w[1], w[2], w[3]);
+    for (int k = 0; k < 4; ++k) w[k] = pack2_rn<BF16>(__uint_as_float(v[8 * c + 2 * k]) * mul, __uint_as_float(v[8 * c + 2 * k + 1]) * mul);
+    *stage_at<64>(st, threadIdx.x & 31, c) = live ? make_uint4(w[0], w[1], w[2], w[3]) : make_uint4(0u, 0u, 0u, 0u);
   }
+  stage_flush<64>(st, reinterpret_cast<uint8_t*>(dst), row_elements * 2, rows);
 }
-__device__ __forceinline__ void store_zero(uint16_t* dst, int elements) {
-  for (int i = 0; i < elements; i += 8) *reinterpret_cast<uint4*>(dst + i) = make_uint4(0u, 0u, 0u, 0u);
+// ... or as fp32 parts of a split run (128 bytes per row, rows of 128 floats)
+__device__ __forceinline__ void store_part32(uint8_t* st, const uint32_t (&v)[32], float mul, bool live, float* dst, int rows) {
+#pragma unroll
+  for (int c = 0; c < 8; ++c) {
+    uint32_t w[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) w[k] = live ? __float_as_uint(__uint_as_float(v[4 * c + k]) * mul) : 0u;
+    *stage_at<128>(st, threadIdx.x & 31, c) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  stage_flush<128>(st, reinterpret_cast<uint8_t*>(dst), 512, rows);
+}
+// `rows` rows of `bytes` zeros, by the whole block
+__device__ __forceinline__ void zero_rows(void* dst, int64_t row_bytes, int rows, int bytes) {
+  const int chunks = bytes / 16;
+  for (int i = threadIdx.x; i < rows * chunks; i += blockDim.x)
+    *reinterpret_cast<uint4*>(static_cast<uint8_t*>(dst) + (i / chunks) * row_bytes + (i % chunks) * 16) = make_uint4(0u, 0u, 0u, 0u);
 }
 
 // ---- ring of tiles --------------------------------------------------------------------------------------------------
@@ -141,13 +201,12 @@ __device__ __forceinline__ void mma_ts_k(uint32_t d, uint32_t a_tmem, uint32_t b
     umma_ts_f16(d, a_tmem + 8 * i, b + adv, idesc, i != 0 ? 1u : 0u);
   }
 }
-// D += A[tmem] . B[smem] with the contraction over the tile's rows: B is MN-major, 16 rows per step.  The second four
-// steps take A from `a_hi` columns further.
-__device__ __forceinline__ void mma_ts_mn(uint32_t d, uint32_t a_tmem, uint32_t a_hi, uint32_t b_smem, uint32_t idesc, bool first) {
+// D += A[tmem] . B[smem] with the contraction over the tile's rows: B is MN-major, 16 rows per step
+__device__ __forceinline__ void mma_ts_mn(uint32_t d, uint32_t a_tmem, uint32_t b_smem, uint32_t idesc, bool first) {
   const uint64_t b = make_desc_mn_sw128(b_smem, BOX_BYTES);
 #pragma unroll
   for (int i = 0; i < 8; ++i)
-    umma_ts_f16(d, a_tmem + (i >= 4 ? a_hi : 0u) + 8 * (i & 3), b + static_cast<uint64_t>(i * ((16 * 128) >> 4)), idesc,
+    umma_ts_f16(d, a_tmem + 8 * i, b + static_cast<uint64_t>(i * ((16 * 128) >> 4)), idesc,
                 (!first || i != 0) ? 1u : 0u);
 }
 template <bool BF16>
@@ -155,9 +214,18 @@ __device__ __forceinline__ uint32_t idesc_k() { return make_idesc(1, BF16 ? 1 : 
 template <bool BF16>
 __device__ __forceinline__ uint32_t idesc_mn() { return idesc_k<BF16>() | (1u << 16); }  // B is MN-major
 
+// Half `c` of such a product whose A operand is in four groups of 32 columns, 16 of them used, each by one row warp for 32 of
+// the tile's rows: the groups' first (c = 0) or second 16 rows.
+__device__ __forceinline__ void mma_ts_mn_half(uint32_t d, uint32_t a_tmem, int c, uint32_t b_smem, uint32_t idesc, bool first) {
+  const uint64_t b = make_desc_mn_sw128(b_smem, BOX_BYTES);
+#pragma unroll
+  for (int g = 0; g < 4; ++g)
+    umma_ts_f16(d, a_tmem + 32 * g + 8 * c, b + static_cast<uint64_t>((2 * g + c) * ((16 * 128) >> 4)), idesc, (!first || g != 0) ? 1u : 0u);
+}
+
 // Set-up and tear-down shared by the kernels
-__device__ __forceinline__ uint32_t open_tmem(uint32_t* slot, int warp) {
-  if (warp == TMEM_WARP) {
+__device__ __forceinline__ uint32_t open_tmem(uint32_t* slot, bool owner) {
+  if (owner) {
     tmem_alloc(slot, 512);
     tmem_relinquish();
   }
@@ -166,10 +234,10 @@ __device__ __forceinline__ uint32_t open_tmem(uint32_t* slot, int warp) {
   tc_fence_after_sync();
   return *slot;
 }
-__device__ __forceinline__ void close_tmem(uint32_t base, int warp, volatile uint32_t* abort_flag, int* status) {
+__device__ __forceinline__ void close_tmem(uint32_t base, bool owner, volatile uint32_t* abort_flag, int* status) {
   tc_fence_before_sync();
   __syncthreads();
-  if (warp == TMEM_WARP) {
+  if (owner) {
     tc_fence_after_sync();
     tmem_dealloc(base, 512);
   }
@@ -177,23 +245,36 @@ __device__ __forceinline__ void close_tmem(uint32_t base, int warp, volatile uin
 }
 
 // ---- dq ----------------------------------------------------------------------------------------------------------------
-// One CTA = 128 query rows of one head.  q and do of these rows are the A operands of the first two products for every
-// tile of keys, so they live in TENSOR memory, as does ds: every product takes A from there and only k and v tiles pass
-// through shared memory.
-//   warps 0..7   one thread = one query row x 64 keys of the tile (warps 0-3: the first 64)
-//   warp  8      TMA producer: k_0, v_0, k_1, ... through the ring
-//   warp  9      issues s = q.k_j^T        warp 10  issues dp = do.v_j^T and dq += ds.k_j
-// Tensor memory: s [0,128)  dp [128,256), ds over the first half of each thread's own columns of it  dq [256,384)
-// q [384,448)  do [448,512).  s is free as soon as it is in registers, so s of the next tile is computed under ds of this
-// one, and dp of the next tile under its exponentials.
-constexpr int DQ_SLOTS = 6;
-constexpr int DQ_OFF_STAT = DQ_SLOTS * TILE_BYTES;
-constexpr int DQ_OFF_BAR = DQ_OFF_STAT + 1024;
+// One CTA = 128 query rows of one head, walking over the tiles of keys.
+//   warps 0..15  one thread = one query row x 32 keys of the tile (warp / 4: which 32).  Sixteen warps and not eight: the
+//                exponentials and the rest alternate, and four warps per scheduler hide each other's waits
+//   producer     q, and do and o in the ring's last two slots; then k_0, v_0, k_1, ... through the ring, at last k's first tile
+//   issuer 0     s = q.k_j^T and dp = do.v_j^T        issuer 1     dq += ds.k_j
+// Tensor memory: s [0,128)  dp [128,256)  dq [256,384)  do [384,448)  ds [448,512).  do and ds are A operands in tensor
+// memory, so of the three products only s reads both operands from shared memory, whose bandwidth would otherwise be the
+// bound.  s and dp are free as soon as they are in registers, and ds has columns of its own: the next tile's products
+// never wait for this tile's arithmetic.
+//
+// Keys often share an offset (the mean of trained keys is far from zero).  sum_j ds_ij is zero, so the offset has no part in
+// dq, but the roundings of ds have: their sum times the offset would be the largest error by far.  The kernel adds up the
+// rounded ds of each row, e_i, and subtracts e_i m for an m near the mean key (the first tile's), which is what rounding
+// left of it.
+constexpr int DQ_SLOTS = 5;
+constexpr int DQ_OFF_Q = DQ_SLOTS * TILE_BYTES;
+constexpr int DQ_OFF_D = DQ_OFF_Q + TILE_BYTES;     // [4][128] floats: parts of D
+constexpr int DQ_OFF_E = DQ_OFF_D + 4 * 512;        // [4][128] floats: parts of e
+constexpr int DQ_OFF_MEAN = DQ_OFF_E + 4 * 512;     // [16][128] floats: sums of keys, in the end m in the first row
+constexpr int DQ_OFF_BAR = DQ_OFF_MEAN + 16 * 512;
 constexpr int DQ_SMEM = DQ_OFF_BAR + 256 + 1024;
 
+__device__ __forceinline__ void row_warps_sync() { asm volatile("bar.sync 1, 512;" ::: "memory"); }  // warps 0..15
+
 template <bool BF16>
-__global__ void __launch_bounds__(THREADS, 1)
-attn_bwd_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const TrainParams p) {
+__global__ void __launch_bounds__(Warps<ROW_WARPS_B>::threads, 1)
+attn_bwd_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_do,
+                   const __grid_constant__ CUtensorMap map_o, const __grid_constant__ CUtensorMap map_k,
+                   const __grid_constant__ CUtensorMap map_v, const TrainParams p) {
+  using W = Warps<ROW_WARPS_B>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -202,69 +283,89 @@ attn_bwd_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
   const int n_all = q0 < q_len ? (k_len + 127) / 128 : 0;
   const int per = (n_all + p.splits - 1) / p.splits;
   const int j0 = split * per, n = max(0, min(n_all, j0 + per) - j0);
-  const int r = (warp & 3) * 32 + lane, half = (warp >> 2) & 1, q_row = q0 + r;
   // a split run leaves fp32 sums [split][BH][Sq][128] that are joined afterwards
-  float* part = p.part + ((static_cast<int64_t>(split) * p.B * p.heads + bh) * p.Sq + q_row) * 128 + half * 64;
-  const int64_t stat = static_cast<int64_t>(bh) * p.Sq_pad + q_row;
+  float* part = p.part + ((static_cast<int64_t>(split) * p.B * p.heads + bh) * p.Sq + q0) * 128;
+  float* stat = p.row_stats + static_cast<int64_t>(bh) * p.Sq_pad + q0;
   const int64_t stats = static_cast<int64_t>(p.B) * p.heads * p.Sq_pad;
+  const int rows_in = min(128, p.Sq - q0);  // rows of the CTA
 
   if (n == 0) {  // nothing to see: zeros
-    if (warp < 8) {
-      if (half == 0 && split == 0) {
-        p.row_stats[stat] = INFINITY;
-        p.row_stats[stats + stat] = 0.f;
-      }
-      if (q_row < p.Sq) {
-        if (p.splits > 1) {
-          for (int i = 0; i < 64; i += 4) *reinterpret_cast<float4*>(part + i) = make_float4(0.f, 0.f, 0.f, 0.f);
-        } else {
-          store_zero(out_ptr(p.dq, b, h, q_row) + half * 64, 64);
-        }
-      }
+    if (split == 0 && threadIdx.x < 128) {
+      stat[threadIdx.x] = -INFINITY;
+      stat[stats + threadIdx.x] = 0.f;
     }
+    if (p.splits > 1) zero_rows(part, 512, rows_in, 512);
+    else zero_rows(out_ptr(p.dq, b, h, q0), p.dq.st * 2, rows_in, 256);
     return;
   }
 
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + DQ_OFF_BAR);
   uint64_t* full = bars;                 // [DQ_SLOTS]
-  uint64_t* empty = full + DQ_SLOTS;     // [DQ_SLOTS]
+  uint64_t* empty = full + DQ_SLOTS;     // [DQ_SLOTS] k: released by dq; v: by dp
   uint64_t* tail = empty + DQ_SLOTS;
-  uint64_t* a_full = tail + 1;           // q and do are in tensor memory
-  uint64_t* s_full = a_full + 1;
+  uint64_t* q_full = tail + 1;           // q in shared memory
+  uint64_t* rows_full = q_full + 1;      // do and o in shared memory
+  uint64_t* do_full = rows_full + 1;     // do in tensor memory, D in shared memory
+  uint64_t* s_full = do_full + 1;
   uint64_t* s_free = s_full + 1;
   uint64_t* dp_full = s_free + 1;
-  uint64_t* ds_full = dp_full + 1;
+  uint64_t* dp_free = dp_full + 1;
+  uint64_t* ds_full = dp_free + 1;
   uint64_t* dq_done = ds_full + 1;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(dq_done + 1);
   volatile uint32_t* abort_flag = tmem_slot + 1;
-  if (threadIdx.x == 0) {
+  uint8_t* do_smem = smem + (DQ_SLOTS - 2) * TILE_BYTES;
+  uint8_t* o_smem = smem + (DQ_SLOTS - 1) * TILE_BYTES;
+  const int rem = k_len < p.Sk ? k_len % 128 : 0;  // tokens of the last tile that exist (0: no tail of k to clear)
+  const bool early = !(rem != 0 && n_all == j0 + 1);  // the first tile of k has no tail to clear
+  if (warp == W::producer && lane == 0) {
+    tma_prefetch_desc(&map_q);
+    tma_prefetch_desc(&map_k);
+    tma_prefetch_desc(&map_do);
+    tma_prefetch_desc(&map_o);
+    tma_prefetch_desc(&map_v);
     for (int i = 0; i < DQ_SLOTS; ++i) {
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], 1);
     }
     mbar_init(tail, 1);
-    mbar_init(a_full, 8);
+    mbar_init(q_full, 1);
+    mbar_init(rows_full, 1);
+    mbar_init(do_full, ROW_WARPS_B);
     mbar_init(s_full, 1);
-    mbar_init(s_free, 8);
+    mbar_init(s_free, ROW_WARPS_B);
     mbar_init(dp_full, 1);
-    mbar_init(ds_full, 8);
+    mbar_init(dp_free, ROW_WARPS_B);
+    mbar_init(ds_full, ROW_WARPS_B);
     mbar_init(dq_done, 1);
     *abort_flag = 0;
     mbar_fence_init();
+    // the first loads are under way while tensor memory is set up
+    mbar_arrive_expect_tx(q_full, TILE_BYTES);
+    issue_tile({smem + DQ_OFF_Q, &map_q, q0, h, b}, q_full);
+    if (early) {
+      mbar_arrive_expect_tx(&full[0], TILE_BYTES);
+      issue_tile({smem, &map_k, j0 * 128, h, b}, &full[0]);
+    }
+    mbar_arrive_expect_tx(rows_full, 2 * TILE_BYTES);
+    issue_tile({do_smem, &map_do, q0, h, b}, rows_full);
+    issue_tile({o_smem, &map_o, q0, h, b}, rows_full);
   }
-  const uint32_t tm = open_tmem(tmem_slot, warp);
-  constexpr uint32_t T_S = 0, T_DP = 128, T_DQ = 256, T_Q = 384, T_DO = 448;
+  const uint32_t tm = open_tmem(tmem_slot, warp == W::tmem);
+  constexpr uint32_t T_S = 0, T_DP = 128, T_DQ = 256, T_DO = 384, T_DS = 448;
 
-  if (warp >= PRODUCER_WARP) {
-    reg_dealloc_72();
-    if (warp == PRODUCER_WARP) {
-      const int rem = k_len < p.Sk ? k_len % 128 : 0;  // rows of the last tile of k that exist (0: no tail to clear)
-      for (int seq = 0; seq < 2 * n; ++seq) {
-        const int j = j0 + (seq >> 1);
+  if (warp >= W::producer) {
+    other_warp_registers<ROW_WARPS_B>();
+    if (warp == W::producer) {
+      for (int seq = early ? 1 : 0; seq <= 2 * n; ++seq) {
+        // entry 2 n: the first tile of k, for its mean
+        const bool is_k = (seq & 1) == 0, mean = seq == 2 * n;
+        const int j = mean ? 0 : j0 + (seq >> 1);
         const uint32_t s = seq % DQ_SLOTS, ph = (seq / DQ_SLOTS) & 1u;
         if (!mbar_wait(&empty[s], ph ^ 1u, abort_flag)) break;
-        const TileLoad t = {smem + s * TILE_BYTES, (seq & 1) ? &map_v : &map_k, j * 128, h, b};
-        if (rem != 0 && j == n_all - 1 && (seq & 1) == 0) {
+        if (seq >= DQ_SLOTS - 2 && seq < DQ_SLOTS && !mbar_wait(do_full, 0, abort_flag)) break;  // do and o have been read
+        const TileLoad t = {smem + s * TILE_BYTES, is_k ? &map_k : &map_v, j * 128, h, b};
+        if (is_k && !mean && rem != 0 && j == n_all - 1) {
           if (!load_tile_tail(t, tail, 0, rem, &full[s], abort_flag)) break;
         } else if (lane == 0) {
           mbar_arrive_expect_tx(&full[s], TILE_BYTES);
@@ -272,43 +373,41 @@ attn_bwd_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
         }
         __syncwarp();
       }
-    } else if (warp == ISSUER_WARP0) {
+    } else if (warp == W::issuer0) {
       const bool leader = elect_one();
       const uint32_t ring = smem_u32(smem), id = idesc_k<BF16>();
-      bool ok = mbar_wait(a_full, 0, abort_flag);
+      bool ok = mbar_wait(q_full, 0, abort_flag);
       for (int j = 0; ok && j < n; ++j) {
-        const uint32_t seq = 2 * j, s = seq % DQ_SLOTS, ph = (seq / DQ_SLOTS) & 1u;
-        ok = mbar_wait(&full[s], ph, abort_flag) && (j == 0 || mbar_wait(s_free, (j - 1) & 1u, abort_flag));
+        const uint32_t ks = (2 * j) % DQ_SLOTS, kph = ((2 * j) / DQ_SLOTS) & 1u;
+        const uint32_t vs = (2 * j + 1) % DQ_SLOTS, vph = ((2 * j + 1) / DQ_SLOTS) & 1u;
+        ok = mbar_wait(&full[ks], kph, abort_flag) && (j == 0 || mbar_wait(s_free, (j - 1) & 1u, abort_flag));
         if (!ok) break;
         tc_fence_after_sync();
         if (leader) {
-          mma_ts_k(tm + T_S, tm + T_Q, ring + s * TILE_BYTES, id);
+          mma_ss(tm + T_S, ring + DQ_OFF_Q, ring + ks * TILE_BYTES, id);
           umma_commit(s_full);
         }
         __syncwarp();
-      }
-    } else if (warp == ISSUER_WARP1) {
-      const bool leader = elect_one();
-      const uint32_t ring = smem_u32(smem), id = idesc_k<BF16>(), id_mn = idesc_mn<BF16>();
-      bool ok = mbar_wait(a_full, 0, abort_flag);
-      for (int j = 0; ok && j < n; ++j) {
-        const uint32_t seq = 2 * j + 1, s = seq % DQ_SLOTS, ph = (seq / DQ_SLOTS) & 1u;
-        // dp lies where ds of the last tile was read: that product has to be over
-        ok = mbar_wait(&full[s], ph, abort_flag) && (j == 0 || mbar_wait(dq_done, (j - 1) & 1u, abort_flag));
+        ok = mbar_wait(&full[vs], vph, abort_flag) && (j == 0 ? mbar_wait(do_full, 0, abort_flag) : mbar_wait(dp_free, (j - 1) & 1u, abort_flag));
         if (!ok) break;
         tc_fence_after_sync();
         if (leader) {
-          mma_ts_k(tm + T_DP, tm + T_DO, ring + s * TILE_BYTES, id);
+          mma_ts_k(tm + T_DP, tm + T_DO, ring + vs * TILE_BYTES, id);
           umma_commit(dp_full);
-          umma_commit(&empty[s]);
+          umma_commit(&empty[vs]);
         }
         __syncwarp();
-        ok = mbar_wait(ds_full, j & 1u, abort_flag);
-        if (!ok) break;
+      }
+    } else if (warp == W::issuer1) {
+      const bool leader = elect_one();
+      const uint32_t ring = smem_u32(smem), id_mn = idesc_mn<BF16>();
+      for (int j = 0; j < n; ++j) {
+        const uint32_t ks = (2 * j) % DQ_SLOTS, kph = ((2 * j) / DQ_SLOTS) & 1u;
+        // ds exists, so s of this tile is long complete: the slot of k is free with this product
+        if (!(mbar_wait(&full[ks], kph, abort_flag) && mbar_wait(ds_full, j & 1u, abort_flag))) break;
         tc_fence_after_sync();
-        const uint32_t ks = (2 * j) % DQ_SLOTS;
         if (leader) {
-          mma_ts_mn(tm + T_DQ, tm + T_DP, 64, ring + ks * TILE_BYTES, id_mn, j == 0);
+          mma_ts_mn(tm + T_DQ, tm + T_DS, ring + ks * TILE_BYTES, id_mn, j == 0);
           umma_commit(dq_done);
           umma_commit(&empty[ks]);
         }
@@ -316,128 +415,174 @@ attn_bwd_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
       }
     }
   } else {
-    reg_alloc_216();
+    row_warp_registers<ROW_WARPS_B>();
+    const int cg = warp >> 2, r = (warp & 3) * 32 + lane, q_row = q0 + r;
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const bool live = q_row < q_len;
-    float* s_stat = reinterpret_cast<float*>(smem + DQ_OFF_STAT);  // [2][128]: lse * log2 e, D
-    // warps 0-3 bring q, warps 4-7 bring do and compute D
-    {
-      uint32_t w[32];
-      const Rows& src = half == 0 ? p.q : p.dout;
+    float* s_d = reinterpret_cast<float*>(smem + DQ_OFF_D);
+    float* s_e = reinterpret_cast<float*>(smem + DQ_OFF_E);
+    float* s_mean = reinterpret_cast<float*>(smem + DQ_OFF_MEAN);
+    float nl = -INFINITY;
+    if (live) {
+      const float l = p.lse[static_cast<int64_t>(bh) * p.Sq + q_row];
+      nl = l == -INFINITY ? -INFINITY : -l * LOG2E;
+    }
+    bool ok = mbar_wait(rows_full, 0, abort_flag);
+    {  // a quarter of a row of do to tensor memory, and its part of D
+      uint32_t w[16];
       float d = 0.f;
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
+      for (int i = 0; i < 4; ++i) {
+        const int at = (cg >> 1) * BOX_BYTES + r * 128 + ((((cg & 1) * 4 + i) ^ (r & 7)) << 4);
+        uint4 u = *reinterpret_cast<const uint4*>(do_smem + at), o = *reinterpret_cast<const uint4*>(o_smem + at);
+        if (!live) u = o = make_uint4(0u, 0u, 0u, 0u);
+        const uint32_t uw[4] = {u.x, u.y, u.z, u.w}, ow[4] = {o.x, o.y, o.z, o.w};
 #pragma unroll
-        for (int i = 0; i < 32; i += 4) {
-          uint4 u = make_uint4(0u, 0u, 0u, 0u);
-          if (live) u = *reinterpret_cast<const uint4*>(row_ptr(src, b, h, q_row) + c * 64 + 2 * i);
-          w[i] = u.x; w[i + 1] = u.y; w[i + 2] = u.z; w[i + 3] = u.w;
-        }
-        tmem_st32(tm + lanes + (half == 0 ? T_Q : T_DO) + 32 * c, w);
-        if (half == 1 && live) {
-#pragma unroll
-          for (int i = 0; i < 32; i += 4) {
-            const uint4 u = *reinterpret_cast<const uint4*>(row_ptr(p.o, b, h, q_row) + c * 64 + 2 * i);
-            const uint32_t ow[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              float a0, a1, o0, o1;
-              unpack<BF16>(w[i + k], a0, a1);
-              unpack<BF16>(ow[k], o0, o1);
-              d = fmaf(a0, o0, d);
-              d = fmaf(a1, o1, d);
-            }
-          }
+        for (int k = 0; k < 4; ++k) {
+          float a0, a1, o0, o1;
+          unpack2<BF16>(uw[k], a0, a1);
+          unpack2<BF16>(ow[k], o0, o1);
+          d = fmaf(a0, o0, d);
+          d = fmaf(a1, o1, d);
+          w[4 * i + k] = uw[k];
         }
       }
+      tmem_st16(tm + lanes + T_DO + cg * 16, w);
+      s_d[cg * 128 + r] = d;
       tmem_wait_st();
       tc_fence_before_sync();
-      if (half == 1) {
-        float l2 = INFINITY;
-        if (live) {
-          const float l = p.lse[static_cast<int64_t>(bh) * p.Sq + q_row];
-          l2 = l == -INFINITY ? INFINITY : l * LOG2E;
-        }
-        s_stat[r] = l2;
-        s_stat[128 + r] = d;
-        if (split == 0) {
-          p.row_stats[stat] = l2;
-          p.row_stats[stats + stat] = d;
-        }
-      }
       __syncwarp();
-      if (lane == 0) mbar_arrive(a_full);
+      if (lane == 0) mbar_arrive(do_full);
     }
-    bool ok = mbar_wait(a_full, 0, abort_flag);  // all 8 warps have arrived: s_stat is complete
-    const float neg_l2 = -s_stat[r], neg_d = -s_stat[128 + r];
-    const float cmul = p.sm_scale * LOG2E;
+    ok = ok && mbar_wait(do_full, 0, abort_flag);  // all warps have arrived
+    const float nd = -((s_d[r] + s_d[128 + r]) + (s_d[256 + r] + s_d[384 + r]));
+    if (cg == 0 && split == 0) {
+      stat[r] = nl;
+      stat[stats + r] = nd;
+    }
+    const uint64_t nl2 = f2_splat(nl), nd2 = f2_splat(nd), cmul2 = f2_splat(p.sm_scale * LOG2E);
+    uint64_t e2 = f2_splat(0.f);  // sum of the rounded ds
     for (int j = 0; ok && j < n; ++j) {
-      const int valid = k_len - (j0 + j) * 128 - half * 64;  // this thread's columns that exist
+      const int valid = k_len - (j0 + j) * 128 - cg * 32;  // this thread's columns that exist
       if (!(ok = mbar_wait(s_full, j & 1u, abort_flag))) break;
       tc_fence_after_sync();
-      uint32_t sv[64];
-      tmem_ld32(tm + lanes + T_S + half * 64, *reinterpret_cast<uint32_t(*)[32]>(&sv[0]));
-      tmem_ld32(tm + lanes + T_S + half * 64 + 32, *reinterpret_cast<uint32_t(*)[32]>(&sv[32]));
+      uint32_t sv[32];
+      tmem_ld32(tm + lanes + T_S + cg * 32, sv);
       tmem_wait_ld();
       tc_fence_before_sync();
       __syncwarp();
       if (lane == 0) mbar_arrive(s_free);
 #pragma unroll
-      for (int i = 0; i < 64; ++i) sv[i] = __float_as_uint(ex2(fmaf(__uint_as_float(sv[i]), cmul, neg_l2)));
+      for (int i = 0; i < 32; i += 2) {
+        float a, c;
+        f2_unpack(f2_fma(f2_bits(sv[i], sv[i + 1]), cmul2, nl2), a, c);
+        sv[i] = __float_as_uint(ex2(a));
+        sv[i + 1] = __float_as_uint(ex2(c));
+      }
       if (!(ok = mbar_wait(dp_full, j & 1u, abort_flag))) break;
       tc_fence_after_sync();
+      uint32_t dp[32];
+      tmem_ld32(tm + lanes + T_DP + cg * 32, dp);
+      tmem_wait_ld();
+      tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(dp_free);
+      if (valid < 32) {  // keys behind the length: whatever v holds there
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        uint32_t dp[32];
-        tmem_ld32(tm + lanes + T_DP + half * 64 + 32 * c, dp);
-        tmem_wait_ld();
-#pragma unroll
-        for (int i = 0; i < 32; ++i)
-          sv[32 * c + i] = __float_as_uint(__uint_as_float(sv[32 * c + i]) * (__uint_as_float(dp[i]) + neg_d));
+        for (int i = 0; i < 32; ++i) {
+          sv[i] = i < valid ? sv[i] : 0u;
+          dp[i] = i < valid ? dp[i] : 0u;
+        }
       }
-      if (valid < 64) {  // keys behind the length: whatever their scores were
+      uint32_t pk[16];
 #pragma unroll
-        for (int i = 0; i < 64; ++i) sv[i] = i < valid ? sv[i] : 0u;
+      for (int i = 0; i < 16; ++i) {
+        uint64_t hi;
+        pk[i] = pack_signed<BF16>(f2_mul(f2_bits(sv[2 * i], sv[2 * i + 1]), f2_add(f2_bits(dp[2 * i], dp[2 * i + 1]), nd2)), hi);
+        e2 = f2_add(e2, hi);
       }
-      uint32_t pk[32];
-#pragma unroll
-      for (int i = 0; i < 32; ++i) pk[i] = pack_rn<BF16>(__uint_as_float(sv[2 * i]), __uint_as_float(sv[2 * i + 1]));
-      tmem_st32(tm + lanes + T_DP + half * 64, pk);
+      if (j > 0) {  // ds of the last tile has been read (normally long ago)
+        if (!(ok = mbar_wait(dq_done, (j - 1) & 1u, abort_flag))) break;
+        tc_fence_after_sync();
+      }
+      tmem_st16(tm + lanes + T_DS + cg * 16, pk);
       tmem_wait_st();
       tc_fence_before_sync();
       __syncwarp();
       if (lane == 0) mbar_arrive(ds_full);
     }
+    // m: the mean of the first tile's keys; a thread adds eight channels of four keys
+    if (ok) ok = mbar_wait(&full[(2 * n) % DQ_SLOTS], ((2 * n) / DQ_SLOTS) & 1u, abort_flag);
+    {
+      const uint8_t* k_smem = smem + ((2 * n) % DQ_SLOTS) * TILE_BYTES;
+      const int rows = min(128, k_len), chunk = threadIdx.x & 15, k0 = (threadIdx.x >> 4) * 4;
+      float m[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (k0 + i < rows) {
+          const uint4 u = *reinterpret_cast<const uint4*>(k_smem + (chunk >> 3) * BOX_BYTES + (k0 + i) * 128 + (((chunk & 7) ^ ((k0 + i) & 7)) << 4));
+          const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            float a0, a1;
+            unpack2<BF16>(w[k], a0, a1);
+            m[2 * k] += a0;
+            m[2 * k + 1] += a1;
+          }
+        }
+      const float inv = 1.f / static_cast<float>(rows);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) m[k] = (m[k] + __shfl_xor_sync(0xffffffffu, m[k], 16)) * inv;
+      if (lane < 16) {
+        *reinterpret_cast<float4*>(s_mean + warp * 128 + chunk * 8) = make_float4(m[0], m[1], m[2], m[3]);
+        *reinterpret_cast<float4*>(s_mean + warp * 128 + chunk * 8 + 4) = make_float4(m[4], m[5], m[6], m[7]);
+      }
+      float a0, a1;
+      f2_unpack(e2, a0, a1);
+      s_e[cg * 128 + r] = a0 + a1;
+      row_warps_sync();
+      if (threadIdx.x < 128) {
+        float t = 0.f;
+#pragma unroll
+        for (int k = 0; k < 16; ++k) t += s_mean[k * 128 + threadIdx.x];
+        s_mean[threadIdx.x] = t;  // only this thread reads or writes this channel until the barrier
+      }
+      row_warps_sync();
+    }
     if (ok && mbar_wait(dq_done, (n - 1) & 1u, abort_flag)) {
       tc_fence_after_sync();
       // the softmax over one key is constant: its gradient is zero, not the rounding of dp - D
       const float mul = k_len == 1 ? 0.f : p.sm_scale;
-#pragma unroll 1
-      for (int c = 0; c < 2; ++c) {
-        uint32_t v[32];
-        tmem_ld32(tm + lanes + T_DQ + half * 64 + 32 * c, v);
-        tmem_wait_ld();
-        if (q_row >= p.Sq) continue;
-        if (p.splits > 1) {
-          for (int i = 0; i < 32; i += 4)
-            *reinterpret_cast<uint4*>(part + 32 * c + i) = live ? make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]) : make_uint4(0u, 0u, 0u, 0u);
-        } else if (live) {
-          store_row32<BF16>(out_ptr(p.dq, b, h, q_row) + half * 64 + 32 * c, v, mul);
-        } else {
-          store_zero(out_ptr(p.dq, b, h, q_row) + half * 64 + 32 * c, 32);
-        }
+      const float neg_e = -((s_e[r] + s_e[128 + r]) + (s_e[256 + r] + s_e[384 + r]));
+      const int rows = max(0, min(32, rows_in - (warp & 3) * 32));
+      uint8_t* st = smem + warp * 4096;  // every product and every copy is complete: the ring stages the results
+      uint32_t v[32];
+      tmem_ld32(tm + lanes + T_DQ + cg * 32, v);
+      tmem_wait_ld();
+#pragma unroll
+      for (int i = 0; i < 32; i += 4) {
+        const float4 m = *reinterpret_cast<const float4*>(s_mean + cg * 32 + i);
+        v[i] = __float_as_uint(fmaf(neg_e, m.x, __uint_as_float(v[i])));
+        v[i + 1] = __float_as_uint(fmaf(neg_e, m.y, __uint_as_float(v[i + 1])));
+        v[i + 2] = __float_as_uint(fmaf(neg_e, m.z, __uint_as_float(v[i + 2])));
+        v[i + 3] = __float_as_uint(fmaf(neg_e, m.w, __uint_as_float(v[i + 3])));
       }
+      if (p.splits > 1) store_part32(st, v, 1.f, live, part + (warp & 3) * 32 * 128 + cg * 32, rows);
+      else store_cols32<BF16>(st, v, mul, live, out_ptr(p.dq, b, h, q0 + (warp & 3) * 32) + cg * 32, p.dq.st, rows);
     }
   }
-  close_tmem(tm, warp, abort_flag, p.status);
+  close_tmem(tm, warp == W::tmem, abort_flag, p.status);
 }
 
 // ---- dk, dv ------------------------------------------------------------------------------------------------------------
 // One CTA = 128 keys of one head; k and v stay in shared memory, q and do tiles pass through the ring.  Everything is
-// transposed: a thread owns a KEY row x 64 queries, so p^T and ds^T come out as A operands of dv += p^T.do and
+// transposed: a thread owns a KEY row x 32 queries, so p^T and ds^T come out as A operands of dv += p^T.do and
 // dk += ds^T.q and never leave tensor memory; lse and D of the queries are read along the row.
-//   warp 9   issues s^T = k.q_i^T and dv += p^T.do_i        warp 10  issues dp^T = v.do_i^T and dk += ds^T.q_i
-// Tensor memory: s^T [0,128), p^T over it   dp^T [128,256), ds^T over it   dv [256,384)   dk [384,512).
+//   issuer 0     s^T = k.q_i^T and dv += p^T.do_i        issuer 1     dp^T = v.do_i^T and dk += ds^T.q_i
+// Tensor memory: s^T [0,128), p^T over it   dp^T [128,256), ds^T over it   dv [256,384)   dk [384,512): all of it, so s^T of
+// the next tile has to wait for dv of this one, which waits for the exponentials: that chain is the period.  It is kept
+// short by handing p^T over in halves (the first half's product runs under the second half's exponentials) and by issuing
+// the next s^T ahead of this tile's dk.
 constexpr int KV_SLOTS = 4;
 constexpr int KV_OFF_K = KV_SLOTS * TILE_BYTES;
 constexpr int KV_OFF_V = KV_OFF_K + TILE_BYTES;
@@ -446,9 +591,10 @@ constexpr int KV_OFF_BAR = KV_OFF_STAT + 2048;
 constexpr int KV_SMEM = KV_OFF_BAR + 256 + 1024;
 
 template <bool BF16>
-__global__ void __launch_bounds__(THREADS, 1)
+__global__ void __launch_bounds__(Warps<ROW_WARPS_B>::threads, 1)
 attn_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_do,
                      const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const TrainParams p) {
+  using W = Warps<ROW_WARPS_B>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -457,22 +603,18 @@ attn_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
   const int n_all = k0 < k_len ? (q_len + 127) / 128 : 0;
   const int per = (n_all + p.splits - 1) / p.splits;
   const int i0 = split * per, n = max(0, min(n_all, i0 + per) - i0);
-  const int r = (warp & 3) * 32 + lane, half = (warp >> 2) & 1, k_row = k0 + r;
   // a split run leaves fp32 sums: dk [split][BH][Sk][128], then dv the same
   const int64_t part_all = static_cast<int64_t>(p.splits) * p.B * p.heads * p.Sk * 128;
-  float* part = p.part + ((static_cast<int64_t>(split) * p.B * p.heads + bh) * p.Sk + k_row) * 128 + half * 64;
+  float* part = p.part + ((static_cast<int64_t>(split) * p.B * p.heads + bh) * p.Sk + k0) * 128;
+  const int rows_in = min(128, p.Sk - k0);
 
   if (n == 0) {
-    if (warp < 8 && k_row < p.Sk) {
-      if (p.splits > 1) {
-        for (int i = 0; i < 64; i += 4) {
-          *reinterpret_cast<float4*>(part + i) = make_float4(0.f, 0.f, 0.f, 0.f);
-          *reinterpret_cast<float4*>(part + part_all + i) = make_float4(0.f, 0.f, 0.f, 0.f);
-        }
-      } else {
-        store_zero(out_ptr(p.dk, b, h, k_row) + half * 64, 64);
-        store_zero(out_ptr(p.dv, b, h, k_row) + half * 64, 64);
-      }
+    if (p.splits > 1) {
+      zero_rows(part, 512, rows_in, 512);
+      zero_rows(part + part_all, 512, rows_in, 512);
+    } else {
+      zero_rows(out_ptr(p.dk, b, h, k0), p.dk.st * 2, rows_in, 256);
+      zero_rows(out_ptr(p.dv, b, h, k0), p.dv.st * 2, rows_in, 256);
     }
     return;
   }
@@ -481,44 +623,53 @@ attn_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
   uint64_t* full = bars;                // [KV_SLOTS]
   uint64_t* empty = full + KV_SLOTS;    // [KV_SLOTS] released by the two products that read the tile
   uint64_t* tail = empty + KV_SLOTS;
-  uint64_t* kv_full = tail + 1;
-  uint64_t* s_full = kv_full + 1;
-  uint64_t* p_full = s_full + 1;
-  uint64_t* dv_done = p_full + 1;
+  uint64_t* k_full = tail + 1;
+  uint64_t* v_full = k_full + 1;
+  uint64_t* s_full = v_full + 1;
+  uint64_t* s_issued = s_full + 1;
+  uint64_t* p_full = s_issued + 1;      // [2] halves of every thread's queries
+  uint64_t* dv_done = p_full + 2;
   uint64_t* dp_full = dv_done + 1;
-  uint64_t* ds_full = dp_full + 1;
-  uint64_t* dk_done = ds_full + 1;
+  uint64_t* ds_full = dp_full + 1;      // [2]
+  uint64_t* dk_done = ds_full + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(dk_done + 1);
   volatile uint32_t* abort_flag = tmem_slot + 1;
-  if (threadIdx.x == 0) {
+  if (warp == W::producer && lane == 0) {
+    tma_prefetch_desc(&map_k);
+    tma_prefetch_desc(&map_q);
+    tma_prefetch_desc(&map_v);
+    tma_prefetch_desc(&map_do);
     for (int i = 0; i < KV_SLOTS; ++i) {
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], 2);
     }
     mbar_init(tail, 1);
-    mbar_init(kv_full, 1);
+    mbar_init(k_full, 1);
+    mbar_init(v_full, 1);
     mbar_init(s_full, 1);
-    mbar_init(p_full, 8);
+    mbar_init(s_issued, 1);
     mbar_init(dv_done, 1);
     mbar_init(dp_full, 1);
-    mbar_init(ds_full, 8);
     mbar_init(dk_done, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&p_full[i], ROW_WARPS_B);
+      mbar_init(&ds_full[i], ROW_WARPS_B);
+    }
     *abort_flag = 0;
     mbar_fence_init();
+    // the first loads are under way while tensor memory is set up
+    mbar_arrive_expect_tx(k_full, TILE_BYTES);
+    issue_tile({smem + KV_OFF_K, &map_k, k0, h, b}, k_full);
+    mbar_arrive_expect_tx(v_full, TILE_BYTES);
+    issue_tile({smem + KV_OFF_V, &map_v, k0, h, b}, v_full);
   }
-  const uint32_t tm = open_tmem(tmem_slot, warp);
+  const uint32_t tm = open_tmem(tmem_slot, warp == W::tmem);
   constexpr uint32_t T_S = 0, T_DP = 128, T_DV = 256, T_DK = 384;
   const int64_t stats = static_cast<int64_t>(p.B) * p.heads * p.Sq_pad;
 
-  if (warp >= PRODUCER_WARP) {
-    reg_dealloc_72();
-    if (warp == PRODUCER_WARP) {
-      if (lane == 0) {
-        mbar_arrive_expect_tx(kv_full, 2 * TILE_BYTES);
-        issue_tile({smem + KV_OFF_K, &map_k, k0, h, b}, kv_full);
-        issue_tile({smem + KV_OFF_V, &map_v, k0, h, b}, kv_full);
-      }
-      __syncwarp();
+  if (warp >= W::producer) {
+    other_warp_registers<ROW_WARPS_B>();
+    if (warp == W::producer) {
       const int rem = q_len < p.Sq ? q_len % 128 : 0;
       for (int seq = 0; seq < 2 * n; ++seq) {
         const int i = i0 + (seq >> 1);
@@ -527,15 +678,13 @@ attn_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
         const bool is_q = (seq & 1) == 0, clear = rem != 0 && i == n_all - 1;
         const TileLoad t = {smem + s * TILE_BYTES, is_q ? &map_q : &map_do, i * 128, h, b};
         if (lane == 0) {
-          // lse and D of the tile's queries ride on the q tile's barrier; the stage is free with the slot
-          const uint32_t bytes = (is_q ? 1024 : 0) + (clear ? 0 : TILE_BYTES);
-          if (bytes != 0 && !clear) mbar_arrive_expect_tx(&full[s], bytes);
+          // lse and D of the tile's queries ride on the q tile's barrier; the stage is free with the slot.  Where a tail is
+          // cleared, the arrival (and the tile's own bytes) are load_tile_tail's
+          if (!clear) mbar_arrive_expect_tx(&full[s], TILE_BYTES + (is_q ? 1024u : 0u));
+          else if (is_q) mbar_expect_tx(&full[s], 1024u);
           if (is_q) {
             float* dst = reinterpret_cast<float*>(smem + KV_OFF_STAT) + (seq / 2 % 2) * 256;
             const float* src = p.row_stats + static_cast<int64_t>(bh) * p.Sq_pad + i * 128;
-            if (clear) {  // the arrival comes from load_tile_tail
-              asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(&full[s])), "r"(1024u) : "memory");
-            }
             bulk_load(dst, src, 512, &full[s]);
             bulk_load(dst + 128, src + stats, 512, &full[s]);
           }
@@ -544,10 +693,10 @@ attn_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
         __syncwarp();
         if (clear && !load_tile_tail(t, tail, is_q ? 0u : 1u, rem, &full[s], abort_flag)) break;
       }
-    } else if (warp == ISSUER_WARP0) {
+    } else if (warp == W::issuer0) {
       const bool leader = elect_one();
       const uint32_t ring = smem_u32(smem), id = idesc_k<BF16>(), id_mn = idesc_mn<BF16>();
-      bool ok = mbar_wait(kv_full, 0, abort_flag);
+      bool ok = mbar_wait(k_full, 0, abort_flag);
       for (int i = 0; ok && i < n; ++i) {
         const uint32_t seq = 2 * i, s = seq % KV_SLOTS, ph = (seq / KV_SLOTS) & 1u, s1 = (seq + 1) % KV_SLOTS, ph1 = ((seq + 1) / KV_SLOTS) & 1u;
         // s^T lies where p^T of the last tile was read: that product has to be over
@@ -558,22 +707,27 @@ attn_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
           mma_ss(tm + T_S, ring + KV_OFF_K, ring + s * TILE_BYTES, id);
           umma_commit(s_full);
           umma_commit(&empty[s]);
+          mbar_arrive(s_issued);
         }
         __syncwarp();
-        ok = mbar_wait(&full[s1], ph1, abort_flag) && mbar_wait(p_full, i & 1u, abort_flag);
+        ok = mbar_wait(&full[s1], ph1, abort_flag);
+        for (int c = 0; ok && c < 2; ++c) {
+          if (!(ok = mbar_wait(&p_full[c], i & 1u, abort_flag))) break;
+          tc_fence_after_sync();
+          if (leader) mma_ts_mn_half(tm + T_DV, tm + T_S, c, ring + s1 * TILE_BYTES, id_mn, i == 0 && c == 0);
+          __syncwarp();
+        }
         if (!ok) break;
-        tc_fence_after_sync();
         if (leader) {
-          mma_ts_mn(tm + T_DV, tm + T_S, 64, ring + s1 * TILE_BYTES, id_mn, i == 0);
           umma_commit(dv_done);
           umma_commit(&empty[s1]);
         }
         __syncwarp();
       }
-    } else if (warp == ISSUER_WARP1) {
+    } else if (warp == W::issuer1) {
       const bool leader = elect_one();
       const uint32_t ring = smem_u32(smem), id = idesc_k<BF16>(), id_mn = idesc_mn<BF16>();
-      bool ok = mbar_wait(kv_full, 0, abort_flag);
+      bool ok = mbar_wait(v_full, 0, abort_flag) && mbar_wait(s_issued, 0, abort_flag);
       for (int i = 0; ok && i < n; ++i) {
         const uint32_t seq = 2 * i, s = seq % KV_SLOTS, ph = (seq / KV_SLOTS) & 1u, s1 = (seq + 1) % KV_SLOTS, ph1 = ((seq + 1) / KV_SLOTS) & 1u;
         ok = mbar_wait(&full[s1], ph1, abort_flag) && (i == 0 || mbar_wait(dk_done, (i - 1) & 1u, abort_flag));
@@ -585,11 +739,16 @@ attn_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
           umma_commit(&empty[s1]);
         }
         __syncwarp();
-        ok = mbar_wait(&full[s], ph, abort_flag) && mbar_wait(ds_full, i & 1u, abort_flag);
+        // s^T of the next tile goes first: the exponentials wait for it, nothing waits for dk
+        ok = mbar_wait(&full[s], ph, abort_flag) && (i + 1 == n || mbar_wait(s_issued, (i + 1) & 1u, abort_flag));
+        for (int c = 0; ok && c < 2; ++c) {
+          if (!(ok = mbar_wait(&ds_full[c], i & 1u, abort_flag))) break;
+          tc_fence_after_sync();
+          if (leader) mma_ts_mn_half(tm + T_DK, tm + T_DP, c, ring + s * TILE_BYTES, id_mn, i == 0 && c == 0);
+          __syncwarp();
+        }
         if (!ok) break;
-        tc_fence_after_sync();
         if (leader) {
-          mma_ts_mn(tm + T_DK, tm + T_DP, 64, ring + s * TILE_BYTES, id_mn, i == 0);
           umma_commit(dk_done);
           umma_commit(&empty[s]);
         }
@@ -597,88 +756,88 @@ attn_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
       }
     }
   } else {
-    reg_alloc_216();
+    row_warp_registers<ROW_WARPS_B>();
+    const int cg = warp >> 2, k_row = k0 + (warp & 3) * 32 + lane;
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const float cmul = p.sm_scale * LOG2E;
+    const uint64_t cmul2 = f2_splat(p.sm_scale * LOG2E);
     bool ok = true;
     for (int i = 0; ok && i < n; ++i) {
-      const float* stat = reinterpret_cast<const float*>(smem + KV_OFF_STAT) + (i % 2) * 256 + half * 64;
+      const ulonglong2* stat = reinterpret_cast<const ulonglong2*>(smem + KV_OFF_STAT + (i % 2) * 1024 + cg * 128);  // four queries each
       const uint32_t seq = 2 * i;
       ok = mbar_wait(&full[seq % KV_SLOTS], (seq / KV_SLOTS) & 1u, abort_flag) && mbar_wait(s_full, i & 1u, abort_flag);
       if (!ok) break;
       tc_fence_after_sync();
-      uint32_t sv[64];
-      tmem_ld32(tm + lanes + T_S + half * 64, *reinterpret_cast<uint32_t(*)[32]>(&sv[0]));
-      tmem_ld32(tm + lanes + T_S + half * 64 + 32, *reinterpret_cast<uint32_t(*)[32]>(&sv[32]));
+      uint32_t sv[32];
+      tmem_ld32(tm + lanes + T_S + cg * 32, sv);
       tmem_wait_ld();
 #pragma unroll
-      for (int c = 0; c < 64; c += 4) {
-        const float4 l2 = *reinterpret_cast<const float4*>(stat + c);
-        sv[c] = __float_as_uint(ex2(fmaf(__uint_as_float(sv[c]), cmul, -l2.x)));
-        sv[c + 1] = __float_as_uint(ex2(fmaf(__uint_as_float(sv[c + 1]), cmul, -l2.y)));
-        sv[c + 2] = __float_as_uint(ex2(fmaf(__uint_as_float(sv[c + 2]), cmul, -l2.z)));
-        sv[c + 3] = __float_as_uint(ex2(fmaf(__uint_as_float(sv[c + 3]), cmul, -l2.w)));
-      }
-      {
-        uint32_t pk[32];
+      for (int c = 0; c < 2; ++c) {
+        uint32_t pk[8];
 #pragma unroll
-        for (int c = 0; c < 32; ++c) pk[c] = pack_rn<BF16>(__uint_as_float(sv[2 * c]), __uint_as_float(sv[2 * c + 1]));
-        tmem_st32(tm + lanes + T_S + half * 64, pk);
+        for (int k = 0; k < 16; k += 4) {
+          const ulonglong2 nl = stat[4 * c + k / 4];
+          uint32_t* x = &sv[16 * c + k];
+          float a0, a1, a2, a3;
+          f2_unpack(f2_fma(f2_bits(x[0], x[1]), cmul2, nl.x), a0, a1);
+          f2_unpack(f2_fma(f2_bits(x[2], x[3]), cmul2, nl.y), a2, a3);
+          a0 = ex2(a0);
+          a1 = ex2(a1);
+          a2 = ex2(a2);
+          a3 = ex2(a3);
+          x[0] = __float_as_uint(a0);
+          x[1] = __float_as_uint(a1);
+          x[2] = __float_as_uint(a2);
+          x[3] = __float_as_uint(a3);
+          pk[k / 2] = pack_prob<BF16>(a0, a1);
+          pk[k / 2 + 1] = pack_prob<BF16>(a2, a3);
+        }
+        tmem_st8(tm + lanes + T_S + cg * 32 + 8 * c, pk);
+        tmem_wait_st();
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[c]);
       }
-      tmem_wait_st();
-      tc_fence_before_sync();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(p_full);
       if (!(ok = mbar_wait(dp_full, i & 1u, abort_flag))) break;
       tc_fence_after_sync();
-      uint32_t pk[32];
+      uint32_t dp[32];
+      tmem_ld32(tm + lanes + T_DP + cg * 32, dp);
+      tmem_wait_ld();
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        uint32_t dp[32];
-        tmem_ld32(tm + lanes + T_DP + half * 64 + 32 * c, dp);
-        tmem_wait_ld();
+        uint32_t pk[8];
 #pragma unroll
-        for (int k = 0; k < 32; k += 4) {
-          const float4 d = *reinterpret_cast<const float4*>(stat + 128 + 32 * c + k);
-          const float e0 = __uint_as_float(sv[32 * c + k]) * (__uint_as_float(dp[k]) - d.x);
-          const float e1 = __uint_as_float(sv[32 * c + k + 1]) * (__uint_as_float(dp[k + 1]) - d.y);
-          const float e2 = __uint_as_float(sv[32 * c + k + 2]) * (__uint_as_float(dp[k + 2]) - d.z);
-          const float e3 = __uint_as_float(sv[32 * c + k + 3]) * (__uint_as_float(dp[k + 3]) - d.w);
-          pk[16 * c + k / 2] = pack_rn<BF16>(e0, e1);
-          pk[16 * c + k / 2 + 1] = pack_rn<BF16>(e2, e3);
+        for (int k = 0; k < 16; k += 4) {
+          const ulonglong2 nd = stat[32 + 4 * c + k / 4];
+          const uint32_t* x = &sv[16 * c + k];
+          const uint32_t* y = &dp[16 * c + k];
+          uint64_t hi;
+          pk[k / 2] = pack_signed<BF16>(f2_mul(f2_bits(x[0], x[1]), f2_add(f2_bits(y[0], y[1]), nd.x)), hi);
+          pk[k / 2 + 1] = pack_signed<BF16>(f2_mul(f2_bits(x[2], x[3]), f2_add(f2_bits(y[2], y[3]), nd.y)), hi);
         }
+        tmem_st8(tm + lanes + T_DP + cg * 32 + 8 * c, pk);
+        tmem_wait_st();
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ds_full[c]);
       }
-      tmem_st32(tm + lanes + T_DP + half * 64, pk);
-      tmem_wait_st();
-      tc_fence_before_sync();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(ds_full);
     }
     if (ok && mbar_wait(dv_done, (n - 1) & 1u, abort_flag) && mbar_wait(dk_done, (n - 1) & 1u, abort_flag)) {
       tc_fence_after_sync();
       const bool live = k_row < k_len;
       const float mul = k_len == 1 ? 0.f : p.sm_scale;  // one key: see the dq kernel
+      const int row0 = (warp & 3) * 32, rows = max(0, min(32, rows_in - row0));
+      uint8_t* st = smem + warp * 4096;  // every product and every copy is complete: the ring stages the results
 #pragma unroll 1
-      for (int c = 0; c < 4; ++c) {
-        const bool is_k = c < 2;
-        const int at = (c & 1) * 32;
+      for (int c = 0; c < 2; ++c) {
         uint32_t v[32];
-        tmem_ld32(tm + lanes + (is_k ? T_DK : T_DV) + half * 64 + at, v);
+        tmem_ld32(tm + lanes + (c == 0 ? T_DK : T_DV) + cg * 32, v);
         tmem_wait_ld();
-        if (k_row >= p.Sk) continue;
-        if (p.splits > 1) {
-          float* dst = part + (is_k ? 0 : part_all) + at;
-          for (int i = 0; i < 32; i += 4)
-            *reinterpret_cast<uint4*>(dst + i) = live ? make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]) : make_uint4(0u, 0u, 0u, 0u);
-        } else {
-          uint16_t* dst = out_ptr(is_k ? p.dk : p.dv, b, h, k_row) + half * 64 + at;
-          if (live) store_row32<BF16>(dst, v, is_k ? mul : 1.f);
-          else store_zero(dst, 32);
-        }
+        if (p.splits > 1) store_part32(st, v, 1.f, live, part + (c == 0 ? 0 : part_all) + row0 * 128 + cg * 32, rows);
+        else store_cols32<BF16>(st, v, c == 0 ? mul : 1.f, live, out_ptr(c == 0 ? p.dk : p.dv, b, h, k0 + row0) + cg * 32, (c == 0 ? p.dk : p.dv).st, rows);
       }
     }
   }
-  close_tmem(tm, warp, abort_flag, p.status);
+  close_tmem(tm, warp == W::tmem, abort_flag, p.status);
 }
 
 // ---- forward -----------------------------------------------------------------------------------------------------------
@@ -693,7 +852,7 @@ constexpr int F_OFF_BAR = F_OFF_RING + F_SLOTS * TILE_BYTES;
 constexpr int F_SMEM = F_OFF_BAR + 256 + 1024;
 
 template <bool BF16>
-__global__ void __launch_bounds__(THREADS, 1)
+__global__ void __launch_bounds__(Warps<ROW_WARPS_F>::threads, 1)
 attn_fwd_lse_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                     const __grid_constant__ CUtensorMap map_v, const TrainParams p) {
   extern __shared__ uint8_t smem_raw[];
@@ -708,18 +867,16 @@ attn_fwd_lse_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
   const int x = warp >> 2, r = (warp & 3) * 32 + lane, q_row = q0 + x * 128 + r;
   const int64_t row = static_cast<int64_t>(bh) * p.Sq + q_row;
   const int64_t split_row = static_cast<int64_t>(split) * p.B * p.heads * p.Sq + row;
-  auto store_nothing = [&]() {
-    if (q_row >= p.Sq) return;
-    if (p.splits > 1) {  // a part without keys: zero weight
-      p.part_lse[split_row] = -INFINITY;
-      for (int i = 0; i < 128; i += 4) *reinterpret_cast<float4*>(p.part + split_row * 128 + i) = make_float4(0.f, 0.f, 0.f, 0.f);
+  const int rows_in = max(0, min(256, p.Sq - q0));  // rows of the CTA
+  if (n == 0) {  // zeros, or a part of zero weight
+    if (p.splits > 1) {
+      float* part = p.part + (static_cast<int64_t>(split) * p.B * p.heads * p.Sq + static_cast<int64_t>(bh) * p.Sq + q0) * 128;
+      zero_rows(part, 512, rows_in, 512);
+      if (warp < 8 && q_row < p.Sq) p.part_lse[split_row] = -INFINITY;
     } else {
-      p.lse[row] = -INFINITY;
-      store_zero(out_ptr(p.o, b, h, q_row), 128);
+      zero_rows(out_ptr(p.o, b, h, q0), p.o.st * 2, rows_in, 256);
+      if (warp < 8 && q_row < p.Sq) p.lse[row] = -INFINITY;
     }
-  };
-  if (n == 0) {
-    if (warp < 8) store_nothing();
     return;
   }
 
@@ -734,7 +891,12 @@ attn_fwd_lse_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
   uint64_t* pv_done = p_full + 2;          // [2]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(pv_done + 2);
   volatile uint32_t* abort_flag = tmem_slot + 1;
-  if (threadIdx.x == 0) {
+  using W = Warps<ROW_WARPS_F>;
+  const int rem = k_len < p.Sk ? k_len % 128 : 0;  // tokens of the last tile that exist (0: no tail of v to clear)
+  if (warp == W::producer && lane == 0) {
+    tma_prefetch_desc(&map_q);
+    tma_prefetch_desc(&map_k);
+    tma_prefetch_desc(&map_v);
     mbar_init(q_full, 1);
     mbar_init(tail, 1);
     for (int i = 0; i < F_SLOTS; ++i) {
@@ -749,19 +911,18 @@ attn_fwd_lse_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     }
     *abort_flag = 0;
     mbar_fence_init();
+    // the first loads are under way while tensor memory is set up
+    mbar_arrive_expect_tx(q_full, tiles * TILE_BYTES);
+    for (int t = 0; t < tiles; ++t) issue_tile({smem + F_OFF_Q + t * TILE_BYTES, &map_q, q0 + t * 128, h, b}, q_full);
+    mbar_arrive_expect_tx(&kv_full[0], TILE_BYTES);
+    issue_tile({smem + F_OFF_RING, &map_k, j0 * 128, h, b}, &kv_full[0]);
   }
-  const uint32_t tm = open_tmem(tmem_slot, warp);
+  const uint32_t tm = open_tmem(tmem_slot, warp == W::tmem);
 
-  if (warp >= PRODUCER_WARP) {
-    reg_dealloc_72();
-    if (warp == PRODUCER_WARP) {
-      if (lane == 0) {
-        mbar_arrive_expect_tx(q_full, tiles * TILE_BYTES);
-        for (int t = 0; t < tiles; ++t) issue_tile({smem + F_OFF_Q + t * TILE_BYTES, &map_q, q0 + t * 128, h, b}, q_full);
-      }
-      __syncwarp();
-      const int rem = k_len < p.Sk ? k_len % 128 : 0;
-      for (int seq = 0; seq < 2 * n; ++seq) {
+  if (warp >= W::producer) {
+    other_warp_registers<ROW_WARPS_F>();
+    if (warp == W::producer) {
+      for (int seq = 1; seq < 2 * n; ++seq) {
         const int j = j0 + (seq >> 1);
         const uint32_t s = seq % F_SLOTS, ph = (seq / F_SLOTS) & 1u;
         if (!mbar_wait(&kv_empty[s], ph ^ 1u, abort_flag)) break;
@@ -774,7 +935,7 @@ attn_fwd_lse_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         }
         __syncwarp();
       }
-    } else if (warp == ISSUER_WARP0) {
+    } else if (warp == W::issuer0) {
       const bool leader = elect_one();
       const uint32_t q_base = smem_u32(smem + F_OFF_Q), ring = smem_u32(smem + F_OFF_RING), id = idesc_k<BF16>();
       bool ok = mbar_wait(q_full, 0, abort_flag);
@@ -791,7 +952,7 @@ attn_fwd_lse_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         }
         __syncwarp();
       }
-    } else if (warp == ISSUER_WARP1) {
+    } else if (warp == W::issuer1) {
       const bool leader = elect_one();
       const uint32_t ring = smem_u32(smem + F_OFF_RING), id_mn = idesc_mn<BF16>();
       bool ok = true;
@@ -802,7 +963,7 @@ attn_fwd_lse_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         if (!ok) break;
         tc_fence_after_sync();
         if (leader) {
-          mma_ts_mn(tm + 256 + t * 128, tm + 128 + t * 64, 32, ring + s * TILE_BYTES, id_mn, j == 0);
+          mma_ts_mn(tm + 256 + t * 128, tm + 128 + t * 64, ring + s * TILE_BYTES, id_mn, j == 0);
           umma_commit(&pv_done[t]);
           umma_commit(&kv_empty[s]);
         }
@@ -810,7 +971,7 @@ attn_fwd_lse_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
       }
     }
   } else if (x < tiles) {
-    reg_alloc_216();
+    row_warp_registers<ROW_WARPS_F>();
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t s_tmem = tm + lanes, p_tmem = tm + lanes + 128 + x * 64, o_tmem = tm + lanes + 256 + x * 128;
     const float cmul = p.sm_scale * LOG2E;
@@ -865,7 +1026,7 @@ attn_fwd_lse_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
           const float e1 = ex2(fmaf(__uint_as_float(sv[i + 1]), cmul, off));
           sum[c & 3] += e0;
           sum[(c + 2) & 3] += e1;
-          pk[c] = pack_rn<BF16>(e0, e1);
+          pk[c] = pack_prob<BF16>(e0, e1);
         }
         tmem_st32(p_tmem + 32 * hseg, pk);
       }
@@ -880,40 +1041,39 @@ attn_fwd_lse_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
       tc_fence_after_sync();
       const bool live = q_row < q_len;
       const float inv_l = 1.f / l, l2 = m + log2f(l);
-      if (live) {
-        if (p.splits > 1) p.part_lse[split_row] = l2;
-        else p.lse[row] = l2 * LN2;
-      }
+      if (q_row < p.Sq) (p.splits > 1 ? p.part_lse[split_row] : p.lse[row]) = live ? (p.splits > 1 ? l2 : l2 * LN2) : -INFINITY;
+      // the tile's scores are complete, so its q has been read for the last time: its place stages the results
+      uint8_t* st = smem + F_OFF_Q + x * TILE_BYTES + (warp & 3) * 8192;
+      const int row0 = q_row - lane, rows = max(0, min(32, p.Sq - row0));
+      float* part = p.part + (split_row - lane) * 128;
+      uint16_t* dst = out_ptr(p.o, b, h, row0);
 #pragma unroll 1
       for (int c = 0; c < 4; ++c) {
         uint32_t ov[32];
         tmem_ld32(o_tmem + c * 32, ov);
         tmem_wait_ld();
-        if (!live) continue;
-        if (p.splits > 1) {
-#pragma unroll
-          for (int i = 0; i < 32; i += 4)
-            *reinterpret_cast<float4*>(p.part + split_row * 128 + 32 * c + i) =
-                make_float4(__uint_as_float(ov[i]) * inv_l, __uint_as_float(ov[i + 1]) * inv_l, __uint_as_float(ov[i + 2]) * inv_l,
-                            __uint_as_float(ov[i + 3]) * inv_l);
-        } else {
-          store_row32<BF16>(out_ptr(p.o, b, h, q_row) + c * 32, ov, inv_l);
-        }
+        if (p.splits > 1) store_part32(st, ov, inv_l, live, part + 32 * c, rows);
+        else store_cols32<BF16>(st, ov, inv_l, live, dst + 32 * c, p.o.st, rows);
       }
-      if (!live) store_nothing();
     }
-  } else {
-    reg_dealloc_72();
-    store_nothing();
+  } else {  // a second tile without rows that exist: zeros for those of the tensor
+    other_warp_registers<ROW_WARPS_F>();
+    const int row0 = q_row - lane, rows = max(0, min(32, p.Sq - row0));
+    const uint4 z = make_uint4(0u, 0u, 0u, 0u);
+    for (int i = 0; i < rows; ++i) {
+      if (p.splits > 1) *reinterpret_cast<uint4*>(p.part + (split_row - lane + i) * 128 + lane * 4) = z;
+      else if (lane < 16) *reinterpret_cast<uint4*>(out_ptr(p.o, b, h, row0 + i) + lane * 8) = z;
+    }
+    if (lane < rows) (p.splits > 1 ? p.part_lse[split_row] : p.lse[row]) = -INFINITY;
   }
-  close_tmem(tm, warp, abort_flag, p.status);
+  close_tmem(tm, warp == W::tmem, abort_flag, p.status);
 }
 
 // ---- joins of split runs -------------------------------------------------------------------------------------------------
 // One thread = four channels of a row; the parts are added in the order of the splits.
 template <bool BF16>
 __device__ __forceinline__ void store4(uint16_t* dst, float4 v, float mul) {
-  *reinterpret_cast<uint2*>(dst) = make_uint2(pack_rn<BF16>(v.x * mul, v.y * mul), pack_rn<BF16>(v.z * mul, v.w * mul));
+  *reinterpret_cast<uint2*>(dst) = make_uint2(pack2_rn<BF16>(v.x * mul, v.y * mul), pack2_rn<BF16>(v.z * mul, v.w * mul));
 }
 template <bool BF16>
 __global__ void __launch_bounds__(256) attn_fwd_join_kernel(const TrainParams p) {
@@ -1041,7 +1201,7 @@ template <bool BF16>
 int run_forward(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const TrainParams& p, cudaStream_t st) {
   const dim3 grid(static_cast<unsigned>(tiles_of(p.Sq, 256)), static_cast<unsigned>(p.B * p.heads), static_cast<unsigned>(p.splits));
   DAX_CUDA(cudaFuncSetAttribute(attn_fwd_lse_kernel<BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, F_SMEM));
-  attn_fwd_lse_kernel<BF16><<<grid, THREADS, F_SMEM, st>>>(mq, mk, mv, p);
+  attn_fwd_lse_kernel<BF16><<<grid, Warps<ROW_WARPS_F>::threads, F_SMEM, st>>>(mq, mk, mv, p);
   DAX_CUDA(cudaGetLastError());
   if (p.splits > 1) {
     attn_fwd_join_kernel<BF16><<<static_cast<unsigned>(tiles_of(static_cast<int64_t>(p.B) * p.heads * p.Sq, 8)), 256, 0, st>>>(p);
@@ -1051,13 +1211,13 @@ int run_forward(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap&
 }
 
 template <bool BF16>
-int run_backward(const CUtensorMap& mq, const CUtensorMap& mdo, const CUtensorMap& mk, const CUtensorMap& mv, TrainParams p,
+int run_backward(const CUtensorMap& mq, const CUtensorMap& mdo, const CUtensorMap& mo, const CUtensorMap& mk, const CUtensorMap& mv, TrainParams p,
                  int s_q, int s_kv, float* part_q, float* part_kv, cudaStream_t st) {
   const unsigned BH = static_cast<unsigned>(p.B * p.heads);
   p.splits = s_q;
   p.part = part_q;
   DAX_CUDA(cudaFuncSetAttribute(attn_bwd_dq_kernel<BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, DQ_SMEM));
-  attn_bwd_dq_kernel<BF16><<<dim3(static_cast<unsigned>(tiles_of(p.Sq, 128)), BH, static_cast<unsigned>(s_q)), THREADS, DQ_SMEM, st>>>(mk, mv, p);
+  attn_bwd_dq_kernel<BF16><<<dim3(static_cast<unsigned>(tiles_of(p.Sq, 128)), BH, static_cast<unsigned>(s_q)), Warps<ROW_WARPS_B>::threads, DQ_SMEM, st>>>(mq, mdo, mo, mk, mv, p);
   DAX_CUDA(cudaGetLastError());
   if (s_q > 1) {
     const int64_t rows = static_cast<int64_t>(BH) * p.Sq;
@@ -1068,7 +1228,7 @@ int run_backward(const CUtensorMap& mq, const CUtensorMap& mdo, const CUtensorMa
   p.splits = s_kv;
   p.part = part_kv;
   DAX_CUDA(cudaFuncSetAttribute(attn_bwd_dkdv_kernel<BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, KV_SMEM));
-  attn_bwd_dkdv_kernel<BF16><<<dim3(static_cast<unsigned>(tiles_of(p.Sk, 128)), BH, static_cast<unsigned>(s_kv)), THREADS, KV_SMEM, st>>>(mq, mdo, mk, mv, p);
+  attn_bwd_dkdv_kernel<BF16><<<dim3(static_cast<unsigned>(tiles_of(p.Sk, 128)), BH, static_cast<unsigned>(s_kv)), Warps<ROW_WARPS_B>::threads, KV_SMEM, st>>>(mq, mdo, mk, mv, p);
   DAX_CUDA(cudaGetLastError());
   if (s_kv > 1) {
     const int64_t rows = static_cast<int64_t>(BH) * p.Sk;
@@ -1156,16 +1316,14 @@ int dax_attn_backward(const void* dout, const void* q, const void* k, const void
   DAX_REQUIRE(workspace != nullptr && workspace_bytes >= w.bytes, DAX_ERR_INVALID,
               "%s: workspace of %zu bytes is smaller than the %zu required", what, workspace_bytes, w.bytes);
   DAX_REQUIRE(aligned16(workspace), DAX_ERR_ALIGN, "%s: workspace must be 16-byte aligned", what);
-  CUtensorMap mq, mdo, mk, mv;
+  CUtensorMap mq, mdo, mo, mk, mv;
   DAX_TRY(make_map(&mq, q, q_strides, Sq, heads, B));
   DAX_TRY(make_map(&mdo, dout, do_strides, Sq, heads, B));
+  DAX_TRY(make_map(&mo, o, o_strides, Sq, heads, B));
   DAX_TRY(make_map(&mk, k, k_strides, Sk, heads, B));
   DAX_TRY(make_map(&mv, v, v_strides, Sk, heads, B));
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   TrainParams p{};
-  p.q = rows_of(q, q_strides);
-  p.o = rows_of(o, o_strides);
-  p.dout = rows_of(dout, do_strides);
   p.dq = rows_of(dq, dq_strides);
   p.dk = rows_of(dk, dk_strides);
   p.dv = rows_of(dv, dv_strides);
@@ -1185,8 +1343,8 @@ int dax_attn_backward(const void* dout, const void* q, const void* k, const void
   float* part_q = reinterpret_cast<float*>(ws + w.dq);
   float* part_kv = reinterpret_cast<float*>(ws + w.dkdv);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return dtype == DAX_BF16 ? run_backward<true>(mq, mdo, mk, mv, p, s_q, s_kv, part_q, part_kv, st)
-                           : run_backward<false>(mq, mdo, mk, mv, p, s_q, s_kv, part_q, part_kv, st);
+  return dtype == DAX_BF16 ? run_backward<true>(mq, mdo, mo, mk, mv, p, s_q, s_kv, part_q, part_kv, st)
+                           : run_backward<false>(mq, mdo, mo, mk, mv, p, s_q, s_kv, part_q, part_kv, st);
 }
 
 }  // extern "C"

@@ -73,7 +73,11 @@ def reference(q, k, v, do, q_lens, k_lens, c):
     b_D = (da * b_out).sum(3, keepdim=True) + 128 * W * (da * out.abs()).sum(3, keepdim=True)
     b_ds = torch.where(seen, (u + e) * ds.abs() + p * (128 * W * (da @ va.transpose(2, 3)) + b_D) * (1 + u) + tiny, 0.0)
     b_ds = torch.where(one, 0.0, b_ds)
-    b_dq = r(dq) + (1 + u) * c * (b_ds @ ka + Sk * W * (ds.abs() @ ka))
+    # dq is summed as r k - (sum of r) m with the rounded ds r and m the mean of the first (up to 128) keys; the exact ds of a
+    # row add up to zero, so an error of ds counts with its key's distance from m
+    first = (km & (torch.arange(Sk, device=DEV) < 128))[:, None, :, None].double()
+    m = (k * first).sum(2, keepdim=True) / first.sum(2, keepdim=True).clamp_min(1)
+    b_dq = r(dq) + (1 + u) * c * (b_ds @ torch.where(km[:, None, :, None], (k - m).abs(), 0.0) + (Sk + 300) * W * (ds.abs() @ (ka + m.abs())))
     b_dk = r(dk) + (1 + u) * c * (b_ds.transpose(2, 3) @ qa + Sq * W * (ds.abs().transpose(2, 3) @ qa))
     b_dv = r(dv) + (1 + u) * (((u + e + Sq * W) * p + tiny * seen).transpose(2, 3) @ da)
     b_lse = e[..., 0] + 2.0 ** -21 * (lse.abs().nan_to_num(posinf=0) + 1)
@@ -135,6 +139,12 @@ def test_padded_batches(ops, B, H, Sq, Sk, dtype, q_lens, k_lens, fill):
 def test_softmax_scale_and_peaked_rows(ops, scale):
     q, k, v, do = make(1, 2, 300, 400, "bf16", seed=3, offset=0.0)
     check(run(ops, q, k, v, do, sm_scale=scale), *reference(q, k, v, do, None, None, scale))
+
+
+def test_keys_far_from_zero(ops):
+    """An offset that all keys share has no part in dq; neither have the roundings of ds times that offset."""
+    q, k, v, do = make(1, 3, 300, 500, "bf16", seed=13, offset=20.0)
+    check(run(ops, q, k, v, do), *reference(q, k, v, do, None, None, 1 / math.sqrt(128)))
 
 
 def test_rising_maxima(ops):
