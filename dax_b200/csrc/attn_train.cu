@@ -62,37 +62,13 @@ template <int N> __device__ __forceinline__ void other_warp_registers() {
   else asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
 }
 
-// ---- rounding to the operands' type ------------------------------------------------------------------------------------
-// The conversion instructions run on the unit of the exponentials, which the kernels need for those.  bf16 is the upper
-// half of fp32, so rounding can be done on the other pipes and two results taken together with one byte permute.
-__device__ __forceinline__ uint32_t upper_halves(uint32_t a, uint32_t b) {
-  uint32_t r;
-  asm("prmt.b32 %0, %1, %2, 0x7632;" : "=r"(r) : "r"(a), "r"(b));
-  return r;
-}
-// Probabilities, never negative: add half a step of the kept part, in the integer pipe (a tie goes up).  The minimum, part
-// of the same instruction, keeps NaN (0x7fffffff) a NaN.
+// acc += both halves of a pair of rounded values
 template <bool BF16>
-__device__ __forceinline__ uint32_t pack_prob(float lo, float hi) {
+__device__ __forceinline__ void add_pair(float& acc, uint32_t w) {
   if constexpr (BF16)
-    return upper_halves(__viaddmin_u32(__float_as_uint(lo), 0x8000u, 0x7fffffffu), __viaddmin_u32(__float_as_uint(hi), 0x8000u, 0x7fffffffu));
-  else return pack2_rn<false>(lo, hi);
-}
-// Signed values, as a pair: with g = RN(65537 x), g + RN(x - g) is x rounded to its leading 8 bits (Veltkamp's splitting),
-// three fused-multiply-add-pipe instructions for two elements.  `hi` returns the rounded pair.
-template <bool BF16>
-__device__ __forceinline__ uint32_t pack_signed(uint64_t x, uint64_t& hi) {
-  if constexpr (BF16) {
-    const uint64_t g = f2_mul(x, f2_splat(65537.f));
-    hi = f2_add(g, f2_fma(g, f2_splat(-1.f), x));
-    float a, b;
-    f2_unpack(hi, a, b);
-    return upper_halves(__float_as_uint(a), __float_as_uint(b));
-  } else {
-    const uint32_t w = f2_to16_rn<false>(x);
-    hi = f2_from16<false>(w);
-    return w;
-  }
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tadd.rn.f32.bf16 %0, l, %0;\n\tadd.rn.f32.bf16 %0, h, %0;\n\t}" : "+f"(acc) : "r"(w));
+  else
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tadd.rn.f32.f16 %0, l, %0;\n\tadd.rn.f32.f16 %0, h, %0;\n\t}" : "+f"(acc) : "r"(w));
 }
 __device__ __forceinline__ uint64_t f2_bits(uint32_t lo, uint32_t hi) { return f2_pack(__uint_as_float(lo), __uint_as_float(hi)); }
 __device__ __forceinline__ int valid_len(const int* lens, int b, int S) { return lens != nullptr ? min(max(lens[b], 0), S) : S; }
@@ -246,8 +222,9 @@ __device__ __forceinline__ void close_tmem(uint32_t base, bool owner, volatile u
 
 // ---- dq ----------------------------------------------------------------------------------------------------------------
 // One CTA = 128 query rows of one head, walking over the tiles of keys.
-//   warps 0..15  one thread = one query row x 32 keys of the tile (warp / 4: which 32).  Sixteen warps and not eight: the
-//                exponentials and the rest alternate, and four warps per scheduler hide each other's waits
+//   warps 0..15  one thread = one query row x 32 keys of the tile (warp / 4: which 32).  Two teams of eight take turns with
+//                the exponentials (a token goes back and forth): one team's wait for the unit that computes them, the other's
+//                for the multiply-add pipe and for tensor memory, fall into each other
 //   producer     q, and do and o in the ring's last two slots; then k_0, v_0, k_1, ... through the ring, at last k's first tile
 //   issuer 0     s = q.k_j^T and dp = do.v_j^T        issuer 1     dq += ds.k_j
 // Tensor memory: s [0,128)  dp [128,256)  dq [256,384)  do [384,448)  ds [448,512).  do and ds are A operands in tensor
@@ -259,13 +236,14 @@ __device__ __forceinline__ void close_tmem(uint32_t base, bool owner, volatile u
 // dq, but the roundings of ds have: their sum times the offset would be the largest error by far.  The kernel adds up the
 // rounded ds of each row, e_i, and subtracts e_i m for an m near the mean key (the first tile's), which is what rounding
 // left of it.
-constexpr int DQ_SLOTS = 5;
+constexpr int DQ_SLOTS = 6;
 constexpr int DQ_OFF_Q = DQ_SLOTS * TILE_BYTES;
-constexpr int DQ_OFF_D = DQ_OFF_Q + TILE_BYTES;     // [4][128] floats: parts of D
-constexpr int DQ_OFF_E = DQ_OFF_D + 4 * 512;        // [4][128] floats: parts of e
-constexpr int DQ_OFF_MEAN = DQ_OFF_E + 4 * 512;     // [16][128] floats: sums of keys, in the end m in the first row
-constexpr int DQ_OFF_BAR = DQ_OFF_MEAN + 16 * 512;
+constexpr int DQ_OFF_E = DQ_OFF_Q;                  // [4][128] floats: parts of e      (q is no longer needed by then)
+constexpr int DQ_OFF_MEAN = DQ_OFF_Q + 2048;        // [16][128] floats: sums of keys, in the end m in the first row
+constexpr int DQ_OFF_D = DQ_OFF_Q + TILE_BYTES;     // [2][128] floats: parts of D
+constexpr int DQ_OFF_BAR = DQ_OFF_D + 1024;
 constexpr int DQ_SMEM = DQ_OFF_BAR + 256 + 1024;
+static_assert(DQ_SMEM <= 227 * 1024, "shared memory of the dq kernel");
 
 __device__ __forceinline__ void row_warps_sync() { asm volatile("bar.sync 1, 512;" ::: "memory"); }  // warps 0..15
 
@@ -312,7 +290,8 @@ attn_bwd_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
   uint64_t* dp_free = dp_full + 1;
   uint64_t* ds_full = dp_free + 1;
   uint64_t* dq_done = ds_full + 1;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(dq_done + 1);
+  uint64_t* turn = dq_done + 1;          // [2]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(turn + 2);
   volatile uint32_t* abort_flag = tmem_slot + 1;
   uint8_t* do_smem = smem + (DQ_SLOTS - 2) * TILE_BYTES;
   uint8_t* o_smem = smem + (DQ_SLOTS - 1) * TILE_BYTES;
@@ -338,6 +317,8 @@ attn_bwd_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
     mbar_init(dp_free, ROW_WARPS_B);
     mbar_init(ds_full, ROW_WARPS_B);
     mbar_init(dq_done, 1);
+    mbar_init(&turn[0], ROW_WARPS_B / 2);
+    mbar_init(&turn[1], ROW_WARPS_B / 2);
     *abort_flag = 0;
     mbar_fence_init();
     // the first loads are under way while tensor memory is set up
@@ -428,40 +409,47 @@ attn_bwd_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
       nl = l == -INFINITY ? -INFINITY : -l * LOG2E;
     }
     bool ok = mbar_wait(rows_full, 0, abort_flag);
-    {  // a quarter of a row of do to tensor memory, and its part of D
+    {  // a quarter of a row of do to tensor memory; the first two groups of warps compute half of D each
       uint32_t w[16];
-      float d = 0.f;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int at = (cg >> 1) * BOX_BYTES + r * 128 + ((((cg & 1) * 4 + i) ^ (r & 7)) << 4);
-        uint4 u = *reinterpret_cast<const uint4*>(do_smem + at), o = *reinterpret_cast<const uint4*>(o_smem + at);
-        if (!live) u = o = make_uint4(0u, 0u, 0u, 0u);
-        const uint32_t uw[4] = {u.x, u.y, u.z, u.w}, ow[4] = {o.x, o.y, o.z, o.w};
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          float a0, a1, o0, o1;
-          unpack2<BF16>(uw[k], a0, a1);
-          unpack2<BF16>(ow[k], o0, o1);
-          d = fmaf(a0, o0, d);
-          d = fmaf(a1, o1, d);
-          w[4 * i + k] = uw[k];
-        }
+        uint4 u = *reinterpret_cast<const uint4*>(do_smem + (cg >> 1) * BOX_BYTES + r * 128 + ((((cg & 1) * 4 + i) ^ (r & 7)) << 4));
+        if (!live) u = make_uint4(0u, 0u, 0u, 0u);
+        w[4 * i] = u.x; w[4 * i + 1] = u.y; w[4 * i + 2] = u.z; w[4 * i + 3] = u.w;
       }
       tmem_st16(tm + lanes + T_DO + cg * 16, w);
-      s_d[cg * 128 + r] = d;
+      if (cg < 2) {
+        float d[2] = {0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int at = cg * BOX_BYTES + r * 128 + ((i ^ (r & 7)) << 4);
+          const uint4 u = *reinterpret_cast<const uint4*>(do_smem + at), o = *reinterpret_cast<const uint4*>(o_smem + at);
+          const uint32_t uw[4] = {u.x, u.y, u.z, u.w}, ow[4] = {o.x, o.y, o.z, o.w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            float a0, a1, o0, o1;
+            unpack2<BF16>(uw[k], a0, a1);
+            unpack2<BF16>(ow[k], o0, o1);
+            d[0] = fmaf(a0, o0, d[0]);
+            d[1] = fmaf(a1, o1, d[1]);
+          }
+        }
+        s_d[cg * 128 + r] = live ? d[0] + d[1] : 0.f;
+      }
       tmem_wait_st();
       tc_fence_before_sync();
       __syncwarp();
       if (lane == 0) mbar_arrive(do_full);
     }
     ok = ok && mbar_wait(do_full, 0, abort_flag);  // all warps have arrived
-    const float nd = -((s_d[r] + s_d[128 + r]) + (s_d[256 + r] + s_d[384 + r]));
+    const float nd = -(s_d[r] + s_d[128 + r]);
     if (cg == 0 && split == 0) {
       stat[r] = nl;
       stat[stats + r] = nd;
     }
     const uint64_t nl2 = f2_splat(nl), nd2 = f2_splat(nd), cmul2 = f2_splat(p.sm_scale * LOG2E);
-    uint64_t e2 = f2_splat(0.f);  // sum of the rounded ds
+    float e[2] = {0.f, 0.f};  // sums of the rounded ds
+    const int team = warp >> 3;
     for (int j = 0; ok && j < n; ++j) {
       const int valid = k_len - (j0 + j) * 128 - cg * 32;  // this thread's columns that exist
       if (!(ok = mbar_wait(s_full, j & 1u, abort_flag))) break;
@@ -472,6 +460,8 @@ attn_bwd_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
       tc_fence_before_sync();
       __syncwarp();
       if (lane == 0) mbar_arrive(s_free);
+      // turn[0] opens the exponentials of team 0 (team 1 has done its last tile's), turn[1] those of team 1
+      if ((team == 1 || j > 0) && !(ok = mbar_wait(&turn[team], (team == 1 ? j : j - 1) & 1u, abort_flag))) break;
 #pragma unroll
       for (int i = 0; i < 32; i += 2) {
         float a, c;
@@ -479,6 +469,8 @@ attn_bwd_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
         sv[i] = __float_as_uint(ex2(a));
         sv[i + 1] = __float_as_uint(ex2(c));
       }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&turn[team ^ 1]);
       if (!(ok = mbar_wait(dp_full, j & 1u, abort_flag))) break;
       tc_fence_after_sync();
       uint32_t dp[32];
@@ -497,9 +489,8 @@ attn_bwd_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
       uint32_t pk[16];
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        uint64_t hi;
-        pk[i] = pack_signed<BF16>(f2_mul(f2_bits(sv[2 * i], sv[2 * i + 1]), f2_add(f2_bits(dp[2 * i], dp[2 * i + 1]), nd2)), hi);
-        e2 = f2_add(e2, hi);
+        pk[i] = f2_to16_rn<BF16>(f2_mul(f2_bits(sv[2 * i], sv[2 * i + 1]), f2_add(f2_bits(dp[2 * i], dp[2 * i + 1]), nd2)));
+        add_pair<BF16>(e[i & 1], pk[i]);
       }
       if (j > 0) {  // ds of the last tile has been read (normally long ago)
         if (!(ok = mbar_wait(dq_done, (j - 1) & 1u, abort_flag))) break;
@@ -530,6 +521,7 @@ attn_bwd_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
             m[2 * k + 1] += a1;
           }
         }
+      // s of the last tile is complete (this thread has its ds): q's place is free
       const float inv = 1.f / static_cast<float>(rows);
 #pragma unroll
       for (int k = 0; k < 8; ++k) m[k] = (m[k] + __shfl_xor_sync(0xffffffffu, m[k], 16)) * inv;
@@ -537,9 +529,7 @@ attn_bwd_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
         *reinterpret_cast<float4*>(s_mean + warp * 128 + chunk * 8) = make_float4(m[0], m[1], m[2], m[3]);
         *reinterpret_cast<float4*>(s_mean + warp * 128 + chunk * 8 + 4) = make_float4(m[4], m[5], m[6], m[7]);
       }
-      float a0, a1;
-      f2_unpack(e2, a0, a1);
-      s_e[cg * 128 + r] = a0 + a1;
+      s_e[cg * 128 + r] = e[0] + e[1];
       row_warps_sync();
       if (threadIdx.x < 128) {
         float t = 0.f;
@@ -788,8 +778,8 @@ attn_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
           x[1] = __float_as_uint(a1);
           x[2] = __float_as_uint(a2);
           x[3] = __float_as_uint(a3);
-          pk[k / 2] = pack_prob<BF16>(a0, a1);
-          pk[k / 2 + 1] = pack_prob<BF16>(a2, a3);
+          pk[k / 2] = pack2_rn<BF16>(a0, a1);
+          pk[k / 2 + 1] = pack2_rn<BF16>(a2, a3);
         }
         tmem_st8(tm + lanes + T_S + cg * 32 + 8 * c, pk);
         tmem_wait_st();
@@ -810,9 +800,8 @@ attn_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
           const ulonglong2 nd = stat[32 + 4 * c + k / 4];
           const uint32_t* x = &sv[16 * c + k];
           const uint32_t* y = &dp[16 * c + k];
-          uint64_t hi;
-          pk[k / 2] = pack_signed<BF16>(f2_mul(f2_bits(x[0], x[1]), f2_add(f2_bits(y[0], y[1]), nd.x)), hi);
-          pk[k / 2 + 1] = pack_signed<BF16>(f2_mul(f2_bits(x[2], x[3]), f2_add(f2_bits(y[2], y[3]), nd.y)), hi);
+          pk[k / 2] = f2_to16_rn<BF16>(f2_mul(f2_bits(x[0], x[1]), f2_add(f2_bits(y[0], y[1]), nd.x)));
+          pk[k / 2 + 1] = f2_to16_rn<BF16>(f2_mul(f2_bits(x[2], x[3]), f2_add(f2_bits(y[2], y[3]), nd.y)));
         }
         tmem_st8(tm + lanes + T_DP + cg * 32 + 8 * c, pk);
         tmem_wait_st();
@@ -1026,7 +1015,7 @@ attn_fwd_lse_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
           const float e1 = ex2(fmaf(__uint_as_float(sv[i + 1]), cmul, off));
           sum[c & 3] += e0;
           sum[(c + 2) & 3] += e1;
-          pk[c] = pack_prob<BF16>(e0, e1);
+          pk[c] = pack2_rn<BF16>(e0, e1);
         }
         tmem_st32(p_tmem + 32 * hseg, pk);
       }
