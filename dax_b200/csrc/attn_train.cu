@@ -1180,6 +1180,18 @@ int make_map(CUtensorMap* m, const void* t, const int64_t* st, int64_t S, int64_
 }
 inline Rows rows_of(const void* t, const int64_t* st) { return {t, st[0], st[1], st[2]}; }
 
+// The shared-memory limit of a kernel is set once per device (concurrent first calls set the same value).
+template <typename K, K kernel>
+int allow_smem(int bytes) {
+  static bool done[64] = {};
+  int dev = 0;
+  DAX_CUDA(cudaGetDevice(&dev));
+  if (dev < 64 && done[dev]) return DAX_OK;
+  DAX_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  if (dev < 64) done[dev] = true;
+  return DAX_OK;
+}
+
 #define DAX_TRY(expr)              \
   do {                             \
     const int rc__ = (expr);       \
@@ -1189,7 +1201,7 @@ inline Rows rows_of(const void* t, const int64_t* st) { return {t, st[0], st[1],
 template <bool BF16>
 int run_forward(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const TrainParams& p, cudaStream_t st) {
   const dim3 grid(static_cast<unsigned>(tiles_of(p.Sq, 256)), static_cast<unsigned>(p.B * p.heads), static_cast<unsigned>(p.splits));
-  DAX_CUDA(cudaFuncSetAttribute(attn_fwd_lse_kernel<BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, F_SMEM));
+  DAX_TRY((allow_smem<decltype(&attn_fwd_lse_kernel<BF16>), &attn_fwd_lse_kernel<BF16>>(F_SMEM)));
   attn_fwd_lse_kernel<BF16><<<grid, Warps<ROW_WARPS_F>::threads, F_SMEM, st>>>(mq, mk, mv, p);
   DAX_CUDA(cudaGetLastError());
   if (p.splits > 1) {
@@ -1205,7 +1217,7 @@ int run_backward(const CUtensorMap& mq, const CUtensorMap& mdo, const CUtensorMa
   const unsigned BH = static_cast<unsigned>(p.B * p.heads);
   p.splits = s_q;
   p.part = part_q;
-  DAX_CUDA(cudaFuncSetAttribute(attn_bwd_dq_kernel<BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, DQ_SMEM));
+  DAX_TRY((allow_smem<decltype(&attn_bwd_dq_kernel<BF16>), &attn_bwd_dq_kernel<BF16>>(DQ_SMEM)));
   attn_bwd_dq_kernel<BF16><<<dim3(static_cast<unsigned>(tiles_of(p.Sq, 128)), BH, static_cast<unsigned>(s_q)), Warps<ROW_WARPS_B>::threads, DQ_SMEM, st>>>(mq, mdo, mo, mk, mv, p);
   DAX_CUDA(cudaGetLastError());
   if (s_q > 1) {
@@ -1216,7 +1228,7 @@ int run_backward(const CUtensorMap& mq, const CUtensorMap& mdo, const CUtensorMa
   }
   p.splits = s_kv;
   p.part = part_kv;
-  DAX_CUDA(cudaFuncSetAttribute(attn_bwd_dkdv_kernel<BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, KV_SMEM));
+  DAX_TRY((allow_smem<decltype(&attn_bwd_dkdv_kernel<BF16>), &attn_bwd_dkdv_kernel<BF16>>(KV_SMEM)));
   attn_bwd_dkdv_kernel<BF16><<<dim3(static_cast<unsigned>(tiles_of(p.Sk, 128)), BH, static_cast<unsigned>(s_kv)), Warps<ROW_WARPS_B>::threads, KV_SMEM, st>>>(mq, mdo, mk, mv, p);
   DAX_CUDA(cudaGetLastError());
   if (s_kv > 1) {

@@ -410,13 +410,39 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mode: str = "bf
 # ---- training: operators with a gradient ---------------------------------------------------------------------------------
 # The backward passes recompute what they need from the inputs and the row statistics that the forward passes return.
 # Workspaces come from torch for every call (nothing is shared between calls, streams or captured graphs).
+class _OnDevice:
+    """Makes a device the current one for a call, if it is not (``torch.cuda.device`` costs as much as a launch)."""
+
+    __slots__ = ("index", "previous")
+
+    def __init__(self, index: int):
+        self.index = index
+
+    def __enter__(self) -> int:
+        """The raw handle of the device's current stream."""
+        self.previous = torch.cuda.current_device()
+        if self.previous != self.index:
+            torch.cuda.set_device(self.index)
+        return torch._C._cuda_getCurrentRawStream(self.index)
+
+    def __exit__(self, *exc) -> None:
+        if self.previous != self.index:
+            torch.cuda.set_device(self.previous)
+
+
 def _on_one_device(what: str, *ts) -> torch.device:
     """The device all tensors live on (the call goes to that device's current stream)."""
-    _need_cuda(*ts)
-    devs = {t.device for t in ts if t is not None}
-    if len(devs) != 1:
-        raise ValueError(f"{what}: tensors are on different devices: {sorted(map(str, devs))}")
-    return devs.pop()
+    dev = None
+    for t in ts:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            _need_cuda(t)
+        if dev is None:
+            dev = t.device
+        elif t.device != dev:
+            raise ValueError(f"{what}: tensors are on different devices, {dev} and {t.device}")
+    return dev
 
 
 def _rows3(t: torch.Tensor) -> torch.Tensor:
@@ -472,13 +498,14 @@ def layernorm_modulate(x: torch.Tensor, *, eps: float = 1e-6, ln_weight: Optiona
     _modulation(what, "scale", scale, x)
     dev = _on_one_device(what, x, ln_weight, ln_bias, shift, scale)
     y = torch.empty(x.shape, dtype=x.dtype, device=dev)
-    mean, rstd = torch.empty((2, *x.shape[:-1]), dtype=torch.float32, device=dev).unbind(0)
+    mean = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev)
+    rstd = torch.empty_like(mean)
     x3 = _rows3(x)
-    with torch.cuda.device(dev):
+    with _OnDevice(dev.index) as stream:
         tok = TRACE.begin(what)
         check(load().dax_layernorm_modulate(x3.data_ptr(), _dt(x.dtype), B, S, D, *_row_strides(x3), _ptr(ln_weight),
                                             _ptr(ln_bias), _ptr(shift), _ptr(scale), float(eps), y.data_ptr(), S * D, D,
-                                            mean.data_ptr(), rstd.data_ptr(), _stream()))
+                                            mean.data_ptr(), rstd.data_ptr(), stream))
         TRACE.end(tok, (B, S, D))
     return y, mean, rstd
 
@@ -501,9 +528,9 @@ def layernorm_modulate_backward(dy: torch.Tensor, x: torch.Tensor, mean: torch.T
     dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
     dweight = torch.empty_like(ln_weight) if need_params and ln_weight is not None else None
     dbias = torch.empty_like(ln_bias) if need_params and ln_bias is not None else None
-    dshift, dscale = torch.empty((2, *scale.shape), dtype=torch.float32, device=dev).unbind(0) if need_params and scale is not None else (None, None)
+    dshift, dscale = (torch.empty_like(scale), torch.empty_like(scale)) if need_params and scale is not None else (None, None)
     x3, dy3 = _rows3(x), _rows3(dy)
-    with torch.cuda.device(dev):
+    with _OnDevice(dev.index) as stream:
         lib, dt = load(), _dt(x.dtype)
         n = lib.dax_norm_backward_workspace_bytes(B, S, D, dt) if dweight is not None or dscale is not None else 0
         ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
@@ -511,7 +538,7 @@ def layernorm_modulate_backward(dy: torch.Tensor, x: torch.Tensor, mean: torch.T
         check(lib.dax_layernorm_modulate_backward(dy3.data_ptr(), x3.data_ptr(), dt, B, S, D, *_row_strides(dy3), *_row_strides(x3),
                                                   mean.data_ptr(), rstd.data_ptr(), _ptr(ln_weight), _ptr(ln_bias), _ptr(scale),
                                                   dx.data_ptr(), S * D, D, _ptr(dweight), _ptr(dbias), _ptr(dshift), _ptr(dscale),
-                                                  _ptr(ws), n, _stream()))
+                                                  _ptr(ws), n, stream))
         TRACE.end(tok, (B, S, D))
     return dx, dweight, dbias, dshift, dscale
 
@@ -540,10 +567,10 @@ def rmsnorm_rope(x: torch.Tensor, norm_weight: Optional[torch.Tensor] = None, *,
     y = torch.empty(x.shape, dtype=x.dtype, device=dev)
     rstd = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev)
     x3 = _rows3(x)
-    with torch.cuda.device(dev):
+    with _OnDevice(dev.index) as stream:
         tok = TRACE.begin(what)
         check(load().dax_rmsnorm_rope(x3.data_ptr(), _dt(x.dtype), B, S, D, *_row_strides(x3), _ptr(norm_weight), _ptr(rope_cos),
-                                      _ptr(rope_sin), float(eps), y.data_ptr(), S * D, D, rstd.data_ptr(), _stream()))
+                                      _ptr(rope_sin), float(eps), y.data_ptr(), S * D, D, rstd.data_ptr(), stream))
         TRACE.end(tok, (B, S, D))
     return y, rstd
 
@@ -563,14 +590,14 @@ def rmsnorm_rope_backward(dy: torch.Tensor, x: torch.Tensor, rstd: torch.Tensor,
     dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
     dweight = torch.empty_like(norm_weight) if need_params and norm_weight is not None else None
     x3, dy3 = _rows3(x), _rows3(dy)
-    with torch.cuda.device(dev):
+    with _OnDevice(dev.index) as stream:
         lib, dt = load(), _dt(x.dtype)
         n = lib.dax_norm_backward_workspace_bytes(B, S, D, dt) if dweight is not None else 0
         ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
         tok = TRACE.begin(what)
         check(lib.dax_rmsnorm_rope_backward(dy3.data_ptr(), x3.data_ptr(), dt, B, S, D, *_row_strides(dy3), *_row_strides(x3),
                                             rstd.data_ptr(), _ptr(norm_weight), _ptr(rope_cos), _ptr(rope_sin), dx.data_ptr(), S * D, D,
-                                            _ptr(dweight), _ptr(ws), n, _stream()))
+                                            _ptr(dweight), _ptr(ws), n, stream))
         TRACE.end(tok, (B, S, D))
     return dx, dweight
 
@@ -578,9 +605,15 @@ def rmsnorm_rope_backward(dy: torch.Tensor, x: torch.Tensor, rstd: torch.Tensor,
 def _heads_view(t: torch.Tensor) -> Tuple[torch.Tensor, I64x3]:
     """``t [B, heads, S, 128]`` and its strides for the kernels; a tensor they cannot address (channels not contiguous,
     broadcast dimensions, misaligned) is copied into token-major memory."""
-    if t.stride(3) != 1 or t.data_ptr() % 16 or any(n > 1 and (st <= 0 or st % 8) for n, st in zip(t.shape, t.stride()[:3])):
+    s0, s1, s2, s3 = t.stride()
+    if s3 == 1 and s0 > 0 and s1 > 0 and s2 > 0 and (s0 | s1 | s2) % 8 == 0 and t.data_ptr() % 16 == 0:
+        return t, I64x3(s0, s1, s2)
+    # a dimension of one may have any stride: the kernels get a valid one
+    st = [st if n > 1 else 128 for n, st in zip(t.shape, (s0, s1, s2))]
+    if s3 != 1 or t.data_ptr() % 16 or any(v <= 0 or v % 8 for v in st):
         t = _token_major(t).copy_(t)
-    return t, I64x3(*(st if n > 1 else 128 for n, st in zip(t.shape, t.stride()[:3])))  # a dimension of one: any valid stride
+        st = t.stride()[:3]
+    return t, I64x3(*st)
 
 
 def _attention_inputs(what: str, q, k, v, q_lens, k_lens, sm_scale, *more) -> Tuple[int, int, int, int, float, torch.device]:
@@ -603,8 +636,13 @@ def _attention_inputs(what: str, q, k, v, q_lens, k_lens, sm_scale, *more) -> Tu
 
 
 def _token_major(t: torch.Tensor) -> torch.Tensor:
+    """An uninitialised ``[B, heads, S, 128]`` tensor like ``t`` whose memory is ``[B, S, heads, 128]``."""
     B, heads, S, d = t.shape
-    return torch.empty((B, S, heads, d), dtype=t.dtype, device=t.device).transpose(1, 2)
+    return torch.empty_strided((B, heads, S, d), (S * heads * d, d, heads * d, 1), dtype=t.dtype, device=t.device)
+
+
+def _token_major_strides(heads: int, S: int) -> I64x3:
+    return I64x3(S * heads * 128, 128, heads * 128)
 
 
 def attention_lse(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, q_lens: Optional[torch.Tensor] = None,
@@ -622,14 +660,14 @@ def attention_lse(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, q_lens: 
     if Sk == 0:
         return out.zero_(), lse.fill_(-math.inf)
     (q, qs), (k, ks), (v, vs) = _heads_view(q), _heads_view(k), _heads_view(v)
-    with torch.cuda.device(dev):
+    with _OnDevice(dev.index) as stream:
         lib = load()
         n = lib.dax_attn_lse_workspace_bytes(B, heads, Sq, Sk)
         ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
         tok = TRACE.begin(what)
         check(lib.dax_attn_forward_lse(q.data_ptr(), k.data_ptr(), v.data_ptr(), _dt(q.dtype), B, heads, Sq, Sk, qs, ks, vs, sm_scale,
-                                       _ptr(q_lens), _ptr(k_lens), out.data_ptr(), _heads_view(out)[1], lse.data_ptr(),
-                                       _ptr(ws), n, _stream()))
+                                       _ptr(q_lens), _ptr(k_lens), out.data_ptr(), _token_major_strides(heads, Sq), lse.data_ptr(),
+                                       _ptr(ws), n, stream))
         TRACE.end(tok, (B, heads, Sq, Sk))
     return out, lse
 
@@ -650,14 +688,14 @@ def attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: 
     if lse.numel() == 0 or Sk == 0:
         return dq.zero_(), dk.zero_(), dv.zero_()
     (dout, dos), (q, qs), (k, ks), (v, vs), (out, os_) = map(_heads_view, (dout, q, k, v, out))
-    with torch.cuda.device(dev):
+    kv = _token_major_strides(heads, Sk)
+    with _OnDevice(dev.index) as stream:
         lib = load()
         n = lib.dax_attn_backward_workspace_bytes(B, heads, Sq, Sk)
         ws = torch.empty(n, dtype=torch.uint8, device=dev)
         tok = TRACE.begin(what)
         check(lib.dax_attn_backward(dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), _dt(q.dtype),
                                     B, heads, Sq, Sk, dos, qs, ks, vs, os_, sm_scale, _ptr(q_lens), _ptr(k_lens), dq.data_ptr(),
-                                    dk.data_ptr(), dv.data_ptr(), _heads_view(dq)[1], _heads_view(dk)[1],
-                                    _heads_view(dv)[1], ws.data_ptr(), n, _stream()))
+                                    dk.data_ptr(), dv.data_ptr(), _token_major_strides(heads, Sq), kv, kv, ws.data_ptr(), n, stream))
         TRACE.end(tok, (B, heads, Sq, Sk))
     return dq, dk, dv
