@@ -59,7 +59,7 @@ SIGNATURES = {
                                        I64x3, I64x3, c_float, c_int, c_int, c_void_p, c_size_t, c_void_p]),
     "dax_attn_forward": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_int64, I64x3, c_int64, c_int64,
                                  c_int64, c_int64, c_int, c_void_p, c_size_t, c_void_p]),
-    "dax_norm_backward_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int64, c_int]),
+    "dax_norm_backward_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int64]),
     "dax_layernorm_modulate": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_float, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p]),
     "dax_layernorm_modulate_backward": (c_int, [c_void_p, c_void_p, c_int, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
     "dax_rmsnorm_rope": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_float, c_void_p, c_int64, c_int64, c_void_p, c_void_p]),

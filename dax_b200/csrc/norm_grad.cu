@@ -10,11 +10,15 @@
 //               h = R_s^T dy, g = h w    dx = rstd (g - n mean(g n)),   dw = sum_{b, s} h n
 //
 // Bound by HBM: the forward pass reads x and writes y, the backward pass reads x and dy and writes dx, each once.  One
-// CTA owns a row at a time and walks over the rows of one sample; a thread owns the same 16-byte pieces of every row, so
+// CTA owns one or two rows at a time and walks over the rows of one sample; a thread owns the same 16-byte pieces of every
+// row, so
 //  - the rows travel through a ring in shared memory that each thread fills (cp.async) and reads back for itself: the
-//    bytes in flight cost neither registers nor barriers;
+//    bytes in flight cost neither registers nor barriers.  The backward pass reads a row from there twice, before and after
+//    its sums, because the registers are full of column sums;
 //  - the column sums over the CTA's rows stay in the thread's registers (fp32, rows in a fixed order) and reach memory
 //    once per CTA; a second kernel adds the CTAs' partial sums in a fixed order, so results do not depend on timing.
+// What a row costs beside its bytes is the wait for its sums (shuffles, one barrier): two rows share one where registers and
+// shared memory allow, and two to four CTAs per SM fill each other's waits.
 // Statistics, coefficients and sums are fp32; y and dx are rounded once, when they are stored.
 #include <algorithm>
 
@@ -23,8 +27,8 @@
 namespace dax {
 namespace {
 
-constexpr int kStages = 3;          // rows in the ring: one in use, two in flight
 constexpr int64_t kMaxWidth = 8192;
+constexpr int kMaxWarps = 10;         // of a CTA
 
 struct NormArgs {
   const uint8_t* x;       // input rows
@@ -92,21 +96,29 @@ __device__ __forceinline__ float warp_sum(float v) {
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
-// Sums of a pair of values over the CTA, the same number in every thread.  The caller alternates between two slots, so
-// one barrier per reduction is enough: a slot is written again only after the barrier of the reduction in between.
-__device__ __forceinline__ void cta_sum2(float& a, float& c, float2* slot) {
-  a = warp_sum(a);
-  c = warp_sum(c);
+// Sums of N values over the CTA, the same numbers in every thread.  `slots` (one per warp) may be written again after the
+// next barrier: callers alternate between two sets, so one barrier per reduction is enough.
+template <int N> struct alignas(N * 4) Sums { float v[N]; };
+template <int N>
+__device__ __forceinline__ void cta_sum(float (&v)[N], Sums<N>* slots) {
+#pragma unroll
+  for (int k = 0; k < N; ++k) v[k] = warp_sum(v[k]);
   const int warps = blockDim.x >> 5;
   if (warps == 1) return;
-  if ((threadIdx.x & 31) == 0) slot[threadIdx.x >> 5] = make_float2(a, c);
-  __syncthreads();
-  a = slot[0].x;
-  c = slot[0].y;
-  for (int k = 1; k < warps; ++k) {
-    a += slot[k].x;
-    c += slot[k].y;
+  if ((threadIdx.x & 31) == 0) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) slots[threadIdx.x >> 5].v[k] = v[k];
   }
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < N; ++k) v[k] = 0.f;
+#pragma unroll
+  for (int w = 0; w < kMaxWarps; ++w)
+    if (w < warps) {
+      const Sums<N> s = slots[w];
+#pragma unroll
+      for (int k = 0; k < N; ++k) v[k] += s.v[k];
+    }
 }
 
 // The rotary factors of this thread's pairs: a head has 128 channels and blockDim.x pieces are a whole number of heads,
@@ -123,12 +135,25 @@ __device__ __forceinline__ void load_rotary(const NormArgs& p, int64_t row, Rota
   }
 }
 
+// ---- launch shapes -----------------------------------------------------------------------------------------------------
+// ELEMS elements of a row per thread (8, 16 or 32, so NV pieces), at most T threads, at least MINB CTAs per SM (which bounds
+// the registers), R rows at a time, STAGES groups of rows in the ring.  Two rows at a time while the ring of two CTAs fits
+// the SM: not for fp32 and not for the widest rows.
+template <int DT, int ELEMS, bool BACKWARD> struct Shape {
+  static constexpr int NV = ELEMS / Piece<DT>::value;
+  static constexpr int T = ELEMS == 16 ? 320 : 256;
+  static constexpr int MINB = ELEMS == 8 ? 3 : 2;
+  static constexpr int R = DT != DAX_F32 && ELEMS <= 16 ? 2 : 1;
+  static constexpr int STAGES = BACKWARD ? 2 : 3;
+};
+
 // ---- forward ---------------------------------------------------------------------------------------------------------
-template <int DT, int NV, bool LN>
-__global__ void __launch_bounds__(512) norm_forward_kernel(const NormArgs p) {
-  constexpr int E = Piece<DT>::value;
-  extern __shared__ uint4 ring[];  // [kStages][NV][blockDim.x], then the coefficients
-  __shared__ float2 red[2][16];
+template <int DT, int ELEMS, bool LN>
+__global__ void __launch_bounds__(Shape<DT, ELEMS, false>::T, Shape<DT, ELEMS, false>::MINB) norm_forward_kernel(const NormArgs p) {
+  using Sh = Shape<DT, ELEMS, false>;
+  constexpr int E = Piece<DT>::value, NV = Sh::NV, R = Sh::R, STAGES = Sh::STAGES, N = LN ? 2 * R : R;
+  extern __shared__ uint4 ring[];  // [STAGES][R][NV][blockDim.x], then the coefficients
+  __shared__ Sums<N> red[2][kMaxWarps], red_c[2][kMaxWarps];
   const int T = blockDim.x, tid = threadIdx.x, b = blockIdx.y;
   const int pieces = p.D / E;
   const uint8_t* x = p.x + b * p.x_sb;
@@ -136,8 +161,25 @@ __global__ void __launch_bounds__(512) norm_forward_kernel(const NormArgs p) {
 
   // y = n mul + add per channel, folded once per CTA; a thread reads back only what it wrote: no barrier
   const bool coef = p.weight != nullptr || p.scale != nullptr;
-  float4* mul_s = reinterpret_cast<float4*>(ring + kStages * NV * T);
+  float4* mul_s = reinterpret_cast<float4*>(ring + STAGES * R * NV * T);
   float4* add_s = mul_s + NV * (E / 4) * T;
+
+  auto fetch = [&](int64_t row0, int stage) {
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+      if (row0 + r < p.S) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+          const int v = tid + i * T;
+          if (v < pieces) cp_async16(&ring[((stage * R + r) * NV + i) * T + tid], x + (row0 + r) * p.x_ss + v * 16);
+        }
+      }
+    cp_async_commit();  // one group per stage, empty past the end: the group count stays uniform
+  };
+  const int64_t step = static_cast<int64_t>(gridDim.x) * R;
+  int64_t row0 = static_cast<int64_t>(blockIdx.x) * R;
+#pragma unroll
+  for (int k = 0; k < STAGES - 1; ++k) fetch(row0 + k * step, k);
   if (coef) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -163,109 +205,123 @@ __global__ void __launch_bounds__(512) norm_forward_kernel(const NormArgs p) {
       }
     }
   }
-
-  auto fetch = [&](int64_t row, int stage) {
-    if (row < p.S) {
-#pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const int v = tid + i * T;
-        if (v < pieces) cp_async16(&ring[(stage * NV + i) * T + tid], x + row * p.x_ss + v * 16);
-      }
-    }
-    cp_async_commit();  // one group per row, empty past the end: the group count stays uniform
-  };
-  const int64_t step = gridDim.x;
-  int64_t row = blockIdx.x;
-#pragma unroll
-  for (int k = 0; k < kStages - 1; ++k) fetch(row + k * step, k);
   const float inv_d = 1.f / static_cast<float>(p.D);
-  int stage = 0;
-  for (; row < p.S; row += step) {
-    fetch(row + (kStages - 1) * step, stage == 0 ? kStages - 1 : stage - 1);
-    Rotary<DT> rot;
-    if (!LN && p.cos != nullptr) load_rotary<DT>(p, row, rot);
-    cp_async_wait<kStages - 1>();  // this thread's pieces of the row have landed
-    float f[NV][E];
-    float s0 = 0.f, s1 = 0.f;
+  int stage = 0, parity = 0;
+  for (; row0 < p.S; row0 += step) {
+    fetch(row0 + (STAGES - 1) * step, stage == 0 ? STAGES - 1 : stage - 1);
+    Rotary<DT> rot[R];
+    if (!LN && p.cos != nullptr) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      if (tid + i * T < pieces) {
-        unpack<DT>(ring[(stage * NV + i) * T + tid], f[i]);
-#pragma unroll
-        for (int k = 0; k < E; ++k) {
-          if (LN) s0 += f[i][k];
-          else s0 = fmaf(f[i][k], f[i][k], s0);
-        }
-      }
+      for (int r = 0; r < R; ++r)
+        if (row0 + r < p.S) load_rotary<DT>(p, row0 + r, rot[r]);
     }
-    cta_sum2(s0, s1, red[0]);
-    float mean = 0.f, var;
-    if (LN) {
-      // second pass around the first estimate of the mean: exact enough for rows whose mean dwarfs their spread, and
-      // it takes the rounding of that estimate out again (a constant row normalises to zero)
-      const float m0 = s0 * inv_d;
-      s0 = s1 = 0.f;
+    cp_async_wait<STAGES - 1>();  // this thread's pieces of the rows have landed
+    float f[R][NV][E];
+    float sum[N];
+#pragma unroll
+    for (int k = 0; k < N; ++k) sum[k] = 0.f;
+#pragma unroll
+    for (int r = 0; r < R; ++r)
 #pragma unroll
       for (int i = 0; i < NV; ++i)
-        if (tid + i * T < pieces) {
+        if (tid + i * T < pieces && row0 + r < p.S) {
+          unpack<DT>(ring[((stage * R + r) * NV + i) * T + tid], f[r][i]);
 #pragma unroll
           for (int k = 0; k < E; ++k) {
-            const float d = f[i][k] - m0;
-            s0 += d;
-            s1 = fmaf(d, d, s1);
+            sum[r] = fmaf(f[r][i][k], f[r][i][k], sum[r]);
+            if (LN) sum[R + (LN ? r : 0)] += f[r][i][k];
           }
         }
-      cta_sum2(s0, s1, red[1]);
-      const float dm = s0 * inv_d;
-      mean = m0 + dm;
-      var = fmaxf(fmaf(-dm, dm, s1 * inv_d), 0.f);
-    } else {
-      var = s0 * inv_d;
-      __syncthreads();  // the one slot in use is written again by the next row
+    cta_sum<N>(sum, red[parity]);
+    float mean[R], rstd[R];
+    bool centre = false;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      mean[r] = LN ? sum[R + (LN ? r : 0)] * inv_d : 0.f;
+      const float var = fmaf(-mean[r], mean[r], sum[r] * inv_d);
+      if (LN) centre = centre || !(var >= 4.f * mean[r] * mean[r]);
+      rstd[r] = rsqrtf(var + p.eps);
     }
-    const float rstd = rsqrtf(var + p.eps);
-    if (tid == 0) {
-      if (LN) p.mean[static_cast<int64_t>(b) * p.S + row] = mean;
-      p.rstd[static_cast<int64_t>(b) * p.S + row] = rstd;
+    if (LN && centre) {
+      // E[x^2] - mean^2 loses digits where the mean is not small against the spread (every thread sees the same numbers, so
+      // the branch is uniform): a second pass around the first estimate of the mean.  It takes the rounding of that
+      // estimate out as well, so that a constant row normalises to zero.
+#pragma unroll
+      for (int k = 0; k < N; ++k) sum[k] = 0.f;
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+          if (tid + i * T < pieces && row0 + r < p.S) {
+#pragma unroll
+            for (int k = 0; k < E; ++k) {
+              const float d = f[r][i][k] - mean[r];
+              sum[r] = fmaf(d, d, sum[r]);
+              sum[R + (LN ? r : 0)] += d;
+            }
+          }
+      cta_sum<N>(sum, red_c[parity]);
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const float dm = sum[R + (LN ? r : 0)] * inv_d;
+        mean[r] += dm;
+        rstd[r] = rsqrtf(fmaxf(fmaf(-dm, dm, sum[r] * inv_d), 0.f) + p.eps);
+      }
     }
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+      if (tid == r && row0 + r < p.S) {
+        if (LN) p.mean[static_cast<int64_t>(b) * p.S + row0 + r] = mean[r];
+        p.rstd[static_cast<int64_t>(b) * p.S + row0 + r] = rstd[r];
+      }
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       if (tid + i * T >= pieces) continue;
 #pragma unroll
-      for (int k = 0; k < E; ++k) f[i][k] = (f[i][k] - mean) * rstd;
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int k = 0; k < E; ++k) f[r][i][k] = LN ? (f[r][i][k] - mean[r]) * rstd[r] : f[r][i][k] * rstd[r];
       if (coef) {
 #pragma unroll
         for (int q = 0; q < E / 4; ++q) {
           const float4 m = mul_s[(i * (E / 4) + q) * T + tid];
           float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
           if (LN) a = add_s[(i * (E / 4) + q) * T + tid];
-          f[i][4 * q] = fmaf(f[i][4 * q], m.x, a.x);
-          f[i][4 * q + 1] = fmaf(f[i][4 * q + 1], m.y, a.y);
-          f[i][4 * q + 2] = fmaf(f[i][4 * q + 2], m.z, a.z);
-          f[i][4 * q + 3] = fmaf(f[i][4 * q + 3], m.w, a.w);
-        }
-      }
-      if (!LN && p.cos != nullptr) {
 #pragma unroll
-        for (int k = 0; k < E / 2; ++k) {
-          const float u = f[i][2 * k], w = f[i][2 * k + 1];
-          f[i][2 * k] = u * rot.c[k] - w * rot.s[k];
-          f[i][2 * k + 1] = fmaf(u, rot.s[k], w * rot.c[k]);
+          for (int r = 0; r < R; ++r) {
+            f[r][i][4 * q] = fmaf(f[r][i][4 * q], m.x, a.x);
+            f[r][i][4 * q + 1] = fmaf(f[r][i][4 * q + 1], m.y, a.y);
+            f[r][i][4 * q + 2] = fmaf(f[r][i][4 * q + 2], m.z, a.z);
+            f[r][i][4 * q + 3] = fmaf(f[r][i][4 * q + 3], m.w, a.w);
+          }
         }
       }
-      *reinterpret_cast<uint4*>(y + row * p.out_ss + (tid + i * T) * 16) = pack<DT>(f[i]);
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        if (!LN && p.cos != nullptr) {
+#pragma unroll
+          for (int k = 0; k < E / 2; ++k) {
+            const float u = f[r][i][2 * k], w = f[r][i][2 * k + 1];
+            f[r][i][2 * k] = u * rot[r].c[k] - w * rot[r].s[k];
+            f[r][i][2 * k + 1] = fmaf(u, rot[r].s[k], w * rot[r].c[k]);
+          }
+        }
+        if (row0 + r < p.S) *reinterpret_cast<uint4*>(y + (row0 + r) * p.out_ss + (tid + i * T) * 16) = pack<DT>(f[r][i]);
+      }
     }
-    stage = stage == kStages - 1 ? 0 : stage + 1;
+    stage = stage == STAGES - 1 ? 0 : stage + 1;
+    parity ^= 1;
   }
 }
 
 // ---- backward --------------------------------------------------------------------------------------------------------
 // SUMS: column sums kept (0: none wanted; LayerNorm 2: A and N; RMSNorm 1: N).
-template <int DT, int NV, bool LN, int SUMS>
-__global__ void __launch_bounds__(512) norm_backward_kernel(const NormArgs p) {
-  constexpr int E = Piece<DT>::value;
-  extern __shared__ uint4 ring[];  // [kStages][2][NV][blockDim.x], then the coefficients
-  __shared__ float2 red[2][16];
+template <int DT, int ELEMS, bool LN, int SUMS>
+__global__ void __launch_bounds__(Shape<DT, ELEMS, true>::T, Shape<DT, ELEMS, true>::MINB) norm_backward_kernel(const NormArgs p) {
+  using Sh = Shape<DT, ELEMS, true>;
+  constexpr int E = Piece<DT>::value, NV = Sh::NV, R = Sh::R, STAGES = Sh::STAGES, N = LN ? 2 * R : R;
+  extern __shared__ uint4 ring[];  // [STAGES][R][2][NV][blockDim.x], then the coefficients
+  __shared__ Sums<N> red[2][kMaxWarps];
   const int T = blockDim.x, tid = threadIdx.x, b = blockIdx.y;
   const int pieces = p.D / E;
   const uint8_t* x = p.x + b * p.x_sb;
@@ -274,8 +330,29 @@ __global__ void __launch_bounds__(512) norm_backward_kernel(const NormArgs p) {
   const float* mean_b = LN ? p.mean + static_cast<int64_t>(b) * p.S : nullptr;
   const float* rstd_b = p.rstd + static_cast<int64_t>(b) * p.S;
 
+  auto fetch = [&](int64_t row0, int stage) {
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+      if (row0 + r < p.S) {
+        uint4* at = &ring[(stage * R + r) * 2 * NV * T + tid];
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+          const int v = tid + i * T;
+          if (v < pieces) {
+            cp_async16(at + i * T, x + (row0 + r) * p.x_ss + v * 16);
+            cp_async16(at + (NV + i) * T, dy + (row0 + r) * p.dy_ss + v * 16);
+          }
+        }
+      }
+    cp_async_commit();
+  };
+  const int64_t step = static_cast<int64_t>(gridDim.x) * R;
+  int64_t row0 = static_cast<int64_t>(blockIdx.x) * R;
+#pragma unroll
+  for (int k = 0; k < STAGES - 1; ++k) fetch(row0 + k * step, k);
+
   const bool coef = p.weight != nullptr || p.scale != nullptr;  // g = dy mul
-  float4* mul_s = reinterpret_cast<float4*>(ring + kStages * 2 * NV * T);
+  float4* mul_s = reinterpret_cast<float4*>(ring + STAGES * R * 2 * NV * T);
   if (coef) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -294,20 +371,6 @@ __global__ void __launch_bounds__(512) norm_backward_kernel(const NormArgs p) {
       for (int q = 0; q < E / 4; ++q) mul_s[(i * (E / 4) + q) * T + tid] = *reinterpret_cast<float4*>(&m[4 * q]);
     }
   }
-
-  auto fetch = [&](int64_t row, int stage) {
-    if (row < p.S) {
-#pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const int v = tid + i * T;
-        if (v < pieces) {
-          cp_async16(&ring[(stage * 2 * NV + i) * T + tid], x + row * p.x_ss + v * 16);
-          cp_async16(&ring[((stage * 2 + 1) * NV + i) * T + tid], dy + row * p.dy_ss + v * 16);
-        }
-      }
-    }
-    cp_async_commit();
-  };
   float sum_n[SUMS > 0 ? NV : 1][E], sum_a[SUMS > 1 ? NV : 1][E];
 #pragma unroll
   for (int i = 0; i < NV; ++i)
@@ -317,76 +380,94 @@ __global__ void __launch_bounds__(512) norm_backward_kernel(const NormArgs p) {
       if (SUMS > 1) sum_a[SUMS > 1 ? i : 0][k] = 0.f;
     }
 
-  const int64_t step = gridDim.x;
-  int64_t row = blockIdx.x;
+  // n and g = (dy, rotated back) of piece i; `raw` is dy (rotated back) before the coefficients
+  auto piece = [&](int at, int i, float mean, float rstd, const Rotary<DT>& rot, float (&n)[E], float (&raw)[E], float (&g)[E]) {
+    unpack<DT>(ring[at + i * T], n);
+    unpack<DT>(ring[at + (NV + i) * T], raw);
+    if (!LN && p.cos != nullptr) {
 #pragma unroll
-  for (int k = 0; k < kStages - 1; ++k) fetch(row + k * step, k);
+      for (int k = 0; k < E / 2; ++k) {
+        const float u = raw[2 * k], w = raw[2 * k + 1];
+        raw[2 * k] = fmaf(u, rot.c[k], w * rot.s[k]);
+        raw[2 * k + 1] = w * rot.c[k] - u * rot.s[k];
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < E; ++k) {
+      n[k] = LN ? (n[k] - mean) * rstd : n[k] * rstd;
+      g[k] = raw[k];
+    }
+    if (coef) {
+#pragma unroll
+      for (int q = 0; q < E / 4; ++q) {
+        const float4 m = mul_s[(i * (E / 4) + q) * T + tid];
+        g[4 * q] *= m.x;
+        g[4 * q + 1] *= m.y;
+        g[4 * q + 2] *= m.z;
+        g[4 * q + 3] *= m.w;
+      }
+    }
+  };
+
   const float inv_d = 1.f / static_cast<float>(p.D);
   int stage = 0, parity = 0;
-  // the statistics of a row are read one row ahead
-  float mean_next = 0.f, rstd_next = 0.f;
-  if (row < p.S) {
-    if (LN) mean_next = mean_b[row];
-    rstd_next = rstd_b[row];
-  }
-  for (; row < p.S; row += step) {
-    fetch(row + (kStages - 1) * step, stage == 0 ? kStages - 1 : stage - 1);
-    const float mean = mean_next, rstd = rstd_next;
-    if (row + step < p.S) {
-      if (LN) mean_next = mean_b[row + step];
-      rstd_next = rstd_b[row + step];
+  // the statistics of the rows are read one group ahead
+  float mean_next[R], rstd_next[R];
+  auto statistics = [&](int64_t row) {
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      mean_next[r] = LN && row + r < p.S ? mean_b[row + r] : 0.f;
+      rstd_next[r] = row + r < p.S ? rstd_b[row + r] : 0.f;
     }
-    Rotary<DT> rot;
-    if (!LN && p.cos != nullptr) load_rotary<DT>(p, row, rot);
-    cp_async_wait<kStages - 1>();
-    float n[NV][E], g[NV][E];
-    float s_g = 0.f, s_gn = 0.f;
+  };
+  statistics(row0);
+  for (; row0 < p.S; row0 += step) {
+    fetch(row0 + (STAGES - 1) * step, stage == 0 ? STAGES - 1 : stage - 1);
+    float mean[R], rstd[R], sum[N];
+    Rotary<DT> rot[R];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      if (tid + i * T >= pieces) continue;
-      unpack<DT>(ring[(stage * 2 * NV + i) * T + tid], n[i]);
-      unpack<DT>(ring[((stage * 2 + 1) * NV + i) * T + tid], g[i]);
-      if (!LN && p.cos != nullptr) {  // rotate the gradient back
+    for (int r = 0; r < R; ++r) {
+      mean[r] = mean_next[r];
+      rstd[r] = rstd_next[r];
+      if (!LN && p.cos != nullptr && row0 + r < p.S) load_rotary<DT>(p, row0 + r, rot[r]);
+    }
+    statistics(row0 + step);
 #pragma unroll
-        for (int k = 0; k < E / 2; ++k) {
-          const float u = g[i][2 * k], w = g[i][2 * k + 1];
-          g[i][2 * k] = fmaf(u, rot.c[k], w * rot.s[k]);
-          g[i][2 * k + 1] = w * rot.c[k] - u * rot.s[k];
+    for (int k = 0; k < N; ++k) sum[k] = 0.f;
+    cp_async_wait<STAGES - 1>();
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      if (row0 + r >= p.S) continue;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        if (tid + i * T >= pieces) continue;
+        float n[E], raw[E], g[E];
+        piece((stage * R + r) * 2 * NV * T + tid, i, mean[r], rstd[r], rot[r], n, raw, g);
+#pragma unroll
+        for (int k = 0; k < E; ++k) {
+          if (SUMS > 0) sum_n[SUMS > 0 ? i : 0][k] = fmaf(raw[k], n[k], sum_n[SUMS > 0 ? i : 0][k]);
+          if (SUMS > 1) sum_a[SUMS > 1 ? i : 0][k] += raw[k];
+          sum[r] = fmaf(g[k], n[k], sum[r]);
+          if (LN) sum[R + (LN ? r : 0)] += g[k];
         }
       }
+    }
+    cta_sum<N>(sum, red[parity]);
 #pragma unroll
-      for (int k = 0; k < E; ++k) {
-        n[i][k] = (n[i][k] - mean) * rstd;
-        if (SUMS > 0) sum_n[SUMS > 0 ? i : 0][k] = fmaf(g[i][k], n[i][k], sum_n[SUMS > 0 ? i : 0][k]);
-        if (SUMS > 1) sum_a[SUMS > 1 ? i : 0][k] += g[i][k];
-      }
-      if (coef) {
+    for (int r = 0; r < R; ++r) {
+      if (row0 + r >= p.S) continue;
+      const float m_gn = sum[r] * inv_d, m_g = LN ? sum[R + (LN ? r : 0)] * inv_d : 0.f;
 #pragma unroll
-        for (int q = 0; q < E / 4; ++q) {
-          const float4 m = mul_s[(i * (E / 4) + q) * T + tid];
-          g[i][4 * q] *= m.x;
-          g[i][4 * q + 1] *= m.y;
-          g[i][4 * q + 2] *= m.z;
-          g[i][4 * q + 3] *= m.w;
-        }
-      }
+      for (int i = 0; i < NV; ++i) {
+        if (tid + i * T >= pieces) continue;
+        float n[E], raw[E], g[E];
+        piece((stage * R + r) * 2 * NV * T + tid, i, mean[r], rstd[r], rot[r], n, raw, g);
 #pragma unroll
-      for (int k = 0; k < E; ++k) {
-        if (LN) s_g += g[i][k];
-        s_gn = fmaf(g[i][k], n[i][k], s_gn);
+        for (int k = 0; k < E; ++k) g[k] = (fmaf(-n[k], m_gn, g[k]) - m_g) * rstd[r];
+        *reinterpret_cast<uint4*>(dx + (row0 + r) * p.out_ss + (tid + i * T) * 16) = pack<DT>(g);
       }
     }
-    cta_sum2(s_g, s_gn, red[parity]);
-    const float m_g = s_g * inv_d, m_gn = s_gn * inv_d;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      if (tid + i * T >= pieces) continue;
-      float o[E];
-#pragma unroll
-      for (int k = 0; k < E; ++k) o[k] = (fmaf(-n[i][k], m_gn, g[i][k]) - (LN ? m_g : 0.f)) * rstd;
-      *reinterpret_cast<uint4*>(dx + row * p.out_ss + (tid + i * T) * 16) = pack<DT>(o);
-    }
-    stage = stage == kStages - 1 ? 0 : stage + 1;
+    stage = stage == STAGES - 1 ? 0 : stage + 1;
     parity ^= 1;
   }
   if constexpr (SUMS > 0) {
@@ -402,7 +483,7 @@ __global__ void __launch_bounds__(512) norm_backward_kernel(const NormArgs p) {
 }
 
 // ---- column sums over the CTAs ---------------------------------------------------------------------------------------
-// A block owns 32 channels: 16 thread rows add every 16th partial sum, then one row adds the 16 results, always in the
+// A block owns 32 channels: 32 thread rows add every 32nd partial sum, then one row adds the 32 results, always in the
 // same order.
 struct JoinArgs {
   const float* part;  // [B, ctas, SUMS, D]
@@ -416,31 +497,37 @@ struct JoinArgs {
   int B, ctas, D;
 };
 template <int SUMS>
-__global__ void __launch_bounds__(512) norm_join_kernel(const JoinArgs p) {
-  __shared__ float sm[2][16][33];
+__global__ void __launch_bounds__(1024) norm_join_kernel(const JoinArgs p) {
+  __shared__ float sm[2][32][33];
   const int tx = threadIdx.x, ty = threadIdx.y;
   const int n = blockIdx.x * 32 + tx;
   const bool in = n < p.D;
+  const int64_t stride = static_cast<int64_t>(SUMS) * p.D;
   float dw = 0.f, dc = 0.f;
   for (int b = 0; b < p.B; ++b) {
     float s_n = 0.f, s_a = 0.f;
     if (in) {
-      const float* q = p.part + static_cast<int64_t>(b) * p.ctas * SUMS * p.D + n;
-      for (int c = ty; c < p.ctas; c += 16) {
-        s_n += q[static_cast<int64_t>(c) * SUMS * p.D];
-        if (SUMS > 1) s_a += q[static_cast<int64_t>(c) * SUMS * p.D + p.D];
+      const float* q = p.part + b * p.ctas * stride + n;
+#pragma unroll 4
+      for (int c = ty; c < p.ctas; c += 32) {
+        s_n += q[c * stride];
+        if (SUMS > 1) s_a += q[c * stride + p.D];
       }
     }
     __syncthreads();
     sm[0][ty][tx] = s_n;
-    sm[1][ty][tx] = s_a;
+    if (SUMS > 1) sm[1][ty][tx] = s_a;
+    __syncthreads();
+    if (ty < SUMS) {  // one thread row for each kind of sum
+      float t = 0.f;
+#pragma unroll
+      for (int k = 0; k < 32; ++k) t += sm[ty][k][tx];
+      sm[ty][0][tx] = t;
+    }
     __syncthreads();
     if (ty == 0 && in) {
-      s_n = s_a = 0.f;
-      for (int k = 0; k < 16; ++k) {
-        s_n += sm[0][k][tx];
-        s_a += sm[1][k][tx];
-      }
+      s_n = sm[0][0][tx];
+      s_a = SUMS > 1 ? sm[1][0][tx] : 0.f;
       const int64_t at = static_cast<int64_t>(b) * p.D + n;
       const float m = p.scale != nullptr ? 1.f + p.scale[at] : 1.f;
       if (p.dshift != nullptr) p.dshift[at] = s_a;
@@ -458,55 +545,52 @@ __global__ void __launch_bounds__(512) norm_join_kernel(const JoinArgs p) {
   }
 }
 
-// ---- launch shapes -----------------------------------------------------------------------------------------------------
-// Pieces per thread: one up to 256 pieces per row (threads beyond that add barrier time), two up to 640, else four.
-struct RowShape { int nv, threads; };
-inline RowShape row_shape(int64_t D, int dtype) {
-  const int64_t pieces = D * dtype_bytes(dtype) / 16;
-  const int nv = pieces <= 256 ? 1 : (pieces <= 640 ? 2 : 4);
-  const int64_t threads = ((pieces + nv - 1) / nv + 31) / 32 * 32;
-  return {nv, static_cast<int>(threads)};
-}
-// CTAs that stay resident and stride over the rows, over all samples: what fits on the GPU at once, and no more than 1024
-// threads or 16 CTAs per SM (more adds nothing to the bytes in flight, but partial sums to join).
+// ---- host ----------------------------------------------------------------------------------------------------------------
+// Elements of a row per thread: 8 while that makes at most 256 threads, 16 up to 320, else 32 (more threads only add to
+// the barrier; fewer hold the rows of narrow tensors too long).
+inline int row_elems(int64_t D) { return D <= 2048 ? 8 : (D <= 5120 ? 16 : 32); }
+inline int row_threads(int64_t D) { return static_cast<int>((D / row_elems(D) + (D % row_elems(D) != 0) + 31) / 32 * 32); }
+// CTAs that stay resident and stride over the rows, over all samples: at most what fits on the GPU at once and eight per SM
+// (more adds nothing to the bytes in flight, but partial sums to join).
 inline int64_t max_ctas(int64_t B, int64_t S, int threads) {
-  const int64_t per_sm = std::min<int64_t>(16, std::max<int64_t>(1, 1024 / threads));
+  const int64_t per_sm = std::min<int64_t>(8, std::max<int64_t>(1, 2048 / threads));
   return std::min(S, std::max<int64_t>(1, per_sm * sm_count() / B));
 }
 
 template <typename K>
-int launch_rows(K kernel, const NormArgs& p, int64_t B, int threads, size_t smem, int64_t* ctas, cudaStream_t st) {
+int launch_rows(K kernel, const NormArgs& p, int64_t B, int threads, size_t smem, int rows, int64_t* ctas, cudaStream_t st) {
   if (smem > 40 * 1024) DAX_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
   int per_sm = 0;
   DAX_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, threads, smem));
-  *ctas = std::min(max_ctas(B, p.S, threads), std::max<int64_t>(1, static_cast<int64_t>(per_sm) * sm_count() / B));
+  *ctas = std::min(max_ctas(B, (p.S + rows - 1) / rows, threads), std::max<int64_t>(1, static_cast<int64_t>(per_sm) * sm_count() / B));
   kernel<<<dim3(static_cast<unsigned>(*ctas), static_cast<unsigned>(B)), threads, smem, st>>>(p);
   DAX_CUDA(cudaGetLastError());
   return DAX_OK;
 }
 
-template <int DT, int NV, bool LN>
-int run_nv(const NormArgs& p, int64_t B, int threads, int64_t* ctas, int sums, bool backward, cudaStream_t st) {
-  constexpr size_t coef = static_cast<size_t>(Piece<DT>::value) * 4;  // bytes of one fp32 vector for a piece
-  const bool has_coef = p.weight != nullptr || p.scale != nullptr;
-  const size_t slots = static_cast<size_t>(NV) * threads;
+template <int DT, int ELEMS, bool LN>
+int run_shape(const NormArgs& p, int64_t B, int64_t* ctas, int sums, bool backward, cudaStream_t st) {
+  const int threads = row_threads(p.D);
+  const size_t coef = p.weight != nullptr || p.scale != nullptr ? static_cast<size_t>(threads) * ELEMS * 4 : 0;  // one fp32 vector
+  const size_t row = static_cast<size_t>(threads) * ELEMS * (DT == DAX_F32 ? 4 : 2);
   if (!backward) {
-    const size_t smem = slots * (kStages * 16 + (has_coef ? (LN ? 2 : 1) * coef : 0));
-    return launch_rows(norm_forward_kernel<DT, NV, LN>, p, B, threads, smem, ctas, st);
+    using Sh = Shape<DT, ELEMS, false>;
+    return launch_rows(norm_forward_kernel<DT, ELEMS, LN>, p, B, threads, row * Sh::STAGES * Sh::R + (LN ? 2 : 1) * coef, Sh::R, ctas, st);
   }
-  const size_t smem = slots * (kStages * 32 + (has_coef ? coef : 0));
-  if (sums == 0) return launch_rows(norm_backward_kernel<DT, NV, LN, 0>, p, B, threads, smem, ctas, st);
-  return launch_rows(norm_backward_kernel<DT, NV, LN, LN ? 2 : 1>, p, B, threads, smem, ctas, st);
+  using Sh = Shape<DT, ELEMS, true>;
+  const size_t smem = row * Sh::STAGES * Sh::R * 2 + coef;
+  if (sums == 0) return launch_rows(norm_backward_kernel<DT, ELEMS, LN, 0>, p, B, threads, smem, Sh::R, ctas, st);
+  return launch_rows(norm_backward_kernel<DT, ELEMS, LN, LN ? 2 : 1>, p, B, threads, smem, Sh::R, ctas, st);
 }
 
 template <bool LN>
 int run_rows(const NormArgs& p, int dtype, int64_t B, int64_t* ctas, int sums, bool backward, cudaStream_t st) {
-  const RowShape s = row_shape(p.D, dtype);
+  const int elems = row_elems(p.D);
 #define DAX_ROWS(DT, N) \
-  if (dtype == DT && s.nv == N) return run_nv<DT, N, LN>(p, B, s.threads, ctas, sums, backward, st)
-  DAX_ROWS(DAX_BF16, 1); DAX_ROWS(DAX_BF16, 2); DAX_ROWS(DAX_BF16, 4);
-  DAX_ROWS(DAX_F16, 1); DAX_ROWS(DAX_F16, 2); DAX_ROWS(DAX_F16, 4);
-  DAX_ROWS(DAX_F32, 1); DAX_ROWS(DAX_F32, 2); DAX_ROWS(DAX_F32, 4);
+  if (dtype == DT && elems == N) return run_shape<DT, N, LN>(p, B, ctas, sums, backward, st)
+  DAX_ROWS(DAX_BF16, 8); DAX_ROWS(DAX_BF16, 16); DAX_ROWS(DAX_BF16, 32);
+  DAX_ROWS(DAX_F16, 8); DAX_ROWS(DAX_F16, 16); DAX_ROWS(DAX_F16, 32);
+  DAX_ROWS(DAX_F32, 8); DAX_ROWS(DAX_F32, 16); DAX_ROWS(DAX_F32, 32);
 #undef DAX_ROWS
   return fail(DAX_ERR_UNSUPPORTED, "norm: dtype %d is not BF16/F16/F32", dtype);
 }
@@ -550,7 +634,7 @@ template <bool LN>
 int backward(const char* what, NormArgs p, JoinArgs j, int dtype, int64_t B, int64_t D, void* workspace, size_t bytes, cudaStream_t st) {
   const bool want = j.dweight != nullptr || j.dbias != nullptr || j.dshift != nullptr || j.dscale != nullptr;
   const int sums = want ? (LN ? 2 : 1) : 0;
-  int64_t ctas = B > 0 ? max_ctas(B, p.S, row_shape(D, dtype).threads) : 0;
+  int64_t ctas = B > 0 ? max_ctas(B, p.S, row_threads(D)) : 0;
   if (want) {
     const size_t need = static_cast<size_t>(B) * ctas * sums * D * 4;
     DAX_REQUIRE(bytes >= need && (need == 0 || workspace != nullptr), DAX_ERR_INVALID,
@@ -567,7 +651,7 @@ int backward(const char* what, NormArgs p, JoinArgs j, int dtype, int64_t B, int
     j.B = static_cast<int>(B);
     j.ctas = static_cast<int>(ctas);
     j.D = p.D;
-    norm_join_kernel<LN ? 2 : 1><<<static_cast<unsigned>((D + 31) / 32), dim3(32, 16), 0, st>>>(j);
+    norm_join_kernel<LN ? 2 : 1><<<static_cast<unsigned>((D + 31) / 32), dim3(32, 32), 0, st>>>(j);
     DAX_CUDA(cudaGetLastError());
   }
   return DAX_OK;
@@ -578,9 +662,9 @@ int backward(const char* what, NormArgs p, JoinArgs j, int dtype, int64_t B, int
 
 extern "C" {
 
-size_t dax_norm_backward_workspace_bytes(int64_t B, int64_t S, int64_t D, int dtype) {
-  if (B <= 0 || S <= 0 || D <= 0 || D > dax::kMaxWidth || dax::dtype_bytes(dtype) < 2) return 0;
-  return static_cast<size_t>(B) * dax::max_ctas(B, S, dax::row_shape(D, dtype).threads) * 2 * D * 4;
+size_t dax_norm_backward_workspace_bytes(int64_t B, int64_t S, int64_t D) {
+  if (B <= 0 || S <= 0 || D <= 0 || D > dax::kMaxWidth) return 0;
+  return static_cast<size_t>(B) * dax::max_ctas(B, S, dax::row_threads(D)) * 2 * D * 4;
 }
 
 int dax_layernorm_modulate(const void* x, int dtype, int64_t B, int64_t S, int64_t D, int64_t x_sb, int64_t x_ss,

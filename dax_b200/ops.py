@@ -532,7 +532,7 @@ def layernorm_modulate_backward(dy: torch.Tensor, x: torch.Tensor, mean: torch.T
     x3, dy3 = _rows3(x), _rows3(dy)
     with _OnDevice(dev.index) as stream:
         lib, dt = load(), _dt(x.dtype)
-        n = lib.dax_norm_backward_workspace_bytes(B, S, D, dt) if dweight is not None or dscale is not None else 0
+        n = lib.dax_norm_backward_workspace_bytes(B, S, D) if dweight is not None or dscale is not None else 0
         ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
         tok = TRACE.begin(what)
         check(lib.dax_layernorm_modulate_backward(dy3.data_ptr(), x3.data_ptr(), dt, B, S, D, *_row_strides(dy3), *_row_strides(x3),
@@ -592,7 +592,7 @@ def rmsnorm_rope_backward(dy: torch.Tensor, x: torch.Tensor, rstd: torch.Tensor,
     x3, dy3 = _rows3(x), _rows3(dy)
     with _OnDevice(dev.index) as stream:
         lib, dt = load(), _dt(x.dtype)
-        n = lib.dax_norm_backward_workspace_bytes(B, S, D, dt) if dweight is not None else 0
+        n = lib.dax_norm_backward_workspace_bytes(B, S, D) if dweight is not None else 0
         ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
         tok = TRACE.begin(what)
         check(lib.dax_rmsnorm_rope_backward(dy3.data_ptr(), x3.data_ptr(), dt, B, S, D, *_row_strides(dy3), *_row_strides(x3),

@@ -294,7 +294,7 @@ int dax_attn_forward_direct(const void* q, const void* k, const void* v, int dty
  * The parameter gradients are sums over all rows in a fixed order: equal inputs give equal bits.  `workspace` (16-byte
  * aligned, dax_norm_backward_workspace_bytes) holds partial sums; it may be NULL when no parameter gradient is wanted.
  * ------------------------------------------------------------------------------------------- */
-size_t dax_norm_backward_workspace_bytes(int64_t B, int64_t S, int64_t D, int dtype);
+size_t dax_norm_backward_workspace_bytes(int64_t B, int64_t S, int64_t D);
 
 int dax_layernorm_modulate(const void* x, int dtype, int64_t B, int64_t S, int64_t D, int64_t x_sb, int64_t x_ss,
                            const float* ln_weight, const float* ln_bias, const float* shift, const float* scale, float eps,
