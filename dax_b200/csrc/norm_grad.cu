@@ -28,7 +28,6 @@ namespace dax {
 namespace {
 
 constexpr int64_t kMaxWidth = 8192;
-constexpr int kMaxWarps = 10;         // of a CTA
 
 struct NormArgs {
   const uint8_t* x;       // input rows
@@ -49,9 +48,10 @@ struct NormArgs {
   float eps;
 };
 
-__device__ __forceinline__ void cp_async16(void* smem_dst, const void* gmem_src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(smem_dst))),
-               "l"(gmem_src) : "memory");
+// 16 bytes, or 16 zero bytes where there is nothing to read (then the address is not used)
+__device__ __forceinline__ void cp_async16(void* smem_dst, const void* gmem_src, bool valid) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(smem_dst))),
+               "l"(gmem_src), "r"(valid ? 16 : 0) : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -60,35 +60,55 @@ __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_gr
 // ---- 16-byte pieces: eight 16-bit or four fp32 elements ------------------------------------------------------------
 template <int DT> struct Piece { static constexpr int value = DT == DAX_F32 ? 4 : 8; };
 
+// All arithmetic runs on fp32 pairs: the kernels are closer to the bound of instruction issue than the bytes suggest.
+template <int DT> struct Pairs { uint64_t v[Piece<DT>::value / 2]; };
 template <int DT>
-__device__ __forceinline__ void unpack(const uint4& r, float (&f)[Piece<DT>::value]) {
+__device__ __forceinline__ Pairs<DT> unpack(const uint4& r) {
+  Pairs<DT> f;
   if constexpr (DT == DAX_F32) {
-    f[0] = __uint_as_float(r.x); f[1] = __uint_as_float(r.y); f[2] = __uint_as_float(r.z); f[3] = __uint_as_float(r.w);
+    f.v[0] = f2_pack(__uint_as_float(r.x), __uint_as_float(r.y));
+    f.v[1] = f2_pack(__uint_as_float(r.z), __uint_as_float(r.w));
   } else {
-    unpack2<DT == DAX_BF16>(r.x, f[0], f[1]);
-    unpack2<DT == DAX_BF16>(r.y, f[2], f[3]);
-    unpack2<DT == DAX_BF16>(r.z, f[4], f[5]);
-    unpack2<DT == DAX_BF16>(r.w, f[6], f[7]);
+    f.v[0] = f2_from16<DT == DAX_BF16>(r.x);
+    f.v[1] = f2_from16<DT == DAX_BF16>(r.y);
+    f.v[2] = f2_from16<DT == DAX_BF16>(r.z);
+    f.v[3] = f2_from16<DT == DAX_BF16>(r.w);
+  }
+  return f;
+}
+template <int DT>
+__device__ __forceinline__ uint4 pack(const Pairs<DT>& f) {
+  if constexpr (DT == DAX_F32) {
+    float a, b, c, d;
+    f2_unpack(f.v[0], a, b);
+    f2_unpack(f.v[1], c, d);
+    return make_uint4(__float_as_uint(a), __float_as_uint(b), __float_as_uint(c), __float_as_uint(d));
+  } else {
+    return make_uint4(f2_to16_rn<DT == DAX_BF16>(f.v[0]), f2_to16_rn<DT == DAX_BF16>(f.v[1]), f2_to16_rn<DT == DAX_BF16>(f.v[2]),
+                      f2_to16_rn<DT == DAX_BF16>(f.v[3]));
   }
 }
+// the channels of a piece of a per-channel fp32 vector
 template <int DT>
-__device__ __forceinline__ uint4 pack(const float (&f)[Piece<DT>::value]) {
-  if constexpr (DT == DAX_F32) {
-    return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
-  } else {
-    return make_uint4(pack2_rn<DT == DAX_BF16>(f[0], f[1]), pack2_rn<DT == DAX_BF16>(f[2], f[3]),
-                      pack2_rn<DT == DAX_BF16>(f[4], f[5]), pack2_rn<DT == DAX_BF16>(f[6], f[7]));
+__device__ __forceinline__ Pairs<DT> load_vector(const float* p) {
+  Pairs<DT> f;
+#pragma unroll
+  for (int k = 0; k < Piece<DT>::value / 4; ++k) {
+    const ulonglong2 u = *reinterpret_cast<const ulonglong2*>(p + 4 * k);
+    f.v[2 * k] = u.x;
+    f.v[2 * k + 1] = u.y;
   }
+  return f;
 }
-template <int N>
-__device__ __forceinline__ void load_f32(const float* p, float (&f)[N]) {
+template <int DT>
+__device__ __forceinline__ void store_vector(float* p, const Pairs<DT>& f) {
 #pragma unroll
-  for (int k = 0; k < N; k += 4) *reinterpret_cast<float4*>(&f[k]) = *reinterpret_cast<const float4*>(p + k);
+  for (int k = 0; k < Piece<DT>::value / 4; ++k) *reinterpret_cast<ulonglong2*>(p + 4 * k) = make_ulonglong2(f.v[2 * k], f.v[2 * k + 1]);
 }
-template <int N>
-__device__ __forceinline__ void store_f32(float* p, const float (&f)[N]) {
-#pragma unroll
-  for (int k = 0; k < N; k += 4) *reinterpret_cast<float4*>(p + k) = *reinterpret_cast<const float4*>(&f[k]);
+__device__ __forceinline__ float f2_sum(uint64_t p) {
+  float a, b;
+  f2_unpack(p, a, b);
+  return a + b;
 }
 
 __device__ __forceinline__ float warp_sum(float v) {
@@ -96,15 +116,14 @@ __device__ __forceinline__ float warp_sum(float v) {
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
-// Sums of N values over the CTA, the same numbers in every thread.  `slots` (one per warp) may be written again after the
-// next barrier: callers alternate between two sets, so one barrier per reduction is enough.
+// Sums of N values over the CTA, the same numbers in every thread.  `slots` (one per warp the CTA may have, those of absent
+// warps zero) may be written again after the next barrier: callers alternate between two sets, so one barrier per reduction
+// is enough.
 template <int N> struct alignas(N * 4) Sums { float v[N]; };
-template <int N>
+template <int N, int WARPS>
 __device__ __forceinline__ void cta_sum(float (&v)[N], Sums<N>* slots) {
 #pragma unroll
   for (int k = 0; k < N; ++k) v[k] = warp_sum(v[k]);
-  const int warps = blockDim.x >> 5;
-  if (warps == 1) return;
   if ((threadIdx.x & 31) == 0) {
 #pragma unroll
     for (int k = 0; k < N; ++k) slots[threadIdx.x >> 5].v[k] = v[k];
@@ -113,12 +132,11 @@ __device__ __forceinline__ void cta_sum(float (&v)[N], Sums<N>* slots) {
 #pragma unroll
   for (int k = 0; k < N; ++k) v[k] = 0.f;
 #pragma unroll
-  for (int w = 0; w < kMaxWarps; ++w)
-    if (w < warps) {
-      const Sums<N> s = slots[w];
+  for (int w = 0; w < WARPS; ++w) {
+    const Sums<N> s = slots[w];
 #pragma unroll
-      for (int k = 0; k < N; ++k) v[k] += s.v[k];
-    }
+    for (int k = 0; k < N; ++k) v[k] += s.v[k];
+  }
 }
 
 // The rotary factors of this thread's pairs: a head has 128 channels and blockDim.x pieces are a whole number of heads,
@@ -135,104 +153,127 @@ __device__ __forceinline__ void load_rotary(const NormArgs& p, int64_t row, Rota
   }
 }
 
+// Rotation of the piece's pairs by their angles (SIGN 1) or back (SIGN -1).
+template <int DT, int SIGN>
+__device__ __forceinline__ void rotate(Pairs<DT>& f, const Rotary<DT>& r) {
+#pragma unroll
+  for (int k = 0; k < Piece<DT>::value / 2; ++k) {
+    float u, w;
+    f2_unpack(f.v[k], u, w);
+    const float s = SIGN > 0 ? r.s[k] : -r.s[k];
+    f.v[k] = f2_pack(fmaf(u, r.c[k], -(w * s)), fmaf(w, r.c[k], u * s));
+  }
+}
+
 // ---- launch shapes -----------------------------------------------------------------------------------------------------
-// ELEMS elements of a row per thread (8, 16 or 32, so NV pieces), at most T threads, at least MINB CTAs per SM (which bounds
-// the registers), R rows at a time, STAGES groups of rows in the ring.  Two rows at a time while the ring of two CTAs fits
-// the SM: not for fp32 and not for the widest rows.
+// ELEMS elements of a row per thread (NV pieces), at most T threads, at least MINB CTAs per SM (which bounds the registers),
+// R rows at a time, STAGES groups of rows in the ring.  Two rows at a time while the ring of two CTAs fits the SM: not for
+// fp32 and not for the widest rows.
 template <int DT, int ELEMS, bool BACKWARD> struct Shape {
   static constexpr int NV = ELEMS / Piece<DT>::value;
-  static constexpr int T = ELEMS == 16 ? 320 : 256;
-  static constexpr int MINB = ELEMS == 8 ? 3 : 2;
+  static constexpr int T = ELEMS == 8 ? 128 : ELEMS == 16 ? 320 : 256;
+  static constexpr int WARPS = T / 32;
+  static constexpr int MINB = ELEMS == 8 ? 6 : 2;
   static constexpr int R = DT != DAX_F32 && ELEMS <= 16 ? 2 : 1;
   static constexpr int STAGES = BACKWARD ? 2 : 3;
 };
+
+// Pieces of a thread that lie behind the row's end, and rows behind the last one, are zeros in the ring: they add nothing to
+// any sum, so only stores ask whether they exist.
 
 // ---- forward ---------------------------------------------------------------------------------------------------------
 template <int DT, int ELEMS, bool LN>
 __global__ void __launch_bounds__(Shape<DT, ELEMS, false>::T, Shape<DT, ELEMS, false>::MINB) norm_forward_kernel(const NormArgs p) {
   using Sh = Shape<DT, ELEMS, false>;
-  constexpr int E = Piece<DT>::value, NV = Sh::NV, R = Sh::R, STAGES = Sh::STAGES, N = LN ? 2 * R : R;
+  constexpr int E = Piece<DT>::value, NV = Sh::NV, R = Sh::R, STAGES = Sh::STAGES, N = LN ? 2 * R : R, W = Sh::WARPS;
   extern __shared__ uint4 ring[];  // [STAGES][R][NV][blockDim.x], then the coefficients
-  __shared__ Sums<N> red[2][kMaxWarps], red_c[2][kMaxWarps];
-  const int T = blockDim.x, tid = threadIdx.x, b = blockIdx.y;
-  const int pieces = p.D / E;
-  const uint8_t* x = p.x + b * p.x_sb;
-  uint8_t* y = p.out + b * p.out_sb;
+  __shared__ Sums<N> red[2][W], red_c[2][W];
+  const int T = blockDim.x, tid = threadIdx.x, b = blockIdx.y, S = static_cast<int>(p.S);
+  const int mine = (p.D / E - tid + T - 1) / T;  // pieces of this thread
+  const uint8_t* x = p.x + b * p.x_sb + tid * 16;
+  uint8_t* y = p.out + b * p.out_sb + tid * 16;
+  uint4* slot = ring + tid;
+  for (int k = tid; k < 2 * W * N; k += T) {
+    (&red[0][0].v[0])[k] = 0.f;
+    (&red_c[0][0].v[0])[k] = 0.f;
+  }
 
-  // y = n mul + add per channel, folded once per CTA; a thread reads back only what it wrote: no barrier
-  const bool coef = p.weight != nullptr || p.scale != nullptr;
-  float4* mul_s = reinterpret_cast<float4*>(ring + STAGES * R * NV * T);
-  float4* add_s = mul_s + NV * (E / 4) * T;
-
-  auto fetch = [&](int64_t row0, int stage) {
+  auto fetch = [&](int row0, int stage) {
 #pragma unroll
-    for (int r = 0; r < R; ++r)
-      if (row0 + r < p.S) {
+    for (int r = 0; r < R; ++r) {
+      const uint8_t* src = x + (row0 + r) * p.x_ss;
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-          const int v = tid + i * T;
-          if (v < pieces) cp_async16(&ring[((stage * R + r) * NV + i) * T + tid], x + (row0 + r) * p.x_ss + v * 16);
-        }
-      }
-    cp_async_commit();  // one group per stage, empty past the end: the group count stays uniform
+      for (int i = 0; i < NV; ++i) cp_async16(&slot[((stage * R + r) * NV + i) * T], src + i * T * 16, row0 + r < S && i < mine);
+    }
+    cp_async_commit();
   };
-  const int64_t step = static_cast<int64_t>(gridDim.x) * R;
-  int64_t row0 = static_cast<int64_t>(blockIdx.x) * R;
+  const int step = gridDim.x * R;
+  int row0 = blockIdx.x * R;
 #pragma unroll
   for (int k = 0; k < STAGES - 1; ++k) fetch(row0 + k * step, k);
+  // y = n mul + add per channel: (n w + c) (1 + scale) + shift, folded once per CTA.  In shared memory and not read from
+  // global memory for every row (from L1 they cost a quarter more time); a thread reads what it wrote itself
+  const bool coef = p.weight != nullptr || p.scale != nullptr;
+  ulonglong2* mul_s = reinterpret_cast<ulonglong2*>(ring + STAGES * R * NV * T) + tid;
+  ulonglong2* add_s = mul_s + NV * (E / 4) * T;
   if (coef) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int v = tid + i * T;
-      if (v >= pieces) continue;
-      float m[E], a[E], t[E];
+      if (i >= mine) continue;
+      const int at = (tid + i * T) * E;
+      Pairs<DT> mul, add;
 #pragma unroll
-      for (int k = 0; k < E; ++k) { m[k] = 1.f; a[k] = 0.f; }
-      if (p.weight != nullptr) load_f32<E>(p.weight + v * E, m);
-      if (LN && p.bias != nullptr) load_f32<E>(p.bias + v * E, a);
+      for (int k = 0; k < E / 2; ++k) {
+        mul.v[k] = f2_splat(1.f);
+        add.v[k] = f2_splat(0.f);
+      }
+      if (p.weight != nullptr) mul = load_vector<DT>(p.weight + at);
+      if (LN && p.bias != nullptr) add = load_vector<DT>(p.bias + at);
       if (LN && p.scale != nullptr) {
-        load_f32<E>(p.scale + static_cast<int64_t>(b) * p.D + v * E, t);
+        const int64_t row = static_cast<int64_t>(b) * p.D + at;
+        const Pairs<DT> t = load_vector<DT>(p.scale + row), u = load_vector<DT>(p.shift + row);
 #pragma unroll
-        for (int k = 0; k < E; ++k) { m[k] *= 1.f + t[k]; a[k] *= 1.f + t[k]; }
-        load_f32<E>(p.shift + static_cast<int64_t>(b) * p.D + v * E, t);
-#pragma unroll
-        for (int k = 0; k < E; ++k) a[k] += t[k];
+        for (int k = 0; k < E / 2; ++k) {
+          mul.v[k] = f2_fma(mul.v[k], t.v[k], mul.v[k]);
+          add.v[k] = f2_add(f2_fma(add.v[k], t.v[k], add.v[k]), u.v[k]);
+        }
       }
 #pragma unroll
       for (int q = 0; q < E / 4; ++q) {
-        mul_s[(i * (E / 4) + q) * T + tid] = *reinterpret_cast<float4*>(&m[4 * q]);
-        if (LN) add_s[(i * (E / 4) + q) * T + tid] = *reinterpret_cast<float4*>(&a[4 * q]);
+        mul_s[(i * (E / 4) + q) * T] = make_ulonglong2(mul.v[2 * q], mul.v[2 * q + 1]);
+        if (LN) add_s[(i * (E / 4) + q) * T] = make_ulonglong2(add.v[2 * q], add.v[2 * q + 1]);
       }
     }
   }
+  __syncthreads();  // the sums' slots are zero
   const float inv_d = 1.f / static_cast<float>(p.D);
   int stage = 0, parity = 0;
-  for (; row0 < p.S; row0 += step) {
+  for (; row0 < S; row0 += step) {
     fetch(row0 + (STAGES - 1) * step, stage == 0 ? STAGES - 1 : stage - 1);
     Rotary<DT> rot[R];
     if (!LN && p.cos != nullptr) {
 #pragma unroll
-      for (int r = 0; r < R; ++r)
-        if (row0 + r < p.S) load_rotary<DT>(p, row0 + r, rot[r]);
+      for (int r = 0; r < R; ++r) load_rotary<DT>(p, min(row0 + r, S - 1), rot[r]);
     }
     cp_async_wait<STAGES - 1>();  // this thread's pieces of the rows have landed
-    float f[R][NV][E];
+    Pairs<DT> f[R][NV];
     float sum[N];
 #pragma unroll
-    for (int k = 0; k < N; ++k) sum[k] = 0.f;
+    for (int r = 0; r < R; ++r) {
+      uint64_t q2 = f2_splat(0.f), s2 = f2_splat(0.f);
 #pragma unroll
-    for (int r = 0; r < R; ++r)
+      for (int i = 0; i < NV; ++i) {
+        f[r][i] = unpack<DT>(slot[((stage * R + r) * NV + i) * T]);
 #pragma unroll
-      for (int i = 0; i < NV; ++i)
-        if (tid + i * T < pieces && row0 + r < p.S) {
-          unpack<DT>(ring[((stage * R + r) * NV + i) * T + tid], f[r][i]);
-#pragma unroll
-          for (int k = 0; k < E; ++k) {
-            sum[r] = fmaf(f[r][i][k], f[r][i][k], sum[r]);
-            if (LN) sum[R + (LN ? r : 0)] += f[r][i][k];
-          }
+        for (int k = 0; k < E / 2; ++k) {
+          q2 = f2_fma(f[r][i].v[k], f[r][i].v[k], q2);
+          if (LN) s2 = f2_add(s2, f[r][i].v[k]);
         }
-    cta_sum<N>(sum, red[parity]);
+      }
+      sum[r] = f2_sum(q2);
+      if (LN) sum[R + (LN ? r : 0)] = f2_sum(s2);
+    }
+    cta_sum<N, W>(sum, red[parity]);
     float mean[R], rstd[R];
     bool centre = false;
 #pragma unroll
@@ -247,20 +288,23 @@ __global__ void __launch_bounds__(Shape<DT, ELEMS, false>::T, Shape<DT, ELEMS, f
       // the branch is uniform): a second pass around the first estimate of the mean.  It takes the rounding of that
       // estimate out as well, so that a constant row normalises to zero.
 #pragma unroll
-      for (int k = 0; k < N; ++k) sum[k] = 0.f;
-#pragma unroll
-      for (int r = 0; r < R; ++r)
+      for (int r = 0; r < R; ++r) {
+        uint64_t q2 = f2_splat(0.f), s2 = f2_splat(0.f);
+        const uint64_t nm = f2_splat(-mean[r]);
 #pragma unroll
         for (int i = 0; i < NV; ++i)
-          if (tid + i * T < pieces && row0 + r < p.S) {
+          if (i < mine) {
 #pragma unroll
-            for (int k = 0; k < E; ++k) {
-              const float d = f[r][i][k] - mean[r];
-              sum[r] = fmaf(d, d, sum[r]);
-              sum[R + (LN ? r : 0)] += d;
+            for (int k = 0; k < E / 2; ++k) {
+              const uint64_t d = f2_add(f[r][i].v[k], nm);
+              q2 = f2_fma(d, d, q2);
+              s2 = f2_add(s2, d);
             }
           }
-      cta_sum<N>(sum, red_c[parity]);
+        sum[r] = f2_sum(q2);
+        sum[R + (LN ? r : 0)] = f2_sum(s2);
+      }
+      cta_sum<N, W>(sum, red_c[parity]);
 #pragma unroll
       for (int r = 0; r < R; ++r) {
         const float dm = sum[R + (LN ? r : 0)] * inv_d;
@@ -270,43 +314,36 @@ __global__ void __launch_bounds__(Shape<DT, ELEMS, false>::T, Shape<DT, ELEMS, f
     }
 #pragma unroll
     for (int r = 0; r < R; ++r)
-      if (tid == r && row0 + r < p.S) {
-        if (LN) p.mean[static_cast<int64_t>(b) * p.S + row0 + r] = mean[r];
-        p.rstd[static_cast<int64_t>(b) * p.S + row0 + r] = rstd[r];
+      if (tid == r && row0 + r < S) {
+        if (LN) p.mean[static_cast<int64_t>(b) * S + row0 + r] = mean[r];
+        p.rstd[static_cast<int64_t>(b) * S + row0 + r] = rstd[r];
       }
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      if (tid + i * T >= pieces) continue;
-#pragma unroll
-      for (int r = 0; r < R; ++r)
-#pragma unroll
-        for (int k = 0; k < E; ++k) f[r][i][k] = LN ? (f[r][i][k] - mean[r]) * rstd[r] : f[r][i][k] * rstd[r];
+      Pairs<DT> mul, add;
       if (coef) {
 #pragma unroll
         for (int q = 0; q < E / 4; ++q) {
-          const float4 m = mul_s[(i * (E / 4) + q) * T + tid];
-          float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (LN) a = add_s[(i * (E / 4) + q) * T + tid];
-#pragma unroll
-          for (int r = 0; r < R; ++r) {
-            f[r][i][4 * q] = fmaf(f[r][i][4 * q], m.x, a.x);
-            f[r][i][4 * q + 1] = fmaf(f[r][i][4 * q + 1], m.y, a.y);
-            f[r][i][4 * q + 2] = fmaf(f[r][i][4 * q + 2], m.z, a.z);
-            f[r][i][4 * q + 3] = fmaf(f[r][i][4 * q + 3], m.w, a.w);
+          const ulonglong2 m = mul_s[(i * (E / 4) + q) * T];
+          mul.v[2 * q] = m.x;
+          mul.v[2 * q + 1] = m.y;
+          if (LN) {
+            const ulonglong2 c = add_s[(i * (E / 4) + q) * T];
+            add.v[2 * q] = c.x;
+            add.v[2 * q + 1] = c.y;
           }
         }
       }
 #pragma unroll
       for (int r = 0; r < R; ++r) {
-        if (!LN && p.cos != nullptr) {
+        const uint64_t nm = f2_splat(-mean[r]), rs = f2_splat(rstd[r]);
 #pragma unroll
-          for (int k = 0; k < E / 2; ++k) {
-            const float u = f[r][i][2 * k], w = f[r][i][2 * k + 1];
-            f[r][i][2 * k] = u * rot[r].c[k] - w * rot[r].s[k];
-            f[r][i][2 * k + 1] = fmaf(u, rot[r].s[k], w * rot[r].c[k]);
-          }
+        for (int k = 0; k < E / 2; ++k) {
+          f[r][i].v[k] = f2_mul(LN ? f2_add(f[r][i].v[k], nm) : f[r][i].v[k], rs);
+          if (coef) f[r][i].v[k] = LN ? f2_fma(f[r][i].v[k], mul.v[k], add.v[k]) : f2_mul(f[r][i].v[k], mul.v[k]);
         }
-        if (row0 + r < p.S) *reinterpret_cast<uint4*>(y + (row0 + r) * p.out_ss + (tid + i * T) * 16) = pack<DT>(f[r][i]);
+        if (!LN && p.cos != nullptr) rotate<DT, 1>(f[r][i], rot[r]);
+        if (row0 + r < S && i < mine) *reinterpret_cast<uint4*>(y + (row0 + r) * p.out_ss + i * T * 16) = pack<DT>(f[r][i]);
       }
     }
     stage = stage == STAGES - 1 ? 0 : stage + 1;
@@ -319,92 +356,83 @@ __global__ void __launch_bounds__(Shape<DT, ELEMS, false>::T, Shape<DT, ELEMS, f
 template <int DT, int ELEMS, bool LN, int SUMS>
 __global__ void __launch_bounds__(Shape<DT, ELEMS, true>::T, Shape<DT, ELEMS, true>::MINB) norm_backward_kernel(const NormArgs p) {
   using Sh = Shape<DT, ELEMS, true>;
-  constexpr int E = Piece<DT>::value, NV = Sh::NV, R = Sh::R, STAGES = Sh::STAGES, N = LN ? 2 * R : R;
+  constexpr int E = Piece<DT>::value, NV = Sh::NV, R = Sh::R, STAGES = Sh::STAGES, N = LN ? 2 * R : R, W = Sh::WARPS;
   extern __shared__ uint4 ring[];  // [STAGES][R][2][NV][blockDim.x], then the coefficients
-  __shared__ Sums<N> red[2][kMaxWarps];
-  const int T = blockDim.x, tid = threadIdx.x, b = blockIdx.y;
-  const int pieces = p.D / E;
-  const uint8_t* x = p.x + b * p.x_sb;
-  const uint8_t* dy = p.dy + b * p.dy_sb;
-  uint8_t* dx = p.out + b * p.out_sb;
-  const float* mean_b = LN ? p.mean + static_cast<int64_t>(b) * p.S : nullptr;
-  const float* rstd_b = p.rstd + static_cast<int64_t>(b) * p.S;
+  __shared__ Sums<N> red[2][W];
+  const int T = blockDim.x, tid = threadIdx.x, b = blockIdx.y, S = static_cast<int>(p.S);
+  const int mine = (p.D / E - tid + T - 1) / T;
+  const uint8_t* x = p.x + b * p.x_sb + tid * 16;
+  const uint8_t* dy = p.dy + b * p.dy_sb + tid * 16;
+  uint8_t* dx = p.out + b * p.out_sb + tid * 16;
+  uint4* slot = ring + tid;
+  const float* mean_b = LN ? p.mean + static_cast<int64_t>(b) * S : nullptr;
+  const float* rstd_b = p.rstd + static_cast<int64_t>(b) * S;
+  for (int k = tid; k < 2 * W * N; k += T) (&red[0][0].v[0])[k] = 0.f;
 
-  auto fetch = [&](int64_t row0, int stage) {
+  auto fetch = [&](int row0, int stage) {
 #pragma unroll
-    for (int r = 0; r < R; ++r)
-      if (row0 + r < p.S) {
-        uint4* at = &ring[(stage * R + r) * 2 * NV * T + tid];
+    for (int r = 0; r < R; ++r) {
+      const uint8_t *src = x + (row0 + r) * p.x_ss, *src_g = dy + (row0 + r) * p.dy_ss;
+      uint4* at = slot + (stage * R + r) * 2 * NV * T;
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-          const int v = tid + i * T;
-          if (v < pieces) {
-            cp_async16(at + i * T, x + (row0 + r) * p.x_ss + v * 16);
-            cp_async16(at + (NV + i) * T, dy + (row0 + r) * p.dy_ss + v * 16);
-          }
-        }
+      for (int i = 0; i < NV; ++i) {
+        const bool valid = row0 + r < S && i < mine;
+        cp_async16(at + i * T, src + i * T * 16, valid);
+        cp_async16(at + (NV + i) * T, src_g + i * T * 16, valid);
       }
+    }
     cp_async_commit();
   };
-  const int64_t step = static_cast<int64_t>(gridDim.x) * R;
-  int64_t row0 = static_cast<int64_t>(blockIdx.x) * R;
+  const int step = gridDim.x * R;
+  int row0 = blockIdx.x * R;
 #pragma unroll
   for (int k = 0; k < STAGES - 1; ++k) fetch(row0 + k * step, k);
 
-  const bool coef = p.weight != nullptr || p.scale != nullptr;  // g = dy mul
-  float4* mul_s = reinterpret_cast<float4*>(ring + STAGES * R * 2 * NV * T);
+  const bool coef = p.weight != nullptr || p.scale != nullptr;  // g = dy mul, mul = w (1 + scale)
+  ulonglong2* mul_s = reinterpret_cast<ulonglong2*>(ring + STAGES * R * 2 * NV * T) + tid;
   if (coef) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int v = tid + i * T;
-      if (v >= pieces) continue;
-      float m[E], t[E];
+      const int at = (tid + i * T) * E;
+      Pairs<DT> mul;
 #pragma unroll
-      for (int k = 0; k < E; ++k) m[k] = 1.f;
-      if (p.weight != nullptr) load_f32<E>(p.weight + v * E, m);
-      if (LN && p.scale != nullptr) {
-        load_f32<E>(p.scale + static_cast<int64_t>(b) * p.D + v * E, t);
+      for (int k = 0; k < E / 2; ++k) mul.v[k] = f2_splat(1.f);  // behind the row's end: times zero
+      if (i < mine) {
+        if (p.weight != nullptr) mul = load_vector<DT>(p.weight + at);
+        if (LN && p.scale != nullptr) {
+          const Pairs<DT> t = load_vector<DT>(p.scale + static_cast<int64_t>(b) * p.D + at);
 #pragma unroll
-        for (int k = 0; k < E; ++k) m[k] *= 1.f + t[k];
+          for (int k = 0; k < E / 2; ++k) mul.v[k] = f2_fma(mul.v[k], t.v[k], mul.v[k]);
+        }
       }
 #pragma unroll
-      for (int q = 0; q < E / 4; ++q) mul_s[(i * (E / 4) + q) * T + tid] = *reinterpret_cast<float4*>(&m[4 * q]);
+      for (int q = 0; q < E / 4; ++q) mul_s[(i * (E / 4) + q) * T] = make_ulonglong2(mul.v[2 * q], mul.v[2 * q + 1]);
     }
   }
-  float sum_n[SUMS > 0 ? NV : 1][E], sum_a[SUMS > 1 ? NV : 1][E];
+  __syncthreads();  // the sums' slots are zero
+  Pairs<DT> sum_n[SUMS > 0 ? NV : 1], sum_a[SUMS > 1 ? NV : 1];
 #pragma unroll
   for (int i = 0; i < NV; ++i)
 #pragma unroll
-    for (int k = 0; k < E; ++k) {
-      if (SUMS > 0) sum_n[SUMS > 0 ? i : 0][k] = 0.f;
-      if (SUMS > 1) sum_a[SUMS > 1 ? i : 0][k] = 0.f;
+    for (int k = 0; k < E / 2; ++k) {
+      if (SUMS > 0) sum_n[SUMS > 0 ? i : 0].v[k] = f2_splat(0.f);
+      if (SUMS > 1) sum_a[SUMS > 1 ? i : 0].v[k] = f2_splat(0.f);
     }
 
-  // n and g = (dy, rotated back) of piece i; `raw` is dy (rotated back) before the coefficients
-  auto piece = [&](int at, int i, float mean, float rstd, const Rotary<DT>& rot, float (&n)[E], float (&raw)[E], float (&g)[E]) {
-    unpack<DT>(ring[at + i * T], n);
-    unpack<DT>(ring[at + (NV + i) * T], raw);
-    if (!LN && p.cos != nullptr) {
+  // n and `raw` = dy (rotated back) of piece i, and g = raw times the coefficients
+  auto piece = [&](const uint4* at, int i, uint64_t nm, uint64_t rs, const Rotary<DT>& rot, Pairs<DT>& n, Pairs<DT>& raw, Pairs<DT>& g) {
+    n = unpack<DT>(at[i * T]);
+    raw = unpack<DT>(at[(NV + i) * T]);
+    if (!LN && p.cos != nullptr) rotate<DT, -1>(raw, rot);
 #pragma unroll
-      for (int k = 0; k < E / 2; ++k) {
-        const float u = raw[2 * k], w = raw[2 * k + 1];
-        raw[2 * k] = fmaf(u, rot.c[k], w * rot.s[k]);
-        raw[2 * k + 1] = w * rot.c[k] - u * rot.s[k];
-      }
-    }
-#pragma unroll
-    for (int k = 0; k < E; ++k) {
-      n[k] = LN ? (n[k] - mean) * rstd : n[k] * rstd;
-      g[k] = raw[k];
-    }
+    for (int k = 0; k < E / 2; ++k) n.v[k] = f2_mul(LN ? f2_add(n.v[k], nm) : n.v[k], rs);
+    g = raw;
     if (coef) {
 #pragma unroll
       for (int q = 0; q < E / 4; ++q) {
-        const float4 m = mul_s[(i * (E / 4) + q) * T + tid];
-        g[4 * q] *= m.x;
-        g[4 * q + 1] *= m.y;
-        g[4 * q + 2] *= m.z;
-        g[4 * q + 3] *= m.w;
+        const ulonglong2 m = mul_s[(i * (E / 4) + q) * T];
+        g.v[2 * q] = f2_mul(g.v[2 * q], m.x);
+        g.v[2 * q + 1] = f2_mul(g.v[2 * q + 1], m.y);
       }
     }
   };
@@ -413,71 +441,72 @@ __global__ void __launch_bounds__(Shape<DT, ELEMS, true>::T, Shape<DT, ELEMS, tr
   int stage = 0, parity = 0;
   // the statistics of the rows are read one group ahead
   float mean_next[R], rstd_next[R];
-  auto statistics = [&](int64_t row) {
+  auto statistics = [&](int row) {
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      mean_next[r] = LN && row + r < p.S ? mean_b[row + r] : 0.f;
-      rstd_next[r] = row + r < p.S ? rstd_b[row + r] : 0.f;
+      const int at = min(row + r, S - 1);
+      mean_next[r] = LN ? mean_b[at] : 0.f;
+      rstd_next[r] = rstd_b[at];
     }
   };
-  statistics(row0);
-  for (; row0 < p.S; row0 += step) {
+  statistics(min(row0, S - 1));
+  for (; row0 < S; row0 += step) {
     fetch(row0 + (STAGES - 1) * step, stage == 0 ? STAGES - 1 : stage - 1);
-    float mean[R], rstd[R], sum[N];
+    uint64_t nm[R], rs[R];
     Rotary<DT> rot[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      mean[r] = mean_next[r];
-      rstd[r] = rstd_next[r];
-      if (!LN && p.cos != nullptr && row0 + r < p.S) load_rotary<DT>(p, row0 + r, rot[r]);
+      nm[r] = f2_splat(-mean_next[r]);
+      rs[r] = f2_splat(rstd_next[r]);
+      if (!LN && p.cos != nullptr) load_rotary<DT>(p, min(row0 + r, S - 1), rot[r]);
     }
-    statistics(row0 + step);
-#pragma unroll
-    for (int k = 0; k < N; ++k) sum[k] = 0.f;
+    statistics(min(row0 + step, S - 1));
     cp_async_wait<STAGES - 1>();
+    float sum[N];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      if (row0 + r >= p.S) continue;
+      uint64_t s_gn = f2_splat(0.f), s_g = f2_splat(0.f);
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        if (tid + i * T >= pieces) continue;
-        float n[E], raw[E], g[E];
-        piece((stage * R + r) * 2 * NV * T + tid, i, mean[r], rstd[r], rot[r], n, raw, g);
+        Pairs<DT> n, raw, g;
+        piece(slot + (stage * R + r) * 2 * NV * T, i, nm[r], rs[r], rot[r], n, raw, g);
 #pragma unroll
-        for (int k = 0; k < E; ++k) {
-          if (SUMS > 0) sum_n[SUMS > 0 ? i : 0][k] = fmaf(raw[k], n[k], sum_n[SUMS > 0 ? i : 0][k]);
-          if (SUMS > 1) sum_a[SUMS > 1 ? i : 0][k] += raw[k];
-          sum[r] = fmaf(g[k], n[k], sum[r]);
-          if (LN) sum[R + (LN ? r : 0)] += g[k];
+        for (int k = 0; k < E / 2; ++k) {
+          if (SUMS > 0) sum_n[SUMS > 0 ? i : 0].v[k] = f2_fma(raw.v[k], n.v[k], sum_n[SUMS > 0 ? i : 0].v[k]);
+          if (SUMS > 1) sum_a[SUMS > 1 ? i : 0].v[k] = f2_add(sum_a[SUMS > 1 ? i : 0].v[k], raw.v[k]);
+          s_gn = f2_fma(g.v[k], n.v[k], s_gn);
+          if (LN) s_g = f2_add(s_g, g.v[k]);
         }
       }
+      sum[r] = f2_sum(s_gn);
+      if (LN) sum[R + (LN ? r : 0)] = f2_sum(s_g);
     }
-    cta_sum<N>(sum, red[parity]);
+    cta_sum<N, W>(sum, red[parity]);
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      if (row0 + r >= p.S) continue;
-      const float m_gn = sum[r] * inv_d, m_g = LN ? sum[R + (LN ? r : 0)] * inv_d : 0.f;
+      const uint64_t neg_gn = f2_splat(-sum[r] * inv_d), neg_g = f2_splat(LN ? -sum[R + (LN ? r : 0)] * inv_d : 0.f);
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        if (tid + i * T >= pieces) continue;
-        float n[E], raw[E], g[E];
-        piece((stage * R + r) * 2 * NV * T + tid, i, mean[r], rstd[r], rot[r], n, raw, g);
+        Pairs<DT> n, raw, g;
+        piece(slot + (stage * R + r) * 2 * NV * T, i, nm[r], rs[r], rot[r], n, raw, g);
 #pragma unroll
-        for (int k = 0; k < E; ++k) g[k] = (fmaf(-n[k], m_gn, g[k]) - m_g) * rstd[r];
-        *reinterpret_cast<uint4*>(dx + (row0 + r) * p.out_ss + (tid + i * T) * 16) = pack<DT>(g);
+        for (int k = 0; k < E / 2; ++k) {
+          const uint64_t t = f2_fma(n.v[k], neg_gn, g.v[k]);
+          g.v[k] = f2_mul(LN ? f2_add(t, neg_g) : t, rs[r]);
+        }
+        if (row0 + r < S && i < mine) *reinterpret_cast<uint4*>(dx + (row0 + r) * p.out_ss + i * T * 16) = pack<DT>(g);
       }
     }
     stage = stage == STAGES - 1 ? 0 : stage + 1;
     parity ^= 1;
   }
   if constexpr (SUMS > 0) {
-    float* part = p.part + (static_cast<int64_t>(b) * gridDim.x + blockIdx.x) * SUMS * p.D;
+    float* part = p.part + (static_cast<int64_t>(b) * gridDim.x + blockIdx.x) * SUMS * p.D + tid * E;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int v = tid + i * T;
-      if (v >= pieces) continue;
-      store_f32<E>(part + v * E, sum_n[SUMS > 0 ? i : 0]);
-      if (SUMS > 1) store_f32<E>(part + p.D + v * E, sum_a[SUMS > 1 ? i : 0]);
+      if (i >= mine) continue;
+      store_vector<DT>(part + i * T * E, sum_n[SUMS > 0 ? i : 0]);
+      if (SUMS > 1) store_vector<DT>(part + p.D + i * T * E, sum_a[SUMS > 1 ? i : 0]);
     }
   }
 }
@@ -508,10 +537,19 @@ __global__ void __launch_bounds__(1024) norm_join_kernel(const JoinArgs p) {
     float s_n = 0.f, s_a = 0.f;
     if (in) {
       const float* q = p.part + b * p.ctas * stride + n;
-#pragma unroll 4
-      for (int c = ty; c < p.ctas; c += 32) {
-        s_n += q[c * stride];
-        if (SUMS > 1) s_a += q[c * stride + p.D];
+      for (int c = ty; c < p.ctas; c += 256) {  // eight rows' loads at a time
+        float u[8], v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const bool have = c + 32 * k < p.ctas;
+          u[k] = have ? __ldcg(q + (c + 32 * k) * stride) : 0.f;
+          v[k] = have && SUMS > 1 ? __ldcg(q + (c + 32 * k) * stride + p.D) : 0.f;
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          s_n += u[k];
+          s_a += v[k];
+        }
       }
     }
     __syncthreads();
@@ -546,9 +584,8 @@ __global__ void __launch_bounds__(1024) norm_join_kernel(const JoinArgs p) {
 }
 
 // ---- host ----------------------------------------------------------------------------------------------------------------
-// Elements of a row per thread: 8 while that makes at most 256 threads, 16 up to 320, else 32 (more threads only add to
-// the barrier; fewer hold the rows of narrow tensors too long).
-inline int row_elems(int64_t D) { return D <= 2048 ? 8 : (D <= 5120 ? 16 : 32); }
+// Elements of a row per thread: few while the rows are narrow, so that there are threads; at most 320 threads.
+inline int row_elems(int64_t D) { return D <= 1024 ? 8 : (D <= 5120 ? 16 : 32); }
 inline int row_threads(int64_t D) { return static_cast<int>((D / row_elems(D) + (D % row_elems(D) != 0) + 31) / 32 * 32); }
 // CTAs that stay resident and stride over the rows, over all samples: at most what fits on the GPU at once and eight per SM
 // (more adds nothing to the bytes in flight, but partial sums to join).
@@ -601,6 +638,7 @@ int check_rows(const char* what, int dtype, int64_t B, int64_t S, int64_t D) {
   DAX_REQUIRE(D % 8 == 0 && D <= kMaxWidth, DAX_ERR_UNSUPPORTED, "%s: D=%lld must be a multiple of 8 and at most %lld", what,
               (long long)D, (long long)kMaxWidth);
   DAX_REQUIRE(B <= 65535, DAX_ERR_UNSUPPORTED, "%s: batch %lld exceeds 65535", what, (long long)B);
+  DAX_REQUIRE(S < (1ll << 30), DAX_ERR_UNSUPPORTED, "%s: %lld rows per sample", what, (long long)S);
   return DAX_OK;
 }
 int check_tensor(const char* what, const char* name, const void* t, int64_t sb, int64_t ss, int dtype) {
