@@ -616,7 +616,7 @@ def _heads_view(t: torch.Tensor) -> Tuple[torch.Tensor, I64x3]:
     return t, I64x3(*st)
 
 
-def _attention_inputs(what: str, q, k, v, q_lens, k_lens, sm_scale, *more) -> Tuple[int, int, int, int, float, torch.device]:
+def _attention_inputs(what: str, q, k, v, q_lens, k_lens, sm_scale) -> Tuple[int, int, int, int, float]:
     for name, t in (("q", q), ("k", k), ("v", v)):
         if t.dim() != 4 or t.shape[3] != 128:
             raise ValueError(f"{what}: {name} must be [B, heads, S, 128], got {list(t.shape)}")
@@ -632,7 +632,7 @@ def _attention_inputs(what: str, q, k, v, q_lens, k_lens, sm_scale, *more) -> Tu
         sm_scale = 1.0 / math.sqrt(128)
     if not 0.0 < sm_scale < math.inf:
         raise ValueError(f"{what}: sm_scale must be positive and finite, got {sm_scale}")
-    return B, heads, Sq, k.shape[2], float(sm_scale), _on_one_device(what, q, k, v, q_lens, k_lens, *more)
+    return B, heads, Sq, k.shape[2], float(sm_scale)
 
 
 def _token_major(t: torch.Tensor) -> torch.Tensor:
@@ -652,7 +652,8 @@ def attention_lse(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, q_lens: 
     ``q_lens`` / ``k_lens`` (int32 ``[B]`` on the device): the tokens of each sample of a padded batch that exist; the
     others may hold anything.  Queries that do not exist or see no key get ``out = 0``, ``lse = -inf``."""
     what = "attention_lse"
-    B, heads, Sq, Sk, sm_scale, dev = _attention_inputs(what, q, k, v, q_lens, k_lens, sm_scale)
+    B, heads, Sq, Sk, sm_scale = _attention_inputs(what, q, k, v, q_lens, k_lens, sm_scale)
+    dev = _on_one_device(what, q, k, v, q_lens, k_lens)
     out = _token_major(q)
     lse = torch.empty((B, heads, Sq), dtype=torch.float32, device=dev)
     if lse.numel() == 0:
@@ -679,11 +680,12 @@ def attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: 
     and what it returned.  The probabilities are recomputed; sums are fp32 in a fixed order, so equal inputs give equal
     bits.  Tokens that do not exist get zero gradients and contribute to none."""
     what = "attention_backward"
-    B, heads, Sq, Sk, sm_scale, dev = _attention_inputs(what, q, k, v, q_lens, k_lens, sm_scale, dout, out, lse)
+    B, heads, Sq, Sk, sm_scale = _attention_inputs(what, q, k, v, q_lens, k_lens, sm_scale)
     for name, t in (("dout", dout), ("out", out)):
         if t.shape != q.shape or t.dtype != q.dtype:
             raise ValueError(f"{what}: {name} must be {list(q.shape)} of {q.dtype}, got {list(t.shape)} of {t.dtype}")
     _vector(what, "lse", lse, B, heads, Sq)
+    dev = _on_one_device(what, dout, q, k, v, out, lse, q_lens, k_lens)
     dq, dk, dv = _token_major(q), _token_major(k), _token_major(v)
     if lse.numel() == 0 or Sk == 0:
         return dq.zero_(), dk.zero_(), dv.zero_()
