@@ -18,6 +18,7 @@
 // Scores, probabilities, row statistics, D and all sums are fp32.  p and ds are rounded once to the operands' type, as A
 // operands of the second products (the tensor cores take nothing wider together with 16-bit B operands).
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 
 #include "quant_common.cuh"
@@ -238,14 +239,21 @@ __device__ __forceinline__ void close_tmem(uint32_t base, bool owner, volatile u
 // left of it.
 constexpr int DQ_SLOTS = 6;
 constexpr int DQ_OFF_Q = DQ_SLOTS * TILE_BYTES;
-constexpr int DQ_OFF_E = DQ_OFF_Q;                  // [4][128] floats: parts of e      (q is no longer needed by then)
-constexpr int DQ_OFF_MEAN = DQ_OFF_Q + 2048;        // [16][128] floats: sums of keys, in the end m in the first row
-constexpr int DQ_OFF_D = DQ_OFF_Q + TILE_BYTES;     // [2][128] floats: parts of D
-constexpr int DQ_OFF_BAR = DQ_OFF_D + 1024;
+constexpr int DQ_OFF_MEAN = DQ_OFF_Q;               // [16][128] floats: sums of keys, in the end m in the first row; over q
+constexpr int DQ_OFF_BAR = DQ_OFF_Q + TILE_BYTES;
 constexpr int DQ_SMEM = DQ_OFF_BAR + 256 + 1024;
 static_assert(DQ_SMEM <= 227 * 1024, "shared memory of the dq kernel");
 
 __device__ __forceinline__ void row_warps_sync() { asm volatile("bar.sync 1, 512;" ::: "memory"); }  // warps 0..15
+
+// The four column groups' values of a row, left in tensor memory 32 columns apart.
+__device__ __forceinline__ float sum_of_groups(uint32_t taddr) {
+  uint32_t v[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) tmem_ld1(taddr + 32 * i, v[i]);
+  tmem_wait_ld();
+  return (__uint_as_float(v[0]) + __uint_as_float(v[1])) + (__uint_as_float(v[2]) + __uint_as_float(v[3]));
+}
 
 template <bool BF16>
 __global__ void __launch_bounds__(Warps<ROW_WARPS_B>::threads, 1)
@@ -283,7 +291,7 @@ attn_bwd_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
   uint64_t* tail = empty + DQ_SLOTS;
   uint64_t* q_full = tail + 1;           // q in shared memory
   uint64_t* rows_full = q_full + 1;      // do and o in shared memory
-  uint64_t* do_full = rows_full + 1;     // do in tensor memory, D in shared memory
+  uint64_t* do_full = rows_full + 1;     // do and the parts of D in tensor memory
   uint64_t* s_full = do_full + 1;
   uint64_t* s_free = s_full + 1;
   uint64_t* dp_full = s_free + 1;
@@ -400,49 +408,38 @@ attn_bwd_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
     const int cg = warp >> 2, r = (warp & 3) * 32 + lane, q_row = q0 + r;
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const bool live = q_row < q_len;
-    float* s_d = reinterpret_cast<float*>(smem + DQ_OFF_D);
-    float* s_e = reinterpret_cast<float*>(smem + DQ_OFF_E);
     float* s_mean = reinterpret_cast<float*>(smem + DQ_OFF_MEAN);
-    float nl = -INFINITY;
-    if (live) {
-      const float l = p.lse[static_cast<int64_t>(bh) * p.Sq + q_row];
-      nl = l == -INFINITY ? -INFINITY : -l * LOG2E;
-    }
+    const float l = live ? p.lse[static_cast<int64_t>(bh) * p.Sq + q_row] : -INFINITY;
     bool ok = mbar_wait(rows_full, 0, abort_flag);
-    {  // a quarter of a row of do to tensor memory; the first two groups of warps compute half of D each
+    {  // a quarter of a row of do to tensor memory, and its part of D to where dq will be
       uint32_t w[16];
+      float d[2] = {0.f, 0.f};
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        uint4 u = *reinterpret_cast<const uint4*>(do_smem + (cg >> 1) * BOX_BYTES + r * 128 + ((((cg & 1) * 4 + i) ^ (r & 7)) << 4));
-        if (!live) u = make_uint4(0u, 0u, 0u, 0u);
-        w[4 * i] = u.x; w[4 * i + 1] = u.y; w[4 * i + 2] = u.z; w[4 * i + 3] = u.w;
+        const int at = (cg >> 1) * BOX_BYTES + r * 128 + ((((cg & 1) * 4 + i) ^ (r & 7)) << 4);
+        uint4 u = *reinterpret_cast<const uint4*>(do_smem + at), o = *reinterpret_cast<const uint4*>(o_smem + at);
+        if (!live) u = o = make_uint4(0u, 0u, 0u, 0u);
+        const uint32_t uw[4] = {u.x, u.y, u.z, u.w}, ow[4] = {o.x, o.y, o.z, o.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          float a0, a1, o0, o1;
+          unpack2<BF16>(uw[k], a0, a1);
+          unpack2<BF16>(ow[k], o0, o1);
+          d[0] = fmaf(a0, o0, d[0]);
+          d[1] = fmaf(a1, o1, d[1]);
+          w[4 * i + k] = uw[k];
+        }
       }
       tmem_st16(tm + lanes + T_DO + cg * 16, w);
-      if (cg < 2) {
-        float d[2] = {0.f, 0.f};
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int at = cg * BOX_BYTES + r * 128 + ((i ^ (r & 7)) << 4);
-          const uint4 u = *reinterpret_cast<const uint4*>(do_smem + at), o = *reinterpret_cast<const uint4*>(o_smem + at);
-          const uint32_t uw[4] = {u.x, u.y, u.z, u.w}, ow[4] = {o.x, o.y, o.z, o.w};
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            float a0, a1, o0, o1;
-            unpack2<BF16>(uw[k], a0, a1);
-            unpack2<BF16>(ow[k], o0, o1);
-            d[0] = fmaf(a0, o0, d[0]);
-            d[1] = fmaf(a1, o1, d[1]);
-          }
-        }
-        s_d[cg * 128 + r] = live ? d[0] + d[1] : 0.f;
-      }
+      tmem_st1(tm + lanes + T_DQ + cg * 32, __float_as_uint(d[0] + d[1]));
       tmem_wait_st();
       tc_fence_before_sync();
       __syncwarp();
       if (lane == 0) mbar_arrive(do_full);
     }
     ok = ok && mbar_wait(do_full, 0, abort_flag);  // all warps have arrived
-    const float nd = -(s_d[r] + s_d[128 + r]);
+    tc_fence_after_sync();
+    const float nl = l == -INFINITY ? -INFINITY : -l * LOG2E, nd = -sum_of_groups(tm + lanes + T_DQ);
     if (cg == 0 && split == 0) {
       stat[r] = nl;
       stat[stats + r] = nd;
@@ -529,8 +526,11 @@ attn_bwd_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
         *reinterpret_cast<float4*>(s_mean + warp * 128 + chunk * 8) = make_float4(m[0], m[1], m[2], m[3]);
         *reinterpret_cast<float4*>(s_mean + warp * 128 + chunk * 8 + 4) = make_float4(m[4], m[5], m[6], m[7]);
       }
-      s_e[cg * 128 + r] = e[0] + e[1];
+      tmem_st1(tm + lanes + T_S + cg * 32, __float_as_uint(e[0] + e[1]));  // the scores have all been read
+      tmem_wait_st();
+      tc_fence_before_sync();
       row_warps_sync();
+      tc_fence_after_sync();
       if (threadIdx.x < 128) {
         float t = 0.f;
 #pragma unroll
@@ -543,7 +543,7 @@ attn_bwd_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
       tc_fence_after_sync();
       // the softmax over one key is constant: its gradient is zero, not the rounding of dp - D
       const float mul = k_len == 1 ? 0.f : p.sm_scale;
-      const float neg_e = -((s_e[r] + s_e[128 + r]) + (s_e[256 + r] + s_e[384 + r]));
+      const float neg_e = -sum_of_groups(tm + lanes + T_S);
       const int rows = max(0, min(32, rows_in - (warp & 3) * 32));
       uint8_t* st = smem + warp * 4096;  // every product and every copy is complete: the ring stages the results
       uint32_t v[32];
@@ -1116,15 +1116,15 @@ __global__ void __launch_bounds__(256) attn_bwd_join_kernel(const JoinTarget t0,
 // ---- host ------------------------------------------------------------------------------------------------------------------
 // Splits of the long axis.  `units` CTAs walk over `inner` tiles each; they run in waves of one CTA per SM, so a launch takes
 // waves x (tiles per CTA + `fixed`), `fixed` being the prologue and epilogue of a CTA in tiles.  Splitting fills the last
-// wave and, with few rows, the GPU, but its fp32 parts are written and read again: `join` tiles' time for each split of a
-// whole wave's outputs.
+// wave and, with few rows, the GPU, but costs another launch and its fp32 parts are written and read again: `join` tiles'
+// time for a whole wave's parts (forward: 2 x 132 KB per CTA at 5 TB/s against 1.6 us per tile).
 inline int choose_splits(int64_t units, int64_t inner, double fixed, double join) {
   const int64_t sms = sm_count();
   int best = 1;
   double best_cost = 0;
   for (int s = 1; s <= kMaxSplits && (s == 1 || inner >= 2 * s); ++s) {
     const double waves = static_cast<double>((units * s + sms - 1) / sms);
-    const double cost = waves * (static_cast<double>((inner + s - 1) / s) + fixed) + (s > 1 ? 4.0 + join * static_cast<double>(units * s) / sms : 0.0);
+    const double cost = waves * (static_cast<double>((inner + s - 1) / s) + fixed) + (s > 1 ? 3.0 + join * static_cast<double>(units * s) / sms : 0.0);
     if (s == 1 || cost < 0.97 * best_cost) {
       best = s;
       best_cost = cost;
@@ -1133,9 +1133,9 @@ inline int choose_splits(int64_t units, int64_t inner, double fixed, double join
   return best;
 }
 inline int64_t tiles_of(int64_t S, int64_t t) { return (S + t - 1) / t; }
-inline int forward_splits(int64_t BH, int64_t Sq, int64_t Sk) { return choose_splits(BH * tiles_of(Sq, 256), tiles_of(Sk, 128), 3.0, 0.6); }
-inline int dq_splits(int64_t BH, int64_t Sq, int64_t Sk) { return choose_splits(BH * tiles_of(Sq, 128), tiles_of(Sk, 128), 4.0, 0.3); }
-inline int dkdv_splits(int64_t BH, int64_t Sq, int64_t Sk) { return choose_splits(BH * tiles_of(Sk, 128), tiles_of(Sq, 128), 4.0, 0.6); }
+inline int forward_splits(int64_t BH, int64_t Sq, int64_t Sk) { return choose_splits(BH * tiles_of(Sq, 256), tiles_of(Sk, 128), 3.0, 5.0); }
+inline int dq_splits(int64_t BH, int64_t Sq, int64_t Sk) { return choose_splits(BH * tiles_of(Sq, 128), tiles_of(Sk, 128), 5.0, 3.0); }
+inline int dkdv_splits(int64_t BH, int64_t Sq, int64_t Sk) { return choose_splits(BH * tiles_of(Sk, 128), tiles_of(Sq, 128), 4.0, 4.0); }
 inline int64_t pad128(int64_t S) { return tiles_of(S, 128) * 128; }
 inline size_t round256(size_t n) { return (n + 255) / 256 * 256; }
 
@@ -1183,12 +1183,12 @@ inline Rows rows_of(const void* t, const int64_t* st) { return {t, st[0], st[1],
 // The shared-memory limit of a kernel is set once per device (concurrent first calls set the same value).
 template <typename K, K kernel>
 int allow_smem(int bytes) {
-  static bool done[64] = {};
+  static std::atomic<bool> done[64] = {};
   int dev = 0;
   DAX_CUDA(cudaGetDevice(&dev));
-  if (dev < 64 && done[dev]) return DAX_OK;
+  if (dev < 64 && done[dev].load(std::memory_order_relaxed)) return DAX_OK;
   DAX_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
-  if (dev < 64) done[dev] = true;
+  if (dev < 64) done[dev].store(true, std::memory_order_relaxed);
   return DAX_OK;
 }
 

@@ -445,42 +445,40 @@ def _on_one_device(what: str, *ts) -> torch.device:
     return dev
 
 
-def _rows3(t: torch.Tensor) -> torch.Tensor:
-    """``[B, S, D]`` or ``[S, D]`` as ``[B, S, D]`` that the row kernels can read: channels contiguous, everything else in
-    whole 16 bytes.  A tensor that is not laid out like that is copied."""
-    t = t if t.dim() == 3 else t.unsqueeze(0)
-    e = t.element_size()
-    if t.stride(2) != 1 or t.data_ptr() % 16 or (t.shape[0] > 1 and t.stride(0) * e % 16) or (t.shape[1] > 1 and t.stride(1) * e % 16):
-        t = t.clone(memory_format=torch.contiguous_format)
-    return t
+def _rows(what: str, name: str, t: torch.Tensor) -> Tuple[torch.Tensor, int, int, int, int, int]:
+    """``t [B, S, D]`` or ``[S, D]`` for the row kernels: ``(tensor, B, S, D, sample stride, token stride)``.  They want the
+    channels contiguous and everything else in whole 16 bytes; a tensor that is not laid out like that is copied."""
+    shape, strides = t.shape, t.stride()
+    if len(shape) == 3:
+        (B, S, D), (sb, ss, sd) = shape, strides
+    elif len(shape) == 2:
+        (S, D), (ss, sd), B, sb = shape, strides, 1, 0
+    else:
+        raise ValueError(f"{what}: {name} must be [B, S, D] or [S, D], got {list(shape)}")
+    if t.dtype not in _ROW_PIECE:
+        raise NotImplementedError(f"{what}: {name} must be bf16, fp16 or fp32, got {t.dtype}")
+    # the stride of a dimension of one is never used, and torch may report anything for it
+    sb, ss = sb if B > 1 else 0, ss if S > 1 else 0
+    if sd != 1 or sb % _ROW_PIECE[t.dtype] or ss % _ROW_PIECE[t.dtype] or t.data_ptr() % 16:
+        t, sb, ss = t.clone(memory_format=torch.contiguous_format), S * D, D
+    return t, B, S, D, sb, ss
 
 
-def _row_strides(t: torch.Tensor) -> Tuple[int, int]:
-    """Sample and token stride; those of a dimension of one are never used and torch may report anything for them."""
-    B, S, D = t.shape
-    return t.stride(0) if B > 1 else 0, t.stride(1) if S > 1 else 0
+_ROW_PIECE = {torch.bfloat16: 8, torch.float16: 8, torch.float32: 4}  # elements in 16 bytes
 
 
-def _vector(what: str, name: str, v: Optional[torch.Tensor], *shape: int) -> None:
-    if v is not None and (v.dtype != torch.float32 or tuple(v.shape) != shape or not v.is_contiguous()):
+def _vector(what: str, name: str, v: Optional[torch.Tensor], shape: Tuple[int, ...]) -> None:
+    if v is not None and (v.dtype != torch.float32 or v.shape != shape or not v.is_contiguous()):
         raise ValueError(f"{what}: {name} must be a contiguous fp32 {list(shape)} tensor, got {v.dtype} {list(v.shape)}")
-
-
-def _row_input(what: str, x: torch.Tensor) -> Tuple[int, int, int]:
-    if x.dim() not in (2, 3):
-        raise ValueError(f"{what}: x must be [B, S, D] or [S, D], got {list(x.shape)}")
-    if x.dtype not in (torch.bfloat16, torch.float16, torch.float32):
-        raise NotImplementedError(f"{what}: x must be bf16, fp16 or fp32, got {x.dtype}")
-    return (1, *x.shape) if x.dim() == 2 else tuple(x.shape)
-
-
-def _modulation(what: str, name: str, v: Optional[torch.Tensor], x: torch.Tensor) -> None:
-    _vector(what, name, v, *((x.shape[0], x.shape[2]) if x.dim() == 3 else (x.shape[1],)))
 
 
 def _grad_like(what: str, dy: torch.Tensor, x: torch.Tensor) -> None:
     if dy.shape != x.shape or dy.dtype != x.dtype:
         raise ValueError(f"{what}: dy must be {list(x.shape)} of {x.dtype}, got {list(dy.shape)} of {dy.dtype}")
+
+
+def _dense_like(t: torch.Tensor) -> torch.Tensor:
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
 def layernorm_modulate(x: torch.Tensor, *, eps: float = 1e-6, ln_weight: Optional[torch.Tensor] = None,
@@ -491,19 +489,19 @@ def layernorm_modulate(x: torch.Tensor, *, eps: float = 1e-6, ln_weight: Optiona
     is one sample with ``shift, scale [D]``.  Returns ``(y, mean, rstd)``; the statistics (fp32, one for each row) are what
     ``layernorm_modulate_backward`` needs.  The inference step, which quantises ``y``, is ``layernorm_modulate_quant``."""
     what = "layernorm_modulate"
-    B, S, D = _row_input(what, x)
-    _vector(what, "ln_weight", ln_weight, D)
-    _vector(what, "ln_bias", ln_bias, D)
-    _modulation(what, "shift", shift, x)
-    _modulation(what, "scale", scale, x)
+    rows, B, S, D, sb, ss = _rows(what, "x", x)
+    modulation = (B, D) if x.dim() == 3 else (D,)
+    _vector(what, "ln_weight", ln_weight, (D,))
+    _vector(what, "ln_bias", ln_bias, (D,))
+    _vector(what, "shift", shift, modulation)
+    _vector(what, "scale", scale, modulation)
     dev = _on_one_device(what, x, ln_weight, ln_bias, shift, scale)
-    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    y = _dense_like(x)
     mean = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev)
     rstd = torch.empty_like(mean)
-    x3 = _rows3(x)
     with _OnDevice(dev.index) as stream:
         tok = TRACE.begin(what)
-        check(load().dax_layernorm_modulate(x3.data_ptr(), _dt(x.dtype), B, S, D, *_row_strides(x3), _ptr(ln_weight),
+        check(load().dax_layernorm_modulate(rows.data_ptr(), _dt(x.dtype), B, S, D, sb, ss, _ptr(ln_weight),
                                             _ptr(ln_bias), _ptr(shift), _ptr(scale), float(eps), y.data_ptr(), S * D, D,
                                             mean.data_ptr(), rstd.data_ptr(), stream))
         TRACE.end(tok, (B, S, D))
@@ -517,25 +515,26 @@ def layernorm_modulate_backward(dy: torch.Tensor, x: torch.Tensor, mean: torch.T
     dshift, dscale)``.  The parameter gradients are fp32 sums over the rows, in a fixed order (equal inputs give equal
     bits); those of vectors that were not given, and all of them with ``need_params=False``, are None."""
     what = "layernorm_modulate_backward"
-    B, S, D = _row_input(what, x)
     _grad_like(what, dy, x)
-    _vector(what, "mean", mean, *x.shape[:-1])
-    _vector(what, "rstd", rstd, *x.shape[:-1])
-    _vector(what, "ln_weight", ln_weight, D)
-    _vector(what, "ln_bias", ln_bias, D)
-    _modulation(what, "scale", scale, x)
+    rows, B, S, D, sb, ss = _rows(what, "x", x)
+    grads, _, _, _, gb, gs = _rows(what, "dy", dy)
+    statistics = x.shape[:-1]
+    _vector(what, "mean", mean, statistics)
+    _vector(what, "rstd", rstd, statistics)
+    _vector(what, "ln_weight", ln_weight, (D,))
+    _vector(what, "ln_bias", ln_bias, (D,))
+    _vector(what, "scale", scale, (B, D) if x.dim() == 3 else (D,))
     dev = _on_one_device(what, dy, x, mean, rstd, ln_weight, ln_bias, scale)
-    dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    dx = _dense_like(x)
     dweight = torch.empty_like(ln_weight) if need_params and ln_weight is not None else None
     dbias = torch.empty_like(ln_bias) if need_params and ln_bias is not None else None
     dshift, dscale = (torch.empty_like(scale), torch.empty_like(scale)) if need_params and scale is not None else (None, None)
-    x3, dy3 = _rows3(x), _rows3(dy)
     with _OnDevice(dev.index) as stream:
         lib, dt = load(), _dt(x.dtype)
         n = lib.dax_norm_backward_workspace_bytes(B, S, D) if dweight is not None or dscale is not None else 0
         ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
         tok = TRACE.begin(what)
-        check(lib.dax_layernorm_modulate_backward(dy3.data_ptr(), x3.data_ptr(), dt, B, S, D, *_row_strides(dy3), *_row_strides(x3),
+        check(lib.dax_layernorm_modulate_backward(grads.data_ptr(), rows.data_ptr(), dt, B, S, D, gb, gs, sb, ss,
                                                   mean.data_ptr(), rstd.data_ptr(), _ptr(ln_weight), _ptr(ln_bias), _ptr(scale),
                                                   dx.data_ptr(), S * D, D, _ptr(dweight), _ptr(dbias), _ptr(dshift), _ptr(dscale),
                                                   _ptr(ws), n, stream))
@@ -543,7 +542,7 @@ def layernorm_modulate_backward(dy: torch.Tensor, x: torch.Tensor, mean: torch.T
     return dx, dweight, dbias, dshift, dscale
 
 
-def _rope_check(what: str, x: torch.Tensor, S: int, D: int, cos: Optional[torch.Tensor], sin: Optional[torch.Tensor]) -> None:
+def _rope_check(what: str, S: int, D: int, cos: Optional[torch.Tensor], sin: Optional[torch.Tensor]) -> None:
     if (cos is None) != (sin is None):
         raise ValueError(f"{what}: rope_cos and rope_sin come together")
     for name, t in (("rope_cos", cos), ("rope_sin", sin)):
@@ -560,16 +559,15 @@ def rmsnorm_rope(x: torch.Tensor, norm_weight: Optional[torch.Tensor] = None, *,
     every sample).  Returns ``(y, rstd)``; ``rstd`` is what ``rmsnorm_rope_backward`` needs.  The inference step, which writes
     the exchange layout, is ``rmsnorm_rope_pack``."""
     what = "rmsnorm_rope"
-    B, S, D = _row_input(what, x)
-    _vector(what, "norm_weight", norm_weight, D)
-    _rope_check(what, x, S, D, rope_cos, rope_sin)
+    rows, B, S, D, sb, ss = _rows(what, "x", x)
+    _vector(what, "norm_weight", norm_weight, (D,))
+    _rope_check(what, S, D, rope_cos, rope_sin)
     dev = _on_one_device(what, x, norm_weight, rope_cos, rope_sin)
-    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    y = _dense_like(x)
     rstd = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev)
-    x3 = _rows3(x)
     with _OnDevice(dev.index) as stream:
         tok = TRACE.begin(what)
-        check(load().dax_rmsnorm_rope(x3.data_ptr(), _dt(x.dtype), B, S, D, *_row_strides(x3), _ptr(norm_weight), _ptr(rope_cos),
+        check(load().dax_rmsnorm_rope(rows.data_ptr(), _dt(x.dtype), B, S, D, sb, ss, _ptr(norm_weight), _ptr(rope_cos),
                                       _ptr(rope_sin), float(eps), y.data_ptr(), S * D, D, rstd.data_ptr(), stream))
         TRACE.end(tok, (B, S, D))
     return y, rstd
@@ -581,21 +579,21 @@ def rmsnorm_rope_backward(dy: torch.Tensor, x: torch.Tensor, rstd: torch.Tensor,
     """Gradients of ``rmsnorm_rope``: ``(dx, dweight)``, ``dweight`` (fp32, summed in a fixed order) None without a weight
     or with ``need_params=False``."""
     what = "rmsnorm_rope_backward"
-    B, S, D = _row_input(what, x)
     _grad_like(what, dy, x)
-    _vector(what, "rstd", rstd, *x.shape[:-1])
-    _vector(what, "norm_weight", norm_weight, D)
-    _rope_check(what, x, S, D, rope_cos, rope_sin)
+    rows, B, S, D, sb, ss = _rows(what, "x", x)
+    grads, _, _, _, gb, gs = _rows(what, "dy", dy)
+    _vector(what, "rstd", rstd, x.shape[:-1])
+    _vector(what, "norm_weight", norm_weight, (D,))
+    _rope_check(what, S, D, rope_cos, rope_sin)
     dev = _on_one_device(what, dy, x, rstd, norm_weight, rope_cos, rope_sin)
-    dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    dx = _dense_like(x)
     dweight = torch.empty_like(norm_weight) if need_params and norm_weight is not None else None
-    x3, dy3 = _rows3(x), _rows3(dy)
     with _OnDevice(dev.index) as stream:
         lib, dt = load(), _dt(x.dtype)
         n = lib.dax_norm_backward_workspace_bytes(B, S, D) if dweight is not None else 0
         ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
         tok = TRACE.begin(what)
-        check(lib.dax_rmsnorm_rope_backward(dy3.data_ptr(), x3.data_ptr(), dt, B, S, D, *_row_strides(dy3), *_row_strides(x3),
+        check(lib.dax_rmsnorm_rope_backward(grads.data_ptr(), rows.data_ptr(), dt, B, S, D, gb, gs, sb, ss,
                                             rstd.data_ptr(), _ptr(norm_weight), _ptr(rope_cos), _ptr(rope_sin), dx.data_ptr(), S * D, D,
                                             _ptr(dweight), _ptr(ws), n, stream))
         TRACE.end(tok, (B, S, D))
@@ -617,22 +615,26 @@ def _heads_view(t: torch.Tensor) -> Tuple[torch.Tensor, I64x3]:
 
 
 def _attention_inputs(what: str, q, k, v, q_lens, k_lens, sm_scale) -> Tuple[int, int, int, int, float]:
-    for name, t in (("q", q), ("k", k), ("v", v)):
-        if t.dim() != 4 or t.shape[3] != 128:
-            raise ValueError(f"{what}: {name} must be [B, heads, S, 128], got {list(t.shape)}")
-    if k.shape != v.shape or k.shape[:2] != q.shape[:2]:
-        raise ValueError(f"{what}: q {list(q.shape)}, k {list(k.shape)} and v {list(v.shape)} do not belong together")
-    if q.dtype not in (torch.bfloat16, torch.float16) or k.dtype != q.dtype or v.dtype != q.dtype:
-        raise NotImplementedError(f"{what}: q, k and v must all be bf16 or all fp16, got {q.dtype}, {k.dtype}, {v.dtype}")
-    B, heads, Sq, _ = q.shape
+    qs, ks, vs, dt = q.shape, k.shape, v.shape, q.dtype
+    for name, shape in (("q", qs), ("k", ks), ("v", vs)):
+        if len(shape) != 4 or shape[3] != 128:
+            raise ValueError(f"{what}: {name} must be [B, heads, S, 128], got {list(shape)}")
+    B, heads, Sq, _ = qs
+    if ks != vs or ks[0] != B or ks[1] != heads:
+        raise ValueError(f"{what}: q {list(qs)}, k {list(ks)} and v {list(vs)} do not belong together")
+    if dt not in (torch.bfloat16, torch.float16) or k.dtype != dt or v.dtype != dt:
+        raise NotImplementedError(f"{what}: q, k and v must all be bf16 or all fp16, got {dt}, {k.dtype}, {v.dtype}")
     for name, t in (("q_lens", q_lens), ("k_lens", k_lens)):
         if t is not None and (t.dtype != torch.int32 or tuple(t.shape) != (B,) or not t.is_contiguous()):
             raise ValueError(f"{what}: {name} must be a contiguous int32 [{B}] tensor, got {t.dtype} {list(t.shape)}")
     if sm_scale is None:
-        sm_scale = 1.0 / math.sqrt(128)
-    if not 0.0 < sm_scale < math.inf:
+        sm_scale = _SM_SCALE
+    elif not 0.0 < sm_scale < math.inf:
         raise ValueError(f"{what}: sm_scale must be positive and finite, got {sm_scale}")
-    return B, heads, Sq, k.shape[2], float(sm_scale)
+    return B, heads, Sq, ks[2], float(sm_scale)
+
+
+_SM_SCALE = 1.0 / math.sqrt(128)
 
 
 def _token_major(t: torch.Tensor) -> torch.Tensor:
@@ -684,7 +686,7 @@ def attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: 
     for name, t in (("dout", dout), ("out", out)):
         if t.shape != q.shape or t.dtype != q.dtype:
             raise ValueError(f"{what}: {name} must be {list(q.shape)} of {q.dtype}, got {list(t.shape)} of {t.dtype}")
-    _vector(what, "lse", lse, B, heads, Sq)
+    _vector(what, "lse", lse, (B, heads, Sq))
     dev = _on_one_device(what, dout, q, k, v, out, lse, q_lens, k_lens)
     dq, dk, dv = _token_major(q), _token_major(k), _token_major(v)
     if lse.numel() == 0 or Sk == 0:
