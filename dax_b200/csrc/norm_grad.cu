@@ -584,22 +584,23 @@ __global__ void __launch_bounds__(1024) norm_join_kernel(const JoinArgs p) {
 }
 
 // ---- host ----------------------------------------------------------------------------------------------------------------
-// Elements of a row per thread: few while the rows are narrow, so that there are threads; at most 320 threads.
-inline int row_elems(int64_t D) { return D <= 1024 ? 8 : (D <= 5120 ? 16 : 32); }
-inline int row_threads(int64_t D) { return static_cast<int>((D / row_elems(D) + (D % row_elems(D) != 0) + 31) / 32 * 32); }
+// Elements of a row per thread: few while the rows are narrow, so that there are threads; at most 320 threads.  Between
+// 2,560 and 5,120 channels 16 and 32 both fit; which is faster goes by the registers that the pass needs beside the row
+// (32,760 x 5,120 bf16, us, 16 / 32: LayerNorm forward 117 / 124, backward 205 / 193, RMSNorm 118 / 112 and 211 / 225;
+// fp32 6,240 rows, LayerNorm: 52 / 54 and 89 / 104).
+inline int row_elems(int64_t D, int dtype, bool ln, bool backward) {
+  return D <= 1024 ? 8 : (D <= (dtype != DAX_F32 && ln == backward ? 2560 : 5120) ? 16 : 32);
+}
 // CTAs that stay resident and stride over the rows, over all samples: at most what fits on the GPU at once and eight per SM
 // (more adds nothing to the bytes in flight, but partial sums to join).
-inline int64_t max_ctas(int64_t B, int64_t S, int threads) {
-  const int64_t per_sm = std::min<int64_t>(8, std::max<int64_t>(1, 2048 / threads));
-  return std::min(S, std::max<int64_t>(1, per_sm * sm_count() / B));
-}
+inline int64_t max_ctas(int64_t B, int64_t groups) { return std::min(groups, std::max<int64_t>(1, 8 * static_cast<int64_t>(sm_count()) / B)); }
 
 template <typename K>
 int launch_rows(K kernel, const NormArgs& p, int64_t B, int threads, size_t smem, int rows, int64_t* ctas, cudaStream_t st) {
   if (smem > 40 * 1024) DAX_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
   int per_sm = 0;
   DAX_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, threads, smem));
-  *ctas = std::min(max_ctas(B, (p.S + rows - 1) / rows, threads), std::max<int64_t>(1, static_cast<int64_t>(per_sm) * sm_count() / B));
+  *ctas = std::min(max_ctas(B, (p.S + rows - 1) / rows), std::max<int64_t>(1, static_cast<int64_t>(per_sm) * sm_count() / B));
   kernel<<<dim3(static_cast<unsigned>(*ctas), static_cast<unsigned>(B)), threads, smem, st>>>(p);
   DAX_CUDA(cudaGetLastError());
   return DAX_OK;
@@ -607,7 +608,7 @@ int launch_rows(K kernel, const NormArgs& p, int64_t B, int threads, size_t smem
 
 template <int DT, int ELEMS, bool LN>
 int run_shape(const NormArgs& p, int64_t B, int64_t* ctas, int sums, bool backward, cudaStream_t st) {
-  const int threads = row_threads(p.D);
+  const int threads = ((p.D + ELEMS - 1) / ELEMS + 31) / 32 * 32;
   const size_t coef = p.weight != nullptr || p.scale != nullptr ? static_cast<size_t>(threads) * ELEMS * 4 : 0;  // one fp32 vector
   const size_t row = static_cast<size_t>(threads) * ELEMS * (DT == DAX_F32 ? 4 : 2);
   if (!backward) {
@@ -622,7 +623,7 @@ int run_shape(const NormArgs& p, int64_t B, int64_t* ctas, int sums, bool backwa
 
 template <bool LN>
 int run_rows(const NormArgs& p, int dtype, int64_t B, int64_t* ctas, int sums, bool backward, cudaStream_t st) {
-  const int elems = row_elems(p.D);
+  const int elems = row_elems(p.D, dtype, LN, backward);
 #define DAX_ROWS(DT, N) \
   if (dtype == DT && elems == N) return run_shape<DT, N, LN>(p, B, ctas, sums, backward, st)
   DAX_ROWS(DAX_BF16, 8); DAX_ROWS(DAX_BF16, 16); DAX_ROWS(DAX_BF16, 32);
@@ -672,7 +673,7 @@ template <bool LN>
 int backward(const char* what, NormArgs p, JoinArgs j, int dtype, int64_t B, int64_t D, void* workspace, size_t bytes, cudaStream_t st) {
   const bool want = j.dweight != nullptr || j.dbias != nullptr || j.dshift != nullptr || j.dscale != nullptr;
   const int sums = want ? (LN ? 2 : 1) : 0;
-  int64_t ctas = B > 0 ? max_ctas(B, p.S, row_threads(D)) : 0;
+  int64_t ctas = B > 0 ? max_ctas(B, p.S) : 0;
   if (want) {
     const size_t need = static_cast<size_t>(B) * ctas * sums * D * 4;
     DAX_REQUIRE(bytes >= need && (need == 0 || workspace != nullptr), DAX_ERR_INVALID,
@@ -702,7 +703,7 @@ extern "C" {
 
 size_t dax_norm_backward_workspace_bytes(int64_t B, int64_t S, int64_t D) {
   if (B <= 0 || S <= 0 || D <= 0 || D > dax::kMaxWidth) return 0;
-  return static_cast<size_t>(B) * dax::max_ctas(B, S, dax::row_threads(D)) * 2 * D * 4;
+  return static_cast<size_t>(B) * dax::max_ctas(B, S) * 2 * D * 4;
 }
 
 int dax_layernorm_modulate(const void* x, int dtype, int64_t B, int64_t S, int64_t D, int64_t x_sb, int64_t x_ss,
