@@ -16,7 +16,10 @@
 // see no key at all.
 //
 // Scores, probabilities, row statistics, D and all sums are fp32.  p and ds are rounded once to the operands' type, as A
-// operands of the second products (the tensor cores take nothing wider together with 16-bit B operands).
+// operands of the second products (the tensor cores take nothing wider together with 16-bit B operands).  fp16 has its
+// smallest normal number at 2^-14, and the p of a long row of keys lie below it: the backward pass rounds 2^12 p, which is
+// normal down to p = 2^-26, and takes the factor out of dv again.  ds keeps its size (nothing bounds it from above): in fp16
+// it has the range of the gradients themselves, as in any fp16 training.
 #include <algorithm>
 #include <atomic>
 #include <cmath>
@@ -35,6 +38,8 @@ template <int N> struct Warps {
   static constexpr int threads = (N + 4) * 32, producer = N, issuer0 = N + 1, issuer1 = N + 2, tmem = N + 3;
 };
 constexpr float TAU = 8.f;                 // forward: lazy rescale, p <= 2^8
+template <bool BF16> constexpr float P_SHIFT = BF16 ? 0.f : 12.f;             // backward: p is rounded as 2^P_SHIFT p
+template <bool BF16> constexpr float P_UNSHIFT = BF16 ? 1.f : 1.f / 4096.f;
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr int kMaxSplits = 16;
 
@@ -45,7 +50,7 @@ struct TrainParams {
   float* lse;          // [BH, Sq]
   const int* q_lens;   // [B] or null
   const int* k_lens;
-  float* row_stats;    // backward: [2][BH * Sq_pad]: -lse * log2(e) (-inf: no such row), then -D
+  float* row_stats;    // backward: [2][BH * Sq_pad]: P_SHIFT - lse * log2(e) (-inf: no such row), then -D * P_UNSHIFT
   float* part;         // split runs: fp32 partial sums
   float* part_lse;     // split forward runs: [splits, BH, Sq] log2 of each part's sum of exponentials
   int* status;
@@ -441,8 +446,8 @@ attn_bwd_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
     tc_fence_after_sync();
     const float nl = l == -INFINITY ? -INFINITY : -l * LOG2E, nd = -sum_of_groups(tm + lanes + T_DQ);
     if (cg == 0 && split == 0) {
-      stat[r] = nl;
-      stat[stats + r] = nd;
+      stat[r] = nl + P_SHIFT<BF16>;
+      stat[stats + r] = nd * P_UNSHIFT<BF16>;
     }
     const uint64_t nl2 = f2_splat(nl), nd2 = f2_splat(nd), cmul2 = f2_splat(p.sm_scale * LOG2E);
     float e[2] = {0.f, 0.f};  // sums of the rounded ds
@@ -750,6 +755,11 @@ attn_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
     const int cg = warp >> 2, k_row = k0 + (warp & 3) * 32 + lane;
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint64_t cmul2 = f2_splat(p.sm_scale * LOG2E);
+    // 2^P_SHIFT p (dp - D) 2^-P_SHIFT: the factor of p costs ds nothing
+    const auto minus_d = [](uint32_t y0, uint32_t y1, uint64_t nd) {
+      if constexpr (BF16) return f2_add(f2_bits(y0, y1), nd);
+      else return f2_fma(f2_bits(y0, y1), f2_splat(P_UNSHIFT<BF16>), nd);
+    };
     bool ok = true;
     for (int i = 0; ok && i < n; ++i) {
       const ulonglong2* stat = reinterpret_cast<const ulonglong2*>(smem + KV_OFF_STAT + (i % 2) * 1024 + cg * 128);  // four queries each
@@ -800,8 +810,8 @@ attn_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
           const ulonglong2 nd = stat[32 + 4 * c + k / 4];
           const uint32_t* x = &sv[16 * c + k];
           const uint32_t* y = &dp[16 * c + k];
-          pk[k / 2] = f2_to16_rn<BF16>(f2_mul(f2_bits(x[0], x[1]), f2_add(f2_bits(y[0], y[1]), nd.x)));
-          pk[k / 2 + 1] = f2_to16_rn<BF16>(f2_mul(f2_bits(x[2], x[3]), f2_add(f2_bits(y[2], y[3]), nd.y)));
+          pk[k / 2] = f2_to16_rn<BF16>(f2_mul(f2_bits(x[0], x[1]), minus_d(y[0], y[1], nd.x)));
+          pk[k / 2 + 1] = f2_to16_rn<BF16>(f2_mul(f2_bits(x[2], x[3]), minus_d(y[2], y[3], nd.y)));
         }
         tmem_st8(tm + lanes + T_DP + cg * 32 + 8 * c, pk);
         tmem_wait_st();
@@ -822,7 +832,7 @@ attn_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
         tmem_ld32(tm + lanes + (c == 0 ? T_DK : T_DV) + cg * 32, v);
         tmem_wait_ld();
         if (p.splits > 1) store_part32(st, v, 1.f, live, part + (c == 0 ? 0 : part_all) + row0 * 128 + cg * 32, rows);
-        else store_cols32<BF16>(st, v, c == 0 ? mul : 1.f, live, out_ptr(c == 0 ? p.dk : p.dv, b, h, k0 + row0) + cg * 32, (c == 0 ? p.dk : p.dv).st, rows);
+        else store_cols32<BF16>(st, v, c == 0 ? mul : P_UNSHIFT<BF16>, live, out_ptr(c == 0 ? p.dk : p.dv, b, h, k0 + row0) + cg * 32, (c == 0 ? p.dk : p.dv).st, rows);
       }
     }
   }
@@ -1092,7 +1102,13 @@ __global__ void __launch_bounds__(256) attn_fwd_join_kernel(const TrainParams p)
   if (c == 0) p.lse[row] = top == -INFINITY ? -INFINITY : (top + log2f(total)) * LN2;
 }
 
-struct JoinTarget { Rows out; const float* part; const int* k_lens; float mul; };
+struct JoinTarget {
+  Rows out;
+  const float* part;
+  const int* k_lens;
+  float mul;
+  bool scores;  // dq, dk: a gradient through the scores, zero where there is one key only
+};
 template <bool BF16>
 __global__ void __launch_bounds__(256) attn_bwd_join_kernel(const JoinTarget t0, const JoinTarget t1, int splits, int64_t rows,
                                                             int S, int heads, int Sk) {
@@ -1108,8 +1124,7 @@ __global__ void __launch_bounds__(256) attn_bwd_join_kernel(const JoinTarget t0,
     acc.z += v.z;
     acc.w += v.w;
   }
-  // t.mul 1: dv.  Otherwise a gradient through the scores, zero where there is one key only
-  const float mul = t.k_lens == nullptr && Sk == 1 ? 0.f : t.k_lens != nullptr && valid_len(t.k_lens, b, Sk) == 1 ? 0.f : t.mul;
+  const float mul = t.scores && valid_len(t.k_lens, b, Sk) == 1 ? 0.f : t.mul;
   store4<BF16>(out_ptr(t.out, b, bh % heads, s) + c, acc, mul);
 }
 
@@ -1222,7 +1237,7 @@ int run_backward(const CUtensorMap& mq, const CUtensorMap& mdo, const CUtensorMa
   DAX_CUDA(cudaGetLastError());
   if (s_q > 1) {
     const int64_t rows = static_cast<int64_t>(BH) * p.Sq;
-    const JoinTarget t = {p.dq, part_q, p.k_lens, p.sm_scale};
+    const JoinTarget t = {p.dq, part_q, p.k_lens, p.sm_scale, true};
     attn_bwd_join_kernel<BF16><<<dim3(static_cast<unsigned>(tiles_of(rows, 8)), 1), 256, 0, st>>>(t, t, s_q, rows, p.Sq, p.heads, p.Sk);
     DAX_CUDA(cudaGetLastError());
   }
@@ -1233,7 +1248,8 @@ int run_backward(const CUtensorMap& mq, const CUtensorMap& mdo, const CUtensorMa
   DAX_CUDA(cudaGetLastError());
   if (s_kv > 1) {
     const int64_t rows = static_cast<int64_t>(BH) * p.Sk;
-    const JoinTarget tk = {p.dk, part_kv, p.k_lens, p.sm_scale}, tv = {p.dv, part_kv + s_kv * rows * 128, nullptr, 1.f};
+    const JoinTarget tk = {p.dk, part_kv, p.k_lens, p.sm_scale, true},
+                     tv = {p.dv, part_kv + s_kv * rows * 128, p.k_lens, P_UNSHIFT<BF16>, false};
     attn_bwd_join_kernel<BF16><<<dim3(static_cast<unsigned>(tiles_of(rows, 8)), 2), 256, 0, st>>>(tk, tv, s_kv, rows, p.Sk, p.heads, p.Sk);
     DAX_CUDA(cudaGetLastError());
   }

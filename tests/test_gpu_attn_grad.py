@@ -258,3 +258,27 @@ def test_empty_axes(ops):
     out, lse = ops.attention_lse(q[:, :, :0], k, v)
     _, dk, dv = ops.attention_backward(do[:, :, :0], q[:, :, :0], k, v, out, lse)
     assert out.shape[2] == 0 and not dk.any() and not dv.any()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("lens", [None, [1, 1], [0, 1]])
+def test_one_key_and_many_queries(ops, dtype, lens):
+    """The queries are split over CTAs: the joined gradients through the scores are zero, that of the value is not."""
+    q, k, v, do = make(2, 1, 6000, 1 if lens is None else 3, dtype, seed=14)
+    lens = None if lens is None else torch.tensor(lens, dtype=torch.int32, device=DEV)
+    check(run(ops, q, k, v, do, k_lens=lens), *reference(q, k, v, do, None, lens, 1 / math.sqrt(128)))
+
+
+@pytest.mark.parametrize("rows", [128, 2000])
+def test_fp16_probabilities_of_long_rows(ops, rows):
+    """Equal probabilities of 1 / 225,000, 74.6 steps of the smallest fp16 numbers: they are rounded as normal numbers."""
+    S = 225000
+    g = torch.Generator(device=DEV).manual_seed(15)
+    q = torch.zeros(1, 1, rows, 128, dtype=torch.float16, device=DEV)
+    k, v = (torch.randn(1, 1, S, 128, generator=g, device=DEV).half() for _ in range(2))
+    do = (64 * torch.rand(1, 1, rows, 128, generator=g, device=DEV)).half()
+    dv = run(ops, q, k, v, do)[4].double()
+    want = do.double().sum(2, keepdim=True) / S
+    # the rounding of p, its exponential and that of lse (log 225,000 = 12.3: 2^-21), the additions, the rounding of the result
+    bound = want * (2.0 ** -11 + 2.0 ** -20 + 2.0 ** -20 + rows * W) * (1 + 2.0 ** -10) + want * 2.0 ** -11 + 2.0 ** -25
+    assert bool(((dv - want).abs() <= bound).all())
