@@ -217,6 +217,8 @@ __device__ __forceinline__ uint32_t open_tmem(uint32_t* slot, bool owner) {
   return *slot;
 }
 __device__ __forceinline__ void close_tmem(uint32_t base, bool owner, volatile uint32_t* abort_flag, int* status) {
+  if (*abort_flag)  // a wait gave up: copies and products in flight land (a millisecond) before the block returns its memory
+    for (int i = 0; i < 1000; ++i) __nanosleep(1000);
   tc_fence_before_sync();
   __syncthreads();
   if (owner) {

@@ -349,6 +349,7 @@ __global__ void __launch_bounds__(Shape<DT, ELEMS, false>::T, Shape<DT, ELEMS, f
     stage = stage == STAGES - 1 ? 0 : stage + 1;
     parity ^= 1;
   }
+  cp_async_wait<0>();  // the zeros behind the last row have arrived before the CTA gives back its memory
 }
 
 // ---- backward --------------------------------------------------------------------------------------------------------
@@ -500,6 +501,7 @@ __global__ void __launch_bounds__(Shape<DT, ELEMS, true>::T, Shape<DT, ELEMS, tr
     stage = stage == STAGES - 1 ? 0 : stage + 1;
     parity ^= 1;
   }
+  cp_async_wait<0>();  // the zeros behind the last row have arrived before the CTA gives back its memory
   if constexpr (SUMS > 0) {
     float* part = p.part + (static_cast<int64_t>(b) * gridDim.x + blockIdx.x) * SUMS * p.D + tid * E;
 #pragma unroll
