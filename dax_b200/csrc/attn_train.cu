@@ -196,13 +196,13 @@ __device__ __forceinline__ uint32_t idesc_k() { return make_idesc(1, BF16 ? 1 : 
 template <bool BF16>
 __device__ __forceinline__ uint32_t idesc_mn() { return idesc_k<BF16>() | (1u << 16); }  // B is MN-major
 
-// Half `c` of such a product whose A operand is in four groups of 32 columns, 16 of them used, each by one row warp for 32 of
-// the tile's rows: the groups' first (c = 0) or second 16 rows.
+// Half `c` of such a product whose A operand comes from four row warps, each with 16 columns for 32 of the tile's rows: the
+// first (c = 0) or the second 16 rows of each.
 __device__ __forceinline__ void mma_ts_mn_half(uint32_t d, uint32_t a_tmem, int c, uint32_t b_smem, uint32_t idesc, bool first) {
   const uint64_t b = make_desc_mn_sw128(b_smem, BOX_BYTES);
 #pragma unroll
   for (int g = 0; g < 4; ++g)
-    umma_ts_f16(d, a_tmem + 32 * g + 8 * c, b + static_cast<uint64_t>((2 * g + c) * ((16 * 128) >> 4)), idesc, (!first || g != 0) ? 1u : 0u);
+    umma_ts_f16(d, a_tmem + 16 * g + 8 * c, b + static_cast<uint64_t>((2 * g + c) * ((16 * 128) >> 4)), idesc, (!first || g != 0) ? 1u : 0u);
 }
 
 // Set-up and tear-down shared by the kernels
@@ -575,11 +575,11 @@ attn_bwd_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
 // One CTA = 128 keys of one head; k and v stay in shared memory, q and do tiles pass through the ring.  Everything is
 // transposed: a thread owns a KEY row x 32 queries, so p^T and ds^T come out as A operands of dv += p^T.do and
 // dk += ds^T.q and never leave tensor memory; lse and D of the queries are read along the row.
-//   issuer 0     s^T = k.q_i^T and dv += p^T.do_i        issuer 1     dp^T = v.do_i^T and dk += ds^T.q_i
-// Tensor memory: s^T [0,128), p^T over it   dp^T [128,256), ds^T over it   dv [256,384)   dk [384,512): all of it, so s^T of
-// the next tile has to wait for dv of this one, which waits for the exponentials: that chain is the period.  It is kept
-// short by handing p^T over in halves (the first half's product runs under the second half's exponentials) and by issuing
-// the next s^T ahead of this tile's dk.
+//   issuer 0     s^T = k.q_i^T and dp^T = v.do_i^T        issuer 1     dv += p^T.do_i and dk += ds^T.q_i
+// Tensor memory: s^T, then dp^T in the same place [0,128)   p^T [128,192)   ds^T [192,256)   dv [256,384)   dk [384,512): all
+// of it.  s^T and dp^T are free as soon as they are in registers: dp^T is computed under the exponentials, s^T of the next
+// tile under the arithmetic of ds^T, and neither waits for a product that reads p^T or ds^T.  Those are handed over in
+// halves, so that the first half's product runs under the second half's arithmetic.
 constexpr int KV_SLOTS = 4;
 constexpr int KV_OFF_K = KV_SLOTS * TILE_BYTES;
 constexpr int KV_OFF_V = KV_OFF_K + TILE_BYTES;
@@ -623,11 +623,12 @@ attn_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
   uint64_t* k_full = tail + 1;
   uint64_t* v_full = k_full + 1;
   uint64_t* s_full = v_full + 1;
-  uint64_t* s_issued = s_full + 1;
-  uint64_t* p_full = s_issued + 1;      // [2] halves of every thread's queries
+  uint64_t* s_free = s_full + 1;
+  uint64_t* p_full = s_free + 1;        // [2] halves of every thread's queries
   uint64_t* dv_done = p_full + 2;
   uint64_t* dp_full = dv_done + 1;
-  uint64_t* ds_full = dp_full + 1;      // [2]
+  uint64_t* dp_free = dp_full + 1;
+  uint64_t* ds_full = dp_free + 1;      // [2]
   uint64_t* dk_done = ds_full + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(dk_done + 1);
   volatile uint32_t* abort_flag = tmem_slot + 1;
@@ -644,9 +645,10 @@ attn_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
     mbar_init(k_full, 1);
     mbar_init(v_full, 1);
     mbar_init(s_full, 1);
-    mbar_init(s_issued, 1);
+    mbar_init(s_free, ROW_WARPS_B);
     mbar_init(dv_done, 1);
     mbar_init(dp_full, 1);
+    mbar_init(dp_free, ROW_WARPS_B);
     mbar_init(dk_done, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&p_full[i], ROW_WARPS_B);
@@ -661,7 +663,7 @@ attn_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
     issue_tile({smem + KV_OFF_V, &map_v, k0, h, b}, v_full);
   }
   const uint32_t tm = open_tmem(tmem_slot, warp == W::tmem);
-  constexpr uint32_t T_S = 0, T_DP = 128, T_DV = 256, T_DK = 384;
+  constexpr uint32_t T_S = 0, T_P = 128, T_DS = 192, T_DV = 256, T_DK = 384;
   const int64_t stats = static_cast<int64_t>(p.B) * p.heads * p.Sq_pad;
 
   if (warp >= W::producer) {
@@ -692,26 +694,40 @@ attn_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
       }
     } else if (warp == W::issuer0) {
       const bool leader = elect_one();
-      const uint32_t ring = smem_u32(smem), id = idesc_k<BF16>(), id_mn = idesc_mn<BF16>();
+      const uint32_t ring = smem_u32(smem), id = idesc_k<BF16>();
       bool ok = mbar_wait(k_full, 0, abort_flag);
       for (int i = 0; ok && i < n; ++i) {
         const uint32_t seq = 2 * i, s = seq % KV_SLOTS, ph = (seq / KV_SLOTS) & 1u, s1 = (seq + 1) % KV_SLOTS, ph1 = ((seq + 1) / KV_SLOTS) & 1u;
-        // s^T lies where p^T of the last tile was read: that product has to be over
-        ok = mbar_wait(&full[s], ph, abort_flag) && (i == 0 || mbar_wait(dv_done, (i - 1) & 1u, abort_flag));
+        ok = mbar_wait(&full[s], ph, abort_flag) && (i == 0 || mbar_wait(dp_free, (i - 1) & 1u, abort_flag));
         if (!ok) break;
         tc_fence_after_sync();
         if (leader) {
           mma_ss(tm + T_S, ring + KV_OFF_K, ring + s * TILE_BYTES, id);
           umma_commit(s_full);
           umma_commit(&empty[s]);
-          mbar_arrive(s_issued);
         }
         __syncwarp();
+        ok = (i > 0 || mbar_wait(v_full, 0, abort_flag)) && mbar_wait(&full[s1], ph1, abort_flag) && mbar_wait(s_free, i & 1u, abort_flag);
+        if (!ok) break;
+        tc_fence_after_sync();
+        if (leader) {
+          mma_ss(tm + T_S, ring + KV_OFF_V, ring + s1 * TILE_BYTES, id);
+          umma_commit(dp_full);
+          umma_commit(&empty[s1]);
+        }
+        __syncwarp();
+      }
+    } else if (warp == W::issuer1) {
+      const bool leader = elect_one();
+      const uint32_t ring = smem_u32(smem), id_mn = idesc_mn<BF16>();
+      bool ok = true;
+      for (int i = 0; ok && i < n; ++i) {
+        const uint32_t seq = 2 * i, s = seq % KV_SLOTS, ph = (seq / KV_SLOTS) & 1u, s1 = (seq + 1) % KV_SLOTS, ph1 = ((seq + 1) / KV_SLOTS) & 1u;
         ok = mbar_wait(&full[s1], ph1, abort_flag);
         for (int c = 0; ok && c < 2; ++c) {
           if (!(ok = mbar_wait(&p_full[c], i & 1u, abort_flag))) break;
           tc_fence_after_sync();
-          if (leader) mma_ts_mn_half(tm + T_DV, tm + T_S, c, ring + s1 * TILE_BYTES, id_mn, i == 0 && c == 0);
+          if (leader) mma_ts_mn_half(tm + T_DV, tm + T_P, c, ring + s1 * TILE_BYTES, id_mn, i == 0 && c == 0);
           __syncwarp();
         }
         if (!ok) break;
@@ -720,28 +736,11 @@ attn_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
           umma_commit(&empty[s1]);
         }
         __syncwarp();
-      }
-    } else if (warp == W::issuer1) {
-      const bool leader = elect_one();
-      const uint32_t ring = smem_u32(smem), id = idesc_k<BF16>(), id_mn = idesc_mn<BF16>();
-      bool ok = mbar_wait(v_full, 0, abort_flag) && mbar_wait(s_issued, 0, abort_flag);
-      for (int i = 0; ok && i < n; ++i) {
-        const uint32_t seq = 2 * i, s = seq % KV_SLOTS, ph = (seq / KV_SLOTS) & 1u, s1 = (seq + 1) % KV_SLOTS, ph1 = ((seq + 1) / KV_SLOTS) & 1u;
-        ok = mbar_wait(&full[s1], ph1, abort_flag) && (i == 0 || mbar_wait(dk_done, (i - 1) & 1u, abort_flag));
-        if (!ok) break;
-        tc_fence_after_sync();
-        if (leader) {
-          mma_ss(tm + T_DP, ring + KV_OFF_V, ring + s1 * TILE_BYTES, id);
-          umma_commit(dp_full);
-          umma_commit(&empty[s1]);
-        }
-        __syncwarp();
-        // s^T of the next tile goes first: the exponentials wait for it, nothing waits for dk
-        ok = mbar_wait(&full[s], ph, abort_flag) && (i + 1 == n || mbar_wait(s_issued, (i + 1) & 1u, abort_flag));
+        ok = mbar_wait(&full[s], ph, abort_flag);
         for (int c = 0; ok && c < 2; ++c) {
           if (!(ok = mbar_wait(&ds_full[c], i & 1u, abort_flag))) break;
           tc_fence_after_sync();
-          if (leader) mma_ts_mn_half(tm + T_DK, tm + T_DP, c, ring + s * TILE_BYTES, id_mn, i == 0 && c == 0);
+          if (leader) mma_ts_mn_half(tm + T_DK, tm + T_DS, c, ring + s * TILE_BYTES, id_mn, i == 0 && c == 0);
           __syncwarp();
         }
         if (!ok) break;
@@ -772,6 +771,9 @@ attn_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
       uint32_t sv[32];
       tmem_ld32(tm + lanes + T_S + cg * 32, sv);
       tmem_wait_ld();
+      tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(s_free);
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         uint32_t pk[8];
@@ -793,17 +795,24 @@ attn_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
           pk[k / 2] = pack2_rn<BF16>(a0, a1);
           pk[k / 2 + 1] = pack2_rn<BF16>(a2, a3);
         }
-        tmem_st8(tm + lanes + T_S + cg * 32 + 8 * c, pk);
+        if (c == 0 && i > 0) {  // p of the last tile has been read (normally long ago)
+          if (!(ok = mbar_wait(dv_done, (i - 1) & 1u, abort_flag))) break;
+          tc_fence_after_sync();
+        }
+        tmem_st8(tm + lanes + T_P + cg * 16 + 8 * c, pk);
         tmem_wait_st();
         tc_fence_before_sync();
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[c]);
       }
-      if (!(ok = mbar_wait(dp_full, i & 1u, abort_flag))) break;
+      if (!ok || !(ok = mbar_wait(dp_full, i & 1u, abort_flag))) break;
       tc_fence_after_sync();
       uint32_t dp[32];
-      tmem_ld32(tm + lanes + T_DP + cg * 32, dp);
+      tmem_ld32(tm + lanes + T_S + cg * 32, dp);
       tmem_wait_ld();
+      tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(dp_free);
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         uint32_t pk[8];
@@ -815,7 +824,11 @@ attn_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
           pk[k / 2] = f2_to16_rn<BF16>(f2_mul(f2_bits(x[0], x[1]), minus_d(y[0], y[1], nd.x)));
           pk[k / 2 + 1] = f2_to16_rn<BF16>(f2_mul(f2_bits(x[2], x[3]), minus_d(y[2], y[3], nd.y)));
         }
-        tmem_st8(tm + lanes + T_DP + cg * 32 + 8 * c, pk);
+        if (c == 0 && i > 0) {  // and so has ds
+          if (!(ok = mbar_wait(dk_done, (i - 1) & 1u, abort_flag))) break;
+          tc_fence_after_sync();
+        }
+        tmem_st8(tm + lanes + T_DS + cg * 16 + 8 * c, pk);
         tmem_wait_st();
         tc_fence_before_sync();
         __syncwarp();
