@@ -23,6 +23,7 @@
 #include <algorithm>
 #include <atomic>
 #include <cmath>
+#include <type_traits>
 
 #include "quant_common.cuh"
 #include "sm100_ptx.cuh"
@@ -244,6 +245,11 @@ __device__ __forceinline__ void close_tmem(uint32_t base, bool owner, volatile u
 // dq, but the roundings of ds have: their sum times the offset would be the largest error by far.  The kernel adds up the
 // rounded ds of each row, e_i, and subtracts e_i m for an m near the mean key (the first tile's), which is what rounding
 // left of it.
+//
+// D is taken from the rounded o.  What that rounding leaves in ds, p_ij times one number per row, is well below the rounding
+// of ds as long as a row spreads over many keys (from 64 keys on the error of dk does not show it), but with two keys it
+// made dk 2.3 times as inexact as a single rounding.  Where all keys lie in one tile the kernel has sum_j p_ij dp_ij, which is
+// D, at hand, and takes that.
 constexpr int DQ_SLOTS = 6;
 constexpr int DQ_OFF_Q = DQ_SLOTS * TILE_BYTES;
 constexpr int DQ_OFF_MEAN = DQ_OFF_Q;               // [16][128] floats: sums of keys, in the end m in the first row; over q
@@ -306,7 +312,8 @@ attn_bwd_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
   uint64_t* ds_full = dp_free + 1;
   uint64_t* dq_done = ds_full + 1;
   uint64_t* turn = dq_done + 1;          // [2]
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(turn + 2);
+  uint64_t* sums_full = turn + 2;        // one tile of keys: the column groups' sums are in tensor memory
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sums_full + 1);
   volatile uint32_t* abort_flag = tmem_slot + 1;
   uint8_t* do_smem = smem + (DQ_SLOTS - 2) * TILE_BYTES;
   uint8_t* o_smem = smem + (DQ_SLOTS - 1) * TILE_BYTES;
@@ -334,6 +341,7 @@ attn_bwd_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
     mbar_init(dq_done, 1);
     mbar_init(&turn[0], ROW_WARPS_B / 2);
     mbar_init(&turn[1], ROW_WARPS_B / 2);
+    mbar_init(sums_full, ROW_WARPS_B);
     *abort_flag = 0;
     mbar_fence_init();
     // the first loads are under way while tensor memory is set up
@@ -451,12 +459,13 @@ attn_bwd_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
       stat[r] = nl + P_SHIFT<BF16>;
       stat[stats + r] = nd * P_UNSHIFT<BF16>;
     }
-    const uint64_t nl2 = f2_splat(nl), nd2 = f2_splat(nd), cmul2 = f2_splat(p.sm_scale * LOG2E);
+    const uint64_t nl2 = f2_splat(nl), cmul2 = f2_splat(p.sm_scale * LOG2E);
+    uint64_t nd2 = f2_splat(nd);
     float e[2] = {0.f, 0.f};  // sums of the rounded ds
     const int team = warp >> 3;
-    for (int j = 0; ok && j < n; ++j) {
+    const auto tile = [&](int j, auto only) -> bool {  // the arithmetic of a tile of keys; false: a wait gave up
       const int valid = k_len - (j0 + j) * 128 - cg * 32;  // this thread's columns that exist
-      if (!(ok = mbar_wait(s_full, j & 1u, abort_flag))) break;
+      if (!mbar_wait(s_full, j & 1u, abort_flag)) return false;
       tc_fence_after_sync();
       uint32_t sv[32];
       tmem_ld32(tm + lanes + T_S + cg * 32, sv);
@@ -465,7 +474,7 @@ attn_bwd_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
       __syncwarp();
       if (lane == 0) mbar_arrive(s_free);
       // turn[0] opens the exponentials of team 0 (team 1 has done its last tile's), turn[1] those of team 1
-      if ((team == 1 || j > 0) && !(ok = mbar_wait(&turn[team], (team == 1 ? j : j - 1) & 1u, abort_flag))) break;
+      if ((team == 1 || j > 0) && !mbar_wait(&turn[team], (team == 1 ? j : j - 1) & 1u, abort_flag)) return false;
 #pragma unroll
       for (int i = 0; i < 32; i += 2) {
         float a, c;
@@ -475,7 +484,7 @@ attn_bwd_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&turn[team ^ 1]);
-      if (!(ok = mbar_wait(dp_full, j & 1u, abort_flag))) break;
+      if (!mbar_wait(dp_full, j & 1u, abort_flag)) return false;
       tc_fence_after_sync();
       uint32_t dp[32];
       tmem_ld32(tm + lanes + T_DP + cg * 32, dp);
@@ -490,6 +499,26 @@ attn_bwd_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
           dp[i] = i < valid ? dp[i] : 0u;
         }
       }
+      if constexpr (decltype(only)::value) {  // what sum_j p (dp - D) is off zero, D is off
+        uint64_t off2 = f2_splat(0.f);
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          off2 = f2_fma(f2_bits(sv[2 * i], sv[2 * i + 1]), f2_add(f2_bits(dp[2 * i], dp[2 * i + 1]), nd2), off2);
+        float a, c;
+        f2_unpack(off2, a, c);
+        tmem_st1(tm + lanes + T_DP + cg * 32, __float_as_uint(a + c));  // where this warp has read its dp
+        tmem_wait_st();
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(sums_full);
+        if (!mbar_wait(sums_full, 0, abort_flag)) return false;
+        tc_fence_after_sync();
+        const float off = sum_of_groups(tm + lanes + T_DP);  // by the whole warp, rows that do not exist included
+        f2_unpack(nd2, a, c);
+        a = live ? a - off : 0.f;  // a row behind the length holds anything
+        nd2 = f2_splat(a);
+        if (cg == 0) stat[stats + r] = a * P_UNSHIFT<BF16>;  // split 0 has the tile
+      }
       uint32_t pk[16];
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
@@ -497,7 +526,7 @@ attn_bwd_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
         add_pair<BF16>(e[i & 1], pk[i]);
       }
       if (j > 0) {  // ds of the last tile has been read (normally long ago)
-        if (!(ok = mbar_wait(dq_done, (j - 1) & 1u, abort_flag))) break;
+        if (!mbar_wait(dq_done, (j - 1) & 1u, abort_flag)) return false;
         tc_fence_after_sync();
       }
       tmem_st16(tm + lanes + T_DS + cg * 16, pk);
@@ -505,7 +534,12 @@ attn_bwd_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
       tc_fence_before_sync();
       __syncwarp();
       if (lane == 0) mbar_arrive(ds_full);
-    }
+      return true;
+    };
+    // two copies: with the sum over the row as a branch in the loop the backward pass took 2 to 3 % longer at every length
+    if (n_all == 1) ok = ok && tile(0, std::true_type{});
+    else
+      for (int j = 0; ok && j < n; ++j) ok = tile(j, std::false_type{});
     // m: the mean of the first tile's keys; a thread adds eight channels of four keys
     if (ok) ok = mbar_wait(&full[(2 * n) % DQ_SLOTS], ((2 * n) / DQ_SLOTS) & 1u, abort_flag);
     {

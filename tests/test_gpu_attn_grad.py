@@ -46,8 +46,9 @@ def make(B, H, Sq, Sk, dtype, seed=0, offset=2.0):
     return [x.to(DEV) for x in (q, k, v, do)]
 
 
-def reference(q, k, v, do, q_lens, k_lens, c):
-    """Results and their error bounds; padded tokens are replaced by zeros first (they take no part)."""
+def reference(q, k, v, do, q_lens, k_lens, c, one_tile=False):
+    """Results and their error bounds; padded tokens are replaced by zeros first (they take no part).  ``one_tile``: with at
+    most 128 keys D is not taken from the rounded ``out`` but as sum_j p dp."""
     B, H, Sq, _ = q.shape
     Sk = k.shape[2]
     t = q.dtype
@@ -71,6 +72,11 @@ def reference(q, k, v, do, q_lens, k_lens, c):
     r = lambda x: u * x.abs() * (1 + 2 * u) + tiny  # the rounding of a result
     b_out = r(out) + (1 + u) * ((u + e + Sk * W) * (p @ va) + tiny * va.sum(2, keepdim=True))
     b_D = (da * b_out).sum(3, keepdim=True) + 128 * W * (da * out.abs()).sum(3, keepdim=True)
+    if one_tile:
+        # D as D' + sum_j p (dp - D') for a D' that is at most u |do||out| away: the errors of p (e), of dp (128 w) and of the
+        # fp32 arithmetic (2^-18 covers 128 additions)
+        b_D = (p * ((e + 2.0 ** -18) * (dp.abs() + 2 * D.abs()) + 128 * W * (da @ va.transpose(2, 3)))).sum(3, keepdim=True)
+        b_D = b_D + (e + 2.0 ** -18) * (D.abs() + (da * out.abs()).sum(3, keepdim=True) * 2 * u)
     b_ds = torch.where(seen, (u + e) * ds.abs() + p * (128 * W * (da @ va.transpose(2, 3)) + b_D) * (1 + u) + tiny, 0.0)
     b_ds = torch.where(one, 0.0, b_ds)
     # dq is summed as r k - (sum of r) m with the rounded ds r and m the mean of the first (up to 128) keys; the exact ds of a
@@ -282,3 +288,12 @@ def test_fp16_probabilities_of_long_rows(ops, rows):
     # the rounding of p, its exponential and that of lse (log 225,000 = 12.3: 2^-21), the additions, the rounding of the result
     bound = want * (2.0 ** -11 + 2.0 ** -20 + 2.0 ** -20 + rows * W) * (1 + 2.0 ** -10) + want * 2.0 ** -11 + 2.0 ** -25
     assert bool(((dv - want).abs() <= bound).all())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("B,H,Sq,Sk,k_lens", [(1, 2, 300, 2, None), (2, 1, 8, 8, None), (1, 1, 50, 128, None), (3, 2, 200, 300, [2, 128, 1]),
+                                              (2, 1, 100, 3000, [5, 64]), (1, 1, 5000, 16, None)])
+def test_few_keys_do_not_feel_the_rounding_of_out(ops, B, H, Sq, Sk, k_lens, dtype):
+    q, k, v, do = make(B, H, Sq, Sk, dtype, seed=16)
+    lens = None if k_lens is None else torch.tensor(k_lens, dtype=torch.int32, device=DEV)
+    check(run(ops, q, k, v, do, k_lens=lens), *reference(q, k, v, do, None, lens, 1 / math.sqrt(128), one_tile=True))
