@@ -8,7 +8,8 @@ modules the model has (their products are library GEMMs), so adapters around the
 training path; the formulas are those of the block that ``dax/adapters/wan/transformer_adapter.py:127-134`` loops over and
 of the processor ``dax/adapters/wan/attn_adapter.py:62-304``.
 
-Quantised linears have no gradient and the sequence-parallel exchange has no backward pass here: both are refused."""
+Quantised linears have no gradient, the sequence-parallel exchange has no backward pass here, and the forward that
+``optimize_pipe`` binds on the transformer ends in an operator without one: all three are refused."""
 from __future__ import annotations
 
 import types
@@ -21,6 +22,7 @@ from ...parallel import dist as para_dist
 from ...quant.nn.dynamic import Linear as QLinear
 from .attn_adapter import HEAD_DIM, _rope_tables
 from .block_adapter import _block_classes
+from .transformer_adapter import dit_forward
 
 
 class DAXWanTrainingAttnProcessor:
@@ -87,6 +89,9 @@ def enable_training(pipe) -> int:
     for name, m in pipe.transformer.named_modules():
         if isinstance(m, QLinear):
             raise NotImplementedError(f"{name} is quantised and has no gradient: enable training before quantising")
+    if getattr(getattr(pipe.transformer, "forward", None), "__func__", None) is dit_forward:
+        raise NotImplementedError("the transformer has the inference forward of optimize_pipe, which has no gradient: enable training on a pipe "
+                                  "that has not been optimised")
     n = 0
     for _, m in pipe.transformer.named_modules():
         if isinstance(m, _block_classes()):

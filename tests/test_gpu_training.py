@@ -224,3 +224,36 @@ def test_training_step_captured_into_a_graph(ag):
         eager = step(fresh)
         for n in eager:
             assert torch.equal(captured[n], eager[n]), n
+
+
+def test_whole_model_trains(ag):
+    """Loss and gradients of a small DiT through the public calls; the criterion is that of the blocks' test, for gradients
+    that have enough elements for it (4,096).  The others exist and are finite."""
+    import types
+    from dax_b200.adapters.wan.modules import WanDiT, _Pipe
+    from dax_b200.adapters.wan.training import enable_training
+    torch.manual_seed(3)
+    net = WanDiT(layers=2, dim=256, ffn_dim=512, heads=2, text_dim=64, freq_dim=64).bfloat16()
+    latents, target = (torch.randn(2, 16, 2, 8, 16).bfloat16().to(DEV) for _ in range(2))
+    text, timestep = torch.randn(2, 20, 64).bfloat16().to(DEV), torch.tensor([900.0, 100.0], device=DEV)
+    grads = []
+    for kind in ("exact", "plain", "kernels"):
+        m = copy.deepcopy(net).to(DEV)
+        t = (lambda x: x.double()) if kind == "exact" else (lambda x: x)  # noqa: E731
+        if kind == "exact":
+            m = m.double()
+        if kind == "kernels":
+            assert enable_training(_Pipe(m)) == 2
+        else:
+            for b in m.blocks:
+                b.attn1.processor = b.attn2.processor = PlainProcessor()
+                b.forward = types.MethodType(_plain_block, b)
+        out = m(t(latents), timestep, t(text))[0]
+        (out - t(target)).square().mean().backward()
+        grads.append({n: p.grad for n, p in m.named_parameters()})
+    exact, plain, own = grads
+    for n in exact:
+        assert own[n] is not None and torch.isfinite(own[n]).all(), n
+        if exact[n].numel() >= 4096:
+            e_plain, e_own = ((r[n].double() - exact[n]).norm() / exact[n].norm() for r in (plain, own))
+            assert e_own <= 1.5 * e_plain + 2 * 2.0 ** -9, (n, float(e_plain), float(e_own))

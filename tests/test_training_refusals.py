@@ -127,3 +127,15 @@ def test_wrappers_refuse_wrong_tensors():
         ops.rmsnorm_rope(x[..., :200], rope_cos=t, rope_sin=t)
     with pytest.raises(ValueError):
         ops.rmsnorm_rope(x[0, 0])
+
+
+def test_an_optimised_pipe_is_not_trained():
+    """Its forward ends in a quantising operator: gradients would stop there without a word."""
+    from dax_b200.adapters.wan.modules import WanDiT, _Pipe
+    from dax_b200.adapters.wan.training import enable_training
+    from dax_b200.adapters.wan.transformer_adapter import replace_transformer
+    net = WanDiT(layers=1, dim=128, ffn_dim=128, heads=1, text_dim=32, freq_dim=32)
+    assert enable_training(_Pipe(net)) == 1
+    replace_transformer(net)
+    with pytest.raises(NotImplementedError, match="inference forward"):
+        enable_training(_Pipe(net))
