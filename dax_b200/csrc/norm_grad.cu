@@ -20,6 +20,11 @@
 // What a row costs beside its bytes is the wait for its sums (shuffles, one barrier): two rows share one where registers and
 // shared memory allow, and two to four CTAs per SM fill each other's waits.
 // Statistics, coefficients and sums are fp32; y and dx are rounded once, when they are stored.
+//
+// Measured (x and y, or x, dy and dx, once each; a plain copy reaches 6.5 TB/s): 32,760 x 5,120 bf16 LayerNorm + modulation
+// 117 us (5.7 TB/s) forward, 191 (5.3) backward with its sums, RMSNorm + rotation 111 (6.0) and 211 (4.8); 6,240 x 5,120 fp32
+// 53 (4.9) and 89 (4.3).  What is left beside the bytes is issue slots (58 % used in the backward pass, two rounds over a row
+// that lives in shared memory) and the waits for a row's sums.
 #include <algorithm>
 
 #include "quant_common.cuh"
