@@ -26,6 +26,7 @@
 // 53 (4.9) and 89 (4.3).  What is left beside the bytes is issue slots (58 % used in the backward pass, two rounds over a row
 // that lives in shared memory) and the waits for a row's sums.
 #include <algorithm>
+#include <atomic>
 
 #include "quant_common.cuh"
 
@@ -33,6 +34,7 @@ namespace dax {
 namespace {
 
 constexpr int64_t kMaxWidth = 8192;
+constexpr int kMaxSmem = 220 * 1024;  // of a CTA; the widest fp32 rows take 160 KB
 
 struct NormArgs {
   const uint8_t* x;       // input rows
@@ -602,11 +604,22 @@ inline int row_elems(int64_t D, int dtype, bool ln, bool backward) {
 // (more adds nothing to the bytes in flight, but partial sums to join).
 inline int64_t max_ctas(int64_t B, int64_t groups) { return std::min(groups, std::max<int64_t>(1, 8 * static_cast<int64_t>(sm_count()) / B)); }
 
-template <typename K>
-int launch_rows(K kernel, const NormArgs& p, int64_t B, int threads, size_t smem, int rows, int64_t* ctas, cudaStream_t st) {
-  if (smem > 40 * 1024) DAX_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
-  int per_sm = 0;
-  DAX_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, threads, smem));
+template <auto kernel>
+int launch_rows(const NormArgs& p, int64_t B, int threads, size_t smem, int rows, int64_t* ctas, cudaStream_t st) {
+  // The CTAs that fit an SM, asked for again when the device or the launch shape changes.
+  // (device + 1) << 48 | threads << 32 | shared memory << 8 | CTAs
+  static std::atomic<uint64_t> last{0};
+  int dev = 0;
+  DAX_CUDA(cudaGetDevice(&dev));
+  const uint64_t key = static_cast<uint64_t>(dev + 1) << 48 | static_cast<uint64_t>(threads) << 32 | static_cast<uint64_t>(smem) << 8;
+  const uint64_t known = last.load(std::memory_order_relaxed);
+  int per_sm = static_cast<int>(known & 0xff);
+  if ((known & ~uint64_t{0xff}) != key) {
+    // the same limit whatever the shape: calls of other threads may set it at the same time
+    DAX_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem));
+    DAX_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, threads, smem));
+    last.store(key | static_cast<uint64_t>(per_sm), std::memory_order_relaxed);
+  }
   *ctas = std::min(max_ctas(B, (p.S + rows - 1) / rows), std::max<int64_t>(1, static_cast<int64_t>(per_sm) * sm_count() / B));
   kernel<<<dim3(static_cast<unsigned>(*ctas), static_cast<unsigned>(B)), threads, smem, st>>>(p);
   DAX_CUDA(cudaGetLastError());
@@ -620,12 +633,12 @@ int run_shape(const NormArgs& p, int64_t B, int64_t* ctas, int sums, bool backwa
   const size_t row = static_cast<size_t>(threads) * ELEMS * (DT == DAX_F32 ? 4 : 2);
   if (!backward) {
     using Sh = Shape<DT, ELEMS, false>;
-    return launch_rows(norm_forward_kernel<DT, ELEMS, LN>, p, B, threads, row * Sh::STAGES * Sh::R + (LN ? 2 : 1) * coef, Sh::R, ctas, st);
+    return launch_rows<norm_forward_kernel<DT, ELEMS, LN>>(p, B, threads, row * Sh::STAGES * Sh::R + (LN ? 2 : 1) * coef, Sh::R, ctas, st);
   }
   using Sh = Shape<DT, ELEMS, true>;
   const size_t smem = row * Sh::STAGES * Sh::R * 2 + coef;
-  if (sums == 0) return launch_rows(norm_backward_kernel<DT, ELEMS, LN, 0>, p, B, threads, smem, Sh::R, ctas, st);
-  return launch_rows(norm_backward_kernel<DT, ELEMS, LN, LN ? 2 : 1>, p, B, threads, smem, Sh::R, ctas, st);
+  if (sums == 0) return launch_rows<norm_backward_kernel<DT, ELEMS, LN, 0>>(p, B, threads, smem, Sh::R, ctas, st);
+  return launch_rows<norm_backward_kernel<DT, ELEMS, LN, LN ? 2 : 1>>(p, B, threads, smem, Sh::R, ctas, st);
 }
 
 template <bool LN>

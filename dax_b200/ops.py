@@ -5,6 +5,7 @@ torch (the library itself never allocates) and enqueue on the current CUDA strea
 """
 from __future__ import annotations
 
+import functools
 import math
 from typing import Optional, Tuple
 
@@ -477,8 +478,35 @@ def _grad_like(what: str, dy: torch.Tensor, x: torch.Tensor) -> None:
         raise ValueError(f"{what}: dy must be {list(x.shape)} of {x.dtype}, got {list(dy.shape)} of {dy.dtype}")
 
 
+def _row_statistics(x: torch.Tensor, B: int, S: int) -> torch.Tensor:
+    """One fp32 number for each row (``torch.empty`` costs twice as much on the host)."""
+    size, strides = ((B, S), (S, 1)) if x.dim() == 3 else ((S,), (1,))
+    return torch.empty_strided(size, strides, dtype=torch.float32, device=x.device)
+
+
+@functools.lru_cache(maxsize=256)
+def _norm_workspace_bytes(device: int, B: int, S: int, D: int) -> int:
+    return load().dax_norm_backward_workspace_bytes(B, S, D)  # goes by the SM count of the current device, which is `device`
+
+
+@functools.lru_cache(maxsize=256)
+def _attention_workspace_bytes(device: int, backward: bool, B: int, heads: int, Sq: int, Sk: int) -> int:
+    lib = load()
+    return (lib.dax_attn_backward_workspace_bytes if backward else lib.dax_attn_lse_workspace_bytes)(B, heads, Sq, Sk)
+
+
+@functools.lru_cache(maxsize=1024)
+def _strides3(sample: int, head: int, token: int) -> I64x3:
+    """Three strides as the C entries read them."""
+    return I64x3(sample, head, token)
+
+
+def _workspace(n: int, device: torch.device) -> Optional[torch.Tensor]:
+    return torch.empty_strided((n,), (1,), dtype=torch.uint8, device=device) if n else None
+
+
 def _dense_like(t: torch.Tensor) -> torch.Tensor:
-    return torch.empty_like(t, memory_format=torch.contiguous_format)
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
 def layernorm_modulate(x: torch.Tensor, *, eps: float = 1e-6, ln_weight: Optional[torch.Tensor] = None,
@@ -497,7 +525,7 @@ def layernorm_modulate(x: torch.Tensor, *, eps: float = 1e-6, ln_weight: Optiona
     _vector(what, "scale", scale, modulation)
     dev = _on_one_device(what, x, ln_weight, ln_bias, shift, scale)
     y = _dense_like(x)
-    mean = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev)
+    mean = _row_statistics(x, B, S)
     rstd = torch.empty_like(mean)
     with _OnDevice(dev.index) as stream:
         tok = TRACE.begin(what)
@@ -531,8 +559,8 @@ def layernorm_modulate_backward(dy: torch.Tensor, x: torch.Tensor, mean: torch.T
     dshift, dscale = (torch.empty_like(scale), torch.empty_like(scale)) if need_params and scale is not None else (None, None)
     with _OnDevice(dev.index) as stream:
         lib, dt = load(), _dt(x.dtype)
-        n = lib.dax_norm_backward_workspace_bytes(B, S, D) if dweight is not None or dscale is not None else 0
-        ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
+        n = _norm_workspace_bytes(dev.index, B, S, D) if dweight is not None or dscale is not None else 0
+        ws = _workspace(n, dev)
         tok = TRACE.begin(what)
         check(lib.dax_layernorm_modulate_backward(grads.data_ptr(), rows.data_ptr(), dt, B, S, D, gb, gs, sb, ss,
                                                   mean.data_ptr(), rstd.data_ptr(), _ptr(ln_weight), _ptr(ln_bias), _ptr(scale),
@@ -564,7 +592,7 @@ def rmsnorm_rope(x: torch.Tensor, norm_weight: Optional[torch.Tensor] = None, *,
     _rope_check(what, S, D, rope_cos, rope_sin)
     dev = _on_one_device(what, x, norm_weight, rope_cos, rope_sin)
     y = _dense_like(x)
-    rstd = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev)
+    rstd = _row_statistics(x, B, S)
     with _OnDevice(dev.index) as stream:
         tok = TRACE.begin(what)
         check(load().dax_rmsnorm_rope(rows.data_ptr(), _dt(x.dtype), B, S, D, sb, ss, _ptr(norm_weight), _ptr(rope_cos),
@@ -590,8 +618,8 @@ def rmsnorm_rope_backward(dy: torch.Tensor, x: torch.Tensor, rstd: torch.Tensor,
     dweight = torch.empty_like(norm_weight) if need_params and norm_weight is not None else None
     with _OnDevice(dev.index) as stream:
         lib, dt = load(), _dt(x.dtype)
-        n = lib.dax_norm_backward_workspace_bytes(B, S, D) if dweight is not None else 0
-        ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
+        n = _norm_workspace_bytes(dev.index, B, S, D) if dweight is not None else 0
+        ws = _workspace(n, dev)
         tok = TRACE.begin(what)
         check(lib.dax_rmsnorm_rope_backward(grads.data_ptr(), rows.data_ptr(), dt, B, S, D, gb, gs, sb, ss,
                                             rstd.data_ptr(), _ptr(norm_weight), _ptr(rope_cos), _ptr(rope_sin), dx.data_ptr(), S * D, D,
@@ -605,13 +633,13 @@ def _heads_view(t: torch.Tensor) -> Tuple[torch.Tensor, I64x3]:
     broadcast dimensions, misaligned) is copied into token-major memory."""
     s0, s1, s2, s3 = t.stride()
     if s3 == 1 and s0 > 0 and s1 > 0 and s2 > 0 and (s0 | s1 | s2) % 8 == 0 and t.data_ptr() % 16 == 0:
-        return t, I64x3(s0, s1, s2)
+        return t, _strides3(s0, s1, s2)
     # a dimension of one may have any stride: the kernels get a valid one
     st = [st if n > 1 else 128 for n, st in zip(t.shape, (s0, s1, s2))]
     if s3 != 1 or t.data_ptr() % 16 or any(v <= 0 or v % 8 for v in st):
         t = _token_major(t).copy_(t)
         st = t.stride()[:3]
-    return t, I64x3(*st)
+    return t, _strides3(*st)
 
 
 def _attention_inputs(what: str, q, k, v, q_lens, k_lens, sm_scale) -> Tuple[int, int, int, int, float]:
@@ -644,7 +672,7 @@ def _token_major(t: torch.Tensor) -> torch.Tensor:
 
 
 def _token_major_strides(heads: int, S: int) -> I64x3:
-    return I64x3(S * heads * 128, 128, heads * 128)
+    return _strides3(S * heads * 128, 128, heads * 128)
 
 
 def attention_lse(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, q_lens: Optional[torch.Tensor] = None,
@@ -657,7 +685,7 @@ def attention_lse(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, q_lens: 
     B, heads, Sq, Sk, sm_scale = _attention_inputs(what, q, k, v, q_lens, k_lens, sm_scale)
     dev = _on_one_device(what, q, k, v, q_lens, k_lens)
     out = _token_major(q)
-    lse = torch.empty((B, heads, Sq), dtype=torch.float32, device=dev)
+    lse = torch.empty_strided((B, heads, Sq), (heads * Sq, Sq, 1), dtype=torch.float32, device=dev)
     if lse.numel() == 0:
         return out, lse
     if Sk == 0:
@@ -665,8 +693,8 @@ def attention_lse(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, q_lens: 
     (q, qs), (k, ks), (v, vs) = _heads_view(q), _heads_view(k), _heads_view(v)
     with _OnDevice(dev.index) as stream:
         lib = load()
-        n = lib.dax_attn_lse_workspace_bytes(B, heads, Sq, Sk)
-        ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
+        n = _attention_workspace_bytes(dev.index, False, B, heads, Sq, Sk)
+        ws = _workspace(n, dev)
         tok = TRACE.begin(what)
         check(lib.dax_attn_forward_lse(q.data_ptr(), k.data_ptr(), v.data_ptr(), _dt(q.dtype), B, heads, Sq, Sk, qs, ks, vs, sm_scale,
                                        _ptr(q_lens), _ptr(k_lens), out.data_ptr(), _token_major_strides(heads, Sq), lse.data_ptr(),
@@ -688,15 +716,16 @@ def attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: 
             raise ValueError(f"{what}: {name} must be {list(q.shape)} of {q.dtype}, got {list(t.shape)} of {t.dtype}")
     _vector(what, "lse", lse, (B, heads, Sq))
     dev = _on_one_device(what, dout, q, k, v, out, lse, q_lens, k_lens)
-    dq, dk, dv = _token_major(q), _token_major(k), _token_major(v)
+    dq, dk = _token_major(q), _token_major(k)
+    dv = torch.empty_like(dk)
     if lse.numel() == 0 or Sk == 0:
         return dq.zero_(), dk.zero_(), dv.zero_()
     (dout, dos), (q, qs), (k, ks), (v, vs), (out, os_) = map(_heads_view, (dout, q, k, v, out))
     kv = _token_major_strides(heads, Sk)
     with _OnDevice(dev.index) as stream:
         lib = load()
-        n = lib.dax_attn_backward_workspace_bytes(B, heads, Sq, Sk)
-        ws = torch.empty(n, dtype=torch.uint8, device=dev)
+        n = _attention_workspace_bytes(dev.index, True, B, heads, Sq, Sk)
+        ws = _workspace(n, dev)
         tok = TRACE.begin(what)
         check(lib.dax_attn_backward(dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), _dt(q.dtype),
                                     B, heads, Sq, Sk, dos, qs, ks, vs, os_, sm_scale, _ptr(q_lens), _ptr(k_lens), dq.data_ptr(),
