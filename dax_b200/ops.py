@@ -411,6 +411,9 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mode: str = "bf
 # ---- training: operators with a gradient ---------------------------------------------------------------------------------
 # The backward passes recompute what they need from the inputs and the row statistics that the forward passes return.
 # Workspaces come from torch for every call (nothing is shared between calls, streams or captured graphs).
+_get_device = getattr(torch._C, "_cuda_getDevice", None)  # torch.cuda.current_device() without its checks: the tensors are there
+
+
 class _OnDevice:
     """Makes a device the current one for a call, if it is not (``torch.cuda.device`` costs as much as a launch)."""
 
@@ -421,7 +424,7 @@ class _OnDevice:
 
     def __enter__(self) -> int:
         """The raw handle of the device's current stream."""
-        self.previous = torch.cuda.current_device()
+        self.previous = _get_device()
         if self.previous != self.index:
             torch.cuda.set_device(self.index)
         return torch._C._cuda_getCurrentRawStream(self.index)
@@ -431,18 +434,19 @@ class _OnDevice:
             torch.cuda.set_device(self.previous)
 
 
-def _on_one_device(what: str, *ts) -> torch.device:
-    """The device all tensors live on (the call goes to that device's current stream)."""
+def _on_one_device(what: str, *ts) -> int:
+    """The index of the device all tensors live on (the call goes to that device's current stream)."""
     dev = None
     for t in ts:
         if t is None:
             continue
-        if not t.is_cuda:
-            _need_cuda(t)
-        if dev is None:
-            dev = t.device
-        elif t.device != dev:
-            raise ValueError(f"{what}: tensors are on different devices, {dev} and {t.device}")
+        i = t.get_device()
+        if i != dev:
+            if i < 0:
+                _need_cuda(t)
+            if dev is not None:
+                raise ValueError(f"{what}: tensors are on different devices, cuda:{dev} and {t.device}")
+            dev = i
     return dev
 
 
@@ -527,7 +531,7 @@ def layernorm_modulate(x: torch.Tensor, *, eps: float = 1e-6, ln_weight: Optiona
     y = _dense_like(x)
     mean = _row_statistics(x, B, S)
     rstd = torch.empty_like(mean)
-    with _OnDevice(dev.index) as stream:
+    with _OnDevice(dev) as stream:
         tok = TRACE.begin(what)
         check(load().dax_layernorm_modulate(rows.data_ptr(), _dt(x.dtype), B, S, D, sb, ss, _ptr(ln_weight),
                                             _ptr(ln_bias), _ptr(shift), _ptr(scale), float(eps), y.data_ptr(), S * D, D,
@@ -557,10 +561,10 @@ def layernorm_modulate_backward(dy: torch.Tensor, x: torch.Tensor, mean: torch.T
     dweight = torch.empty_like(ln_weight) if need_params and ln_weight is not None else None
     dbias = torch.empty_like(ln_bias) if need_params and ln_bias is not None else None
     dshift, dscale = (torch.empty_like(scale), torch.empty_like(scale)) if need_params and scale is not None else (None, None)
-    with _OnDevice(dev.index) as stream:
+    with _OnDevice(dev) as stream:
         lib, dt = load(), _dt(x.dtype)
-        n = _norm_workspace_bytes(dev.index, B, S, D) if dweight is not None or dscale is not None else 0
-        ws = _workspace(n, dev)
+        n = _norm_workspace_bytes(dev, B, S, D) if dweight is not None or dscale is not None else 0
+        ws = _workspace(n, x.device)
         tok = TRACE.begin(what)
         check(lib.dax_layernorm_modulate_backward(grads.data_ptr(), rows.data_ptr(), dt, B, S, D, gb, gs, sb, ss,
                                                   mean.data_ptr(), rstd.data_ptr(), _ptr(ln_weight), _ptr(ln_bias), _ptr(scale),
@@ -593,7 +597,7 @@ def rmsnorm_rope(x: torch.Tensor, norm_weight: Optional[torch.Tensor] = None, *,
     dev = _on_one_device(what, x, norm_weight, rope_cos, rope_sin)
     y = _dense_like(x)
     rstd = _row_statistics(x, B, S)
-    with _OnDevice(dev.index) as stream:
+    with _OnDevice(dev) as stream:
         tok = TRACE.begin(what)
         check(load().dax_rmsnorm_rope(rows.data_ptr(), _dt(x.dtype), B, S, D, sb, ss, _ptr(norm_weight), _ptr(rope_cos),
                                       _ptr(rope_sin), float(eps), y.data_ptr(), S * D, D, rstd.data_ptr(), stream))
@@ -616,10 +620,10 @@ def rmsnorm_rope_backward(dy: torch.Tensor, x: torch.Tensor, rstd: torch.Tensor,
     dev = _on_one_device(what, dy, x, rstd, norm_weight, rope_cos, rope_sin)
     dx = _dense_like(x)
     dweight = torch.empty_like(norm_weight) if need_params and norm_weight is not None else None
-    with _OnDevice(dev.index) as stream:
+    with _OnDevice(dev) as stream:
         lib, dt = load(), _dt(x.dtype)
-        n = _norm_workspace_bytes(dev.index, B, S, D) if dweight is not None else 0
-        ws = _workspace(n, dev)
+        n = _norm_workspace_bytes(dev, B, S, D) if dweight is not None else 0
+        ws = _workspace(n, x.device)
         tok = TRACE.begin(what)
         check(lib.dax_rmsnorm_rope_backward(grads.data_ptr(), rows.data_ptr(), dt, B, S, D, gb, gs, sb, ss,
                                             rstd.data_ptr(), _ptr(norm_weight), _ptr(rope_cos), _ptr(rope_sin), dx.data_ptr(), S * D, D,
@@ -685,16 +689,16 @@ def attention_lse(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, q_lens: 
     B, heads, Sq, Sk, sm_scale = _attention_inputs(what, q, k, v, q_lens, k_lens, sm_scale)
     dev = _on_one_device(what, q, k, v, q_lens, k_lens)
     out = _token_major(q)
-    lse = torch.empty_strided((B, heads, Sq), (heads * Sq, Sq, 1), dtype=torch.float32, device=dev)
+    lse = torch.empty_strided((B, heads, Sq), (heads * Sq, Sq, 1), dtype=torch.float32, device=q.device)
     if lse.numel() == 0:
         return out, lse
     if Sk == 0:
         return out.zero_(), lse.fill_(-math.inf)
     (q, qs), (k, ks), (v, vs) = _heads_view(q), _heads_view(k), _heads_view(v)
-    with _OnDevice(dev.index) as stream:
+    with _OnDevice(dev) as stream:
         lib = load()
-        n = _attention_workspace_bytes(dev.index, False, B, heads, Sq, Sk)
-        ws = _workspace(n, dev)
+        n = _attention_workspace_bytes(dev, False, B, heads, Sq, Sk)
+        ws = _workspace(n, q.device)
         tok = TRACE.begin(what)
         check(lib.dax_attn_forward_lse(q.data_ptr(), k.data_ptr(), v.data_ptr(), _dt(q.dtype), B, heads, Sq, Sk, qs, ks, vs, sm_scale,
                                        _ptr(q_lens), _ptr(k_lens), out.data_ptr(), _token_major_strides(heads, Sq), lse.data_ptr(),
@@ -722,10 +726,10 @@ def attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: 
         return dq.zero_(), dk.zero_(), dv.zero_()
     (dout, dos), (q, qs), (k, ks), (v, vs), (out, os_) = map(_heads_view, (dout, q, k, v, out))
     kv = _token_major_strides(heads, Sk)
-    with _OnDevice(dev.index) as stream:
+    with _OnDevice(dev) as stream:
         lib = load()
-        n = _attention_workspace_bytes(dev.index, True, B, heads, Sq, Sk)
-        ws = _workspace(n, dev)
+        n = _attention_workspace_bytes(dev, True, B, heads, Sq, Sk)
+        ws = _workspace(n, q.device)
         tok = TRACE.begin(what)
         check(lib.dax_attn_backward(dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), _dt(q.dtype),
                                     B, heads, Sq, Sk, dos, qs, ks, vs, os_, sm_scale, _ptr(q_lens), _ptr(k_lens), dq.data_ptr(),
