@@ -23,8 +23,12 @@
 // Scores, probabilities, row statistics, D and all sums are fp32.  p and ds are rounded once to the operands' type, as A
 // operands of the second products (the tensor cores take nothing wider together with 16-bit B operands).  fp16 has its
 // smallest normal number at 2^-14, and the p of a long row of keys lie below it: the backward pass rounds 2^12 p, which is
-// normal down to p = 2^-26, and takes the factor out of dv again.  ds keeps its size (nothing bounds it from above): in fp16
-// it has the range of the gradients themselves, as in any fp16 training.
+// normal down to p = 2^-26, and takes the factor out of dv again.  ds is smaller than do by a factor of p as well, and larger by
+// that of v; |ds_ij| <= 2 |do_i| max_j |v_j| bounds it.  In fp16 it is rounded times the power of two that brings this bound to
+// 2^15: one for each query in dq (it leaves with the row), one for each head in dk, whose sums run over the queries.  Error of dq
+// of 32,760 keys (in brackets one rounding of the exact result), ds rounded as it is / with the factors: do of 1e-2 3.0e-3 /
+// 3.0e-4 (2.1e-4), 1e-3 3.0e-2 / 5.2e-4 (4.7e-4: results below 2^-14); infinite / finite where ds passes 65,504.  A small kernel
+// finds the largest norms first (fp16 only).
 #include <algorithm>
 #include <atomic>
 #include <cmath>
@@ -48,6 +52,7 @@ template <bool BF16> constexpr float P_SHIFT = BF16 ? 0.f : 12.f;             //
 template <bool BF16> constexpr float P_UNSHIFT = BF16 ? 1.f : 1.f / 4096.f;
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr int kMaxSplits = 16;
+constexpr int kRangeChunks = 32;  // of a head's tokens, for the largest norms: one per lane
 
 struct Rows { const void* p; int64_t sb, sh, st; };  // a [B, heads, S, 128] view: element strides of sample, head, token
 
@@ -57,6 +62,7 @@ struct TrainParams {
   const int* q_lens;   // [B] or null
   const int* k_lens;
   float* row_stats;    // backward: [2][BH * Sq_pad]: P_SHIFT - lse * log2(e) (-inf: no such row), then -D * P_UNSHIFT
+  float* range;        // backward, fp16: [2][BH][kRangeChunks]: largest |v_j|^2, then largest |do_i|^2, of each chunk of the head's tokens
   float* part;         // split runs: fp32 partial sums
   float* part_lse;     // split forward runs: [splits, BH, Sq] log2 of each part's sum of exponentials
   int* status;
@@ -232,6 +238,59 @@ __device__ __forceinline__ void close_tmem(uint32_t base, bool owner, volatile u
     tmem_dealloc(base, 512);
   }
   if (threadIdx.x == 0 && *abort_flag) atomicExch(status, DAX_ERR_TIMEOUT);
+}
+
+// ---- factors of ds in fp16 ---------------------------------------------------------------------------------------------
+__host__ __device__ __forceinline__ int range_rows(int S) { return ((S + kRangeChunks - 1) / kRangeChunks + 15) / 16 * 16; }  // of a chunk
+// The power of two that brings 2 |do| |v| to [2^14, 2^15), from the product of the squares; finite for 0 and infinity too.
+__device__ __forceinline__ float range_factor(float squares) {
+  const int e = static_cast<int>(__float_as_uint(4.f * squares) >> 23) - 127;  // 4 squares < 2^(e + 1)
+  return __uint_as_float(static_cast<uint32_t>(127 + 15 - ((e + 2) >> 1)) << 23);
+}
+__device__ __forceinline__ float power_inverse(float f) { return __uint_as_float((254u << 23) - __float_as_uint(f)); }
+// The largest of a head's squares over its chunks, by the whole warp (none is negative, so their bits order like numbers).
+__device__ __forceinline__ float range_max(const float* range, int S) {
+  const int lane = threadIdx.x & 31;
+  const float v = lane * range_rows(S) < S ? range[lane] : 0.f;
+  return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(v)));
+}
+
+// Largest |v_j|^2 (blockIdx.z 0) and |do_i|^2 (1) of each chunk of tokens that exist: half a warp per token.  A NaN is passed
+// over: what it touches is NaN anyway.  The backward pass of 12 heads x
+// 4,095 x 4,095 takes 316 us with it and the factors, 307 without.
+__global__ void __launch_bounds__(256) attn_range_kernel(const Rows v, const Rows dout, const TrainParams p) {
+  const bool keys = blockIdx.z == 0;
+  const Rows& t = keys ? v : dout;
+  const int bh = blockIdx.y, b = bh / p.heads, h = bh % p.heads, S = keys ? p.Sk : p.Sq;
+  const int per = range_rows(S), row0 = static_cast<int>(blockIdx.x) * per;
+  if (row0 >= S) return;
+  const int end = min(valid_len(keys ? p.k_lens : p.q_lens, b, S), row0 + per);
+  const int piece = threadIdx.x & 15;
+  float top = 0.f;
+#pragma unroll 4
+  for (int s = row0 + (threadIdx.x >> 4); s < row0 + per; s += 16) {  // the same number of steps for all threads
+    uint4 u = make_uint4(0u, 0u, 0u, 0u);
+    if (s < end) u = *reinterpret_cast<const uint4*>(row_ptr(t, b, h, s) + piece * 8);
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+    float n = 0.f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      float a, c;
+      unpack2<false>(w[k], a, c);
+      n = fmaf(a, a, fmaf(c, c, n));
+    }
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+    top = fmaxf(top, n);
+  }
+  __shared__ float tops[8];
+  top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+  if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int k = 1; k < 8; ++k) top = fmaxf(top, tops[k]);
+    p.range[(static_cast<int64_t>(blockIdx.z) * p.B * p.heads + bh) * kRangeChunks + blockIdx.x] = top;
+  }
 }
 
 // ---- dq ----------------------------------------------------------------------------------------------------------------
@@ -432,10 +491,15 @@ attn_bwd_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
     const bool live = q_row < q_len;
     float* s_mean = reinterpret_cast<float*>(smem + DQ_OFF_MEAN);
     const float l = live ? p.lse[static_cast<int64_t>(bh) * p.Sq + q_row] : -INFINITY;
+    float v_top = 0.f, do_top = 0.f;
+    if constexpr (!BF16) {
+      v_top = range_max(p.range + static_cast<int64_t>(bh) * kRangeChunks, p.Sk);
+      do_top = range_max(p.range + (static_cast<int64_t>(p.B) * p.heads + bh) * kRangeChunks, p.Sq);
+    }
     bool ok = mbar_wait(rows_full, 0, abort_flag);
     {  // a quarter of a row of do to tensor memory, and its part of D to where dq will be
       uint32_t w[16];
-      float d[2] = {0.f, 0.f};
+      float d[2] = {0.f, 0.f}, norm = 0.f;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int at = (cg >> 1) * BOX_BYTES + r * 128 + ((((cg & 1) * 4 + i) ^ (r & 7)) << 4);
@@ -449,11 +513,13 @@ attn_bwd_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
           unpack2<BF16>(ow[k], o0, o1);
           d[0] = fmaf(a0, o0, d[0]);
           d[1] = fmaf(a1, o1, d[1]);
+          if constexpr (!BF16) norm = fmaf(a0, a0, fmaf(a1, a1, norm));
           w[4 * i + k] = uw[k];
         }
       }
       tmem_st16(tm + lanes + T_DO + cg * 16, w);
       tmem_st1(tm + lanes + T_DQ + cg * 32, __float_as_uint(d[0] + d[1]));
+      if constexpr (!BF16) tmem_st1(tm + lanes + T_DQ + cg * 32 + 1, __float_as_uint(norm));
       tmem_wait_st();
       tc_fence_before_sync();
       __syncwarp();
@@ -461,13 +527,26 @@ attn_bwd_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
     }
     ok = ok && mbar_wait(do_full, 0, abort_flag);  // all warps have arrived
     tc_fence_after_sync();
-    const float nl = l == -INFINITY ? -INFINITY : -l * LOG2E, nd = -sum_of_groups(tm + lanes + T_DQ);
+    const float nl = l == -INFINITY ? -INFINITY : -l * LOG2E;
+    float nd = -sum_of_groups(tm + lanes + T_DQ);
+    // fp16: ds is computed and rounded times `factor`, so -D is kept times it; `to_stat` makes of that what the dk/dv kernel wants
+    float factor = 1.f, to_stat = 1.f;
+    if constexpr (!BF16) {
+      factor = range_factor(sum_of_groups(tm + lanes + T_DQ + 1) * v_top);
+      nd *= factor;
+      to_stat = range_factor(do_top * v_top) * P_UNSHIFT<BF16> * power_inverse(factor);
+    }
     if (cg == 0 && split == 0) {
       stat[r] = nl + P_SHIFT<BF16>;
-      stat[stats + r] = nd * P_UNSHIFT<BF16>;
+      stat[stats + r] = nd * to_stat;
     }
     const uint64_t nl2 = f2_splat(nl), cmul2 = f2_splat(p.sm_scale * LOG2E);
     uint64_t nd2 = f2_splat(nd);
+    const uint64_t factor2 = f2_splat(factor);
+    const auto minus_d = [factor2](uint32_t y0, uint32_t y1, uint64_t nd) {  // dp - D, times the factor
+      if constexpr (BF16) return f2_add(f2_bits(y0, y1), nd);
+      else return f2_fma(f2_bits(y0, y1), factor2, nd);
+    };
     float e[2] = {0.f, 0.f};  // sums of the rounded ds
     const int team = warp >> 3;
     const auto tile = [&](int j, auto only) -> bool {  // the arithmetic of a tile of keys; false: a wait gave up
@@ -510,7 +589,7 @@ attn_bwd_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
         uint64_t off2 = f2_splat(0.f);
 #pragma unroll
         for (int i = 0; i < 16; ++i)
-          off2 = f2_fma(f2_bits(sv[2 * i], sv[2 * i + 1]), f2_add(f2_bits(dp[2 * i], dp[2 * i + 1]), nd2), off2);
+          off2 = f2_fma(f2_bits(sv[2 * i], sv[2 * i + 1]), minus_d(dp[2 * i], dp[2 * i + 1], nd2), off2);
         float a, c;
         f2_unpack(off2, a, c);
         tmem_st1(tm + lanes + T_DP + cg * 32, __float_as_uint(a + c));  // where this warp has read its dp
@@ -524,12 +603,12 @@ attn_bwd_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
         f2_unpack(nd2, a, c);
         a = live ? a - off : 0.f;  // a row behind the length holds anything
         nd2 = f2_splat(a);
-        if (cg == 0) stat[stats + r] = a * P_UNSHIFT<BF16>;  // split 0 has the tile
+        if (cg == 0) stat[stats + r] = a * to_stat;  // split 0 has the tile
       }
       uint32_t pk[16];
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        pk[i] = f2_to16_rn<BF16>(f2_mul(f2_bits(sv[2 * i], sv[2 * i + 1]), f2_add(f2_bits(dp[2 * i], dp[2 * i + 1]), nd2)));
+        pk[i] = f2_to16_rn<BF16>(f2_mul(f2_bits(sv[2 * i], sv[2 * i + 1]), minus_d(dp[2 * i], dp[2 * i + 1], nd2)));
         add_pair<BF16>(e[i & 1], pk[i]);
       }
       if (j > 0) {  // ds of the last tile has been read (normally long ago)
@@ -590,7 +669,7 @@ attn_bwd_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
     if (ok && mbar_wait(dq_done, (n - 1) & 1u, abort_flag)) {
       tc_fence_after_sync();
       // the softmax over one key is constant: its gradient is zero, not the rounding of dp - D
-      const float mul = k_len == 1 ? 0.f : p.sm_scale;
+      const float unscale = BF16 ? 1.f : power_inverse(factor), mul = k_len == 1 ? 0.f : p.sm_scale * unscale;
       const float neg_e = -sum_of_groups(tm + lanes + T_S);
       const int rows = max(0, min(32, rows_in - (warp & 3) * 32));
       uint8_t* st = smem + warp * 4096;  // every product and every copy is complete: the ring stages the results
@@ -605,7 +684,7 @@ attn_bwd_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
         v[i + 2] = __float_as_uint(fmaf(neg_e, m.z, __uint_as_float(v[i + 2])));
         v[i + 3] = __float_as_uint(fmaf(neg_e, m.w, __uint_as_float(v[i + 3])));
       }
-      if (p.splits > 1) store_part32(st, v, 1.f, live, part + (warp & 3) * 32 * 128 + cg * 32, rows);
+      if (p.splits > 1) store_part32(st, v, unscale, live, part + (warp & 3) * 32 * 128 + cg * 32, rows);
       else store_cols32<BF16>(st, v, mul, live, out_ptr(p.dq, b, h, q0 + (warp & 3) * 32) + cg * 32, p.dq.st, rows);
     }
   }
@@ -800,10 +879,19 @@ attn_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
     const int cg = warp >> 2, k_row = k0 + (warp & 3) * 32 + lane;
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint64_t cmul2 = f2_splat(p.sm_scale * LOG2E);
-    // 2^P_SHIFT p (dp - D) 2^-P_SHIFT: the factor of p costs ds nothing
-    const auto minus_d = [](uint32_t y0, uint32_t y1, uint64_t nd) {
+    // fp16: 2^P_SHIFT p is at hand and the head's factor times ds is wanted (-D comes with both in it)
+    float unscale = 1.f, factor = 1.f;
+    if constexpr (!BF16) {
+      const float v_top = range_max(p.range + static_cast<int64_t>(bh) * kRangeChunks, p.Sk);
+      const float do_top = range_max(p.range + (static_cast<int64_t>(p.B) * p.heads + bh) * kRangeChunks, p.Sq);
+      factor = range_factor(do_top * v_top);
+      unscale = power_inverse(factor);
+      factor *= P_UNSHIFT<BF16>;
+    }
+    const uint64_t factor2 = f2_splat(factor);
+    const auto minus_d = [factor2](uint32_t y0, uint32_t y1, uint64_t nd) {
       if constexpr (BF16) return f2_add(f2_bits(y0, y1), nd);
-      else return f2_fma(f2_bits(y0, y1), f2_splat(P_UNSHIFT<BF16>), nd);
+      else return f2_fma(f2_bits(y0, y1), factor2, nd);
     };
     bool ok = true;
     for (int i = 0; ok && i < n; ++i) {
@@ -882,7 +970,7 @@ attn_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
     if (ok && mbar_wait(dv_done, (n - 1) & 1u, abort_flag) && mbar_wait(dk_done, (n - 1) & 1u, abort_flag)) {
       tc_fence_after_sync();
       const bool live = k_row < k_len;
-      const float mul = k_len == 1 ? 0.f : p.sm_scale;  // one key: see the dq kernel
+      const float mul = k_len == 1 ? 0.f : p.sm_scale * unscale;  // one key: see the dq kernel
       const int row0 = (warp & 3) * 32, rows = max(0, min(32, rows_in - row0));
       uint8_t* st = smem + warp * 4096;  // every product and every copy is complete: the ring stages the results
 #pragma unroll 1
@@ -890,7 +978,7 @@ attn_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
         uint32_t v[32];
         tmem_ld32(tm + lanes + (c == 0 ? T_DK : T_DV) + cg * 32, v);
         tmem_wait_ld();
-        if (p.splits > 1) store_part32(st, v, 1.f, live, part + (c == 0 ? 0 : part_all) + row0 * 128 + cg * 32, rows);
+        if (p.splits > 1) store_part32(st, v, c == 0 ? unscale : P_UNSHIFT<BF16>, live, part + (c == 0 ? 0 : part_all) + row0 * 128 + cg * 32, rows);
         else store_cols32<BF16>(st, v, c == 0 ? mul : P_UNSHIFT<BF16>, live, out_ptr(c == 0 ? p.dk : p.dv, b, h, k0 + row0) + cg * 32, (c == 0 ? p.dk : p.dv).st, rows);
       }
     }
@@ -1216,12 +1304,13 @@ inline int dkdv_splits(int64_t BH, int64_t Sq, int64_t Sk) { return choose_split
 inline int64_t pad128(int64_t S) { return tiles_of(S, 128) * 128; }
 inline size_t round256(size_t n) { return (n + 255) / 256 * 256; }
 
-struct BackwardLayout { size_t stats, dq, dkdv, bytes; };
+struct BackwardLayout { size_t stats, range, dq, dkdv, bytes; };
 inline BackwardLayout backward_layout(int64_t BH, int64_t Sq, int64_t Sk) {
   BackwardLayout w{};
   const int s_q = dq_splits(BH, Sq, Sk), s_kv = dkdv_splits(BH, Sq, Sk);
   w.stats = 0;
-  w.dq = round256(static_cast<size_t>(BH) * pad128(Sq) * 8);
+  w.range = round256(static_cast<size_t>(BH) * pad128(Sq) * 8);
+  w.dq = w.range + round256(static_cast<size_t>(BH) * kRangeChunks * 8);
   w.dkdv = w.dq + (s_q > 1 ? round256(static_cast<size_t>(s_q) * BH * Sq * 512) : 0);
   w.bytes = w.dkdv + (s_kv > 1 ? round256(static_cast<size_t>(s_kv) * BH * Sk * 1024) : 0);
   return w;
@@ -1289,9 +1378,14 @@ int run_forward(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap&
 }
 
 template <bool BF16>
-int run_backward(const CUtensorMap& mq, const CUtensorMap& mdo, const CUtensorMap& mo, const CUtensorMap& mk, const CUtensorMap& mv, TrainParams p,
-                 int s_q, int s_kv, float* part_q, float* part_kv, cudaStream_t st) {
+int run_backward(const CUtensorMap& mq, const CUtensorMap& mdo, const CUtensorMap& mo, const CUtensorMap& mk, const CUtensorMap& mv, const Rows& v,
+                 const Rows& dout, TrainParams p, int s_q, int s_kv, float* part_q, float* part_kv, cudaStream_t st) {
   const unsigned BH = static_cast<unsigned>(p.B * p.heads);
+  if constexpr (!BF16) {
+    const int chunks = std::max((p.Sq + range_rows(p.Sq) - 1) / range_rows(p.Sq), (p.Sk + range_rows(p.Sk) - 1) / range_rows(p.Sk));
+    attn_range_kernel<<<dim3(static_cast<unsigned>(chunks), BH, 2), 256, 0, st>>>(v, dout, p);
+    DAX_CUDA(cudaGetLastError());
+  }
   p.splits = s_q;
   p.part = part_q;
   DAX_TRY((allow_smem<decltype(&attn_bwd_dq_kernel<BF16>), &attn_bwd_dq_kernel<BF16>>(DQ_SMEM)));
@@ -1311,7 +1405,7 @@ int run_backward(const CUtensorMap& mq, const CUtensorMap& mdo, const CUtensorMa
   if (s_kv > 1) {
     const int64_t rows = static_cast<int64_t>(BH) * p.Sk;
     const JoinTarget tk = {p.dk, part_kv, p.k_lens, p.sm_scale, true},
-                     tv = {p.dv, part_kv + s_kv * rows * 128, p.k_lens, P_UNSHIFT<BF16>, false};
+                     tv = {p.dv, part_kv + s_kv * rows * 128, p.k_lens, 1.f, false};
     attn_bwd_join_kernel<BF16><<<dim3(static_cast<unsigned>(tiles_of(rows, 8)), 2), 256, 0, st>>>(tk, tv, s_kv, rows, p.Sk, p.heads, p.Sk);
     DAX_CUDA(cudaGetLastError());
   }
@@ -1410,6 +1504,7 @@ int dax_attn_backward(const void* dout, const void* q, const void* k, const void
   p.q_lens = q_lens;
   p.k_lens = k_lens;
   p.row_stats = reinterpret_cast<float*>(ws + w.stats);
+  p.range = reinterpret_cast<float*>(ws + w.range);
   p.status = device_status_ptr();
   DAX_REQUIRE(p.status != nullptr, DAX_ERR_CUDA, "%s: cannot resolve the device status word", what);
   p.B = static_cast<int>(B);
@@ -1421,9 +1516,10 @@ int dax_attn_backward(const void* dout, const void* q, const void* k, const void
   const int s_q = dq_splits(B * heads, Sq, Sk), s_kv = dkdv_splits(B * heads, Sq, Sk);
   float* part_q = reinterpret_cast<float*>(ws + w.dq);
   float* part_kv = reinterpret_cast<float*>(ws + w.dkdv);
+  const Rows rv = rows_of(v, v_strides), rdo = rows_of(dout, do_strides);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return dtype == DAX_BF16 ? run_backward<true>(mq, mdo, mo, mk, mv, p, s_q, s_kv, part_q, part_kv, st)
-                           : run_backward<false>(mq, mdo, mo, mk, mv, p, s_q, s_kv, part_q, part_kv, st);
+  return dtype == DAX_BF16 ? run_backward<true>(mq, mdo, mo, mk, mv, rv, rdo, p, s_q, s_kv, part_q, part_kv, st)
+                           : run_backward<false>(mq, mdo, mo, mk, mv, rv, rdo, p, s_q, s_kv, part_q, part_kv, st);
 }
 
 }  // extern "C"
