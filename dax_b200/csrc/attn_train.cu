@@ -22,8 +22,9 @@
 //
 // Scores, probabilities, row statistics, D and all sums are fp32.  p and ds are rounded once to the operands' type, as A
 // operands of the second products (the tensor cores take nothing wider together with 16-bit B operands).  fp16 has its
-// smallest normal number at 2^-14, and the p of a long row of keys lie below it: the backward pass rounds 2^12 p, which is
-// normal down to p = 2^-26, and takes the factor out of dv again.  ds is smaller than do by a factor of p as well, and larger by
+// smallest normal number at 2^-14, and the p of a long row of keys, or of keys beside a dominant one, lie below it: the
+// backward pass rounds 2^12 p, which is normal down to p = 2^-26, and takes the factor out of dv again; the forward pass rounds
+// 2^11 p / max p (F_SHIFT), and its factor leaves with the row's sum.  ds is smaller than do by a factor of p as well, and larger by
 // that of v; |ds_ij| <= 2 |do_i| max_j |v_j| bounds it.  In fp16 it is rounded times the power of two that brings this bound to
 // 2^15: one for each query in dq (it leaves with the row), one for each head in dk, whose sums run over the queries.  Error of dq
 // of 32,760 keys (in brackets one rounding of the exact result), ds rounded as it is / with the factors: do of 1e-2 3.0e-3 /
@@ -47,7 +48,10 @@ constexpr int ROW_WARPS_F = 8, ROW_WARPS_B = 16;
 template <int N> struct Warps {
   static constexpr int threads = (N + 4) * 32, producer = N, issuer0 = N + 1, issuer1 = N + 2, tmem = N + 3;
 };
-constexpr float TAU = 8.f;                 // forward: lazy rescale, p <= 2^8
+// Forward: the sums are rescaled when the row's maximum has risen by more than 2^TAU, so p (relative to the maximum then) is at
+// most 2^TAU; it is rounded as 2^F_SHIFT p, and so is its sum taken.  fp16: at most 2^15, and normal down to 2^-25 of the largest.
+template <bool BF16> constexpr float TAU = BF16 ? 8.f : 4.f;
+template <bool BF16> constexpr float F_SHIFT = BF16 ? 0.f : 11.f;
 template <bool BF16> constexpr float P_SHIFT = BF16 ? 0.f : 12.f;             // backward: p is rounded as 2^P_SHIFT p
 template <bool BF16> constexpr float P_UNSHIFT = BF16 ? 1.f : 1.f / 4096.f;
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
@@ -1143,9 +1147,9 @@ attn_fwd_lse_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
       for (int i = 0; i < 128; i += 2)
         fmx[(i >> 1) & 3] = fmax3(fmx[(i >> 1) & 3], __uint_as_float(sv[i]), __uint_as_float(sv[i + 1]));
       const float mx = fmaxf(fmax3(fmx[0], fmx[1], fmx[2]), fmx[3]) * cmul;  // cmul > 0
-      const float m_new = (mx > m + TAU) ? mx : m;
+      const float m_new = (mx > m + TAU<BF16>) ? mx : m;
       const float alpha = ex2(m - m_new);  // m = -inf on the first tile -> 0
-      const float off = -m_new;
+      const float off = F_SHIFT<BF16> - m_new;
       if (j > 0) {
         if (!(ok = mbar_wait(&pv_done[x], (j - 1) & 1u, abort_flag))) break;
         tc_fence_after_sync();
@@ -1186,7 +1190,7 @@ attn_fwd_lse_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     if (ok && mbar_wait(&pv_done[x], (n - 1) & 1u, abort_flag)) {
       tc_fence_after_sync();
       const bool live = q_row < q_len;
-      const float inv_l = 1.f / l, l2 = m + log2f(l);
+      const float inv_l = 1.f / l, l2 = m + (log2f(l) - F_SHIFT<BF16>);
       if (q_row < p.Sq) (p.splits > 1 ? p.part_lse[split_row] : p.lse[row]) = live ? (p.splits > 1 ? l2 : l2 * LN2) : -INFINITY;
       // the tile's scores are complete, so its q has been read for the last time: its place stages the results
       uint8_t* st = smem + F_OFF_Q + x * TILE_BYTES + (warp & 3) * 8192;

@@ -143,3 +143,47 @@ def test_infinite_gradients_stay_in_their_rows_of_dq(ops):
     keep = torch.arange(200, device=DEV) != 17
     assert torch.equal(dq[0, 0, keep], want[0, 0, keep]) and not torch.isfinite(dq[0, 0, 17].float()).any()
     assert not torch.isfinite(dk.float()).all()
+
+
+@pytest.mark.parametrize("gap", [10, 17, 21, 25])
+@pytest.mark.parametrize("at", [0, 700, 1999])
+@pytest.mark.parametrize("rows", [3, 5000])
+def test_keys_far_below_the_largest_score(ops, gap, at, rows):
+    """One key whose score is `gap` powers of two above all others and whose value is zero: the output is what the others add.
+    Their p are 2^-gap of the largest, and rounded as normal numbers down to 2^-25 of it (u).  The offset
+    of some keys and the rounding of k put them up to 2^0.03 lower (u times 1.03).  One product per score, so scores are exact
+    but for the fp32 arithmetic of the exponent (2^-19); sums of S positive terms; the result's rounding."""
+    S, c = 2000, 1 / math.sqrt(128)
+    g = torch.Generator(device=DEV).manual_seed(5)
+    q, k = torch.zeros(1, 1, rows, 128, device=DEV), torch.zeros(1, 1, S, 128, device=DEV)
+    q[..., 0], k[0, 0, at, 0] = 8.0, gap * math.log(2) / (8 * c)
+    k[0, 0, :at, 0] = -0.01  # no two maxima in a row are the same
+    v = 32 + 32 * torch.rand(1, 1, S, 128, generator=g, device=DEV)
+    v[0, 0, at] = 0
+    q, k, v = q.half(), k.half(), v.half()
+    out, lse = ops.attention_lse(q, k, v)
+    s = c * 8 * k[0, 0, :, 0].double()
+    p = torch.softmax(s, 0)
+    want = p @ v[0, 0].double()
+    bound = (1.03 * U + 2.0 ** -19 + S * W) * want * (1 + U) + U * want + HALF_STEP
+    assert bool(((out[0, 0].double() - want).abs() <= bound).all()), float(((out[0, 0].double() - want).abs() / want).max())
+    assert bool(((lse.double() - torch.logsumexp(s, 0)).abs() <= 2.0 ** -18).all())
+
+
+@pytest.mark.parametrize("step", [1.9, 3.9, 4.1, 7.9, 8.1, 30.0])
+def test_maxima_that_rise_tile_by_tile(ops, step):
+    """Every tile of 128 keys is `step` powers of two above the last: p stays inside fp16 whether the running maximum follows
+    or not."""
+    S, rows, c = 1024, 300, 1 / math.sqrt(128)
+    g = torch.Generator(device=DEV).manual_seed(6)
+    q, k = torch.zeros(1, 1, rows, 128, device=DEV), torch.zeros(1, 1, S, 128, device=DEV)
+    q[..., 0], k[0, 0, :, 0] = 8.0, (torch.arange(S, device=DEV) // 128) * (step * math.log(2) / (8 * c))
+    v = 1 + torch.rand(1, 1, S, 128, generator=g, device=DEV)
+    q, k, v = q.half(), k.half(), v.half()
+    out, lse = ops.attention_lse(q, k, v)
+    s = c * 8 * k[0, 0, :, 0].double()
+    want = torch.softmax(s, 0) @ v[0, 0].double()
+    # scores reach 7 * step * ln 2: the exponent's argument is off by 2^-24 of that, the rest as above
+    err = U + 2.0 ** -19 + 2.0 ** -23 * 7 * step + S * W
+    assert bool(((out[0, 0].double() - want).abs() <= (err * (1 + U) + U) * want).all())
+    assert bool(((lse.double() - torch.logsumexp(s, 0)).abs() <= 2.0 ** -18 + 2.0 ** -22 * 7 * step).all())
