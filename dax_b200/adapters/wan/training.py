@@ -20,9 +20,16 @@ import torch
 from ... import autograd
 from ...parallel import dist as para_dist
 from ...quant.nn.dynamic import Linear as QLinear
-from .attn_adapter import HEAD_DIM, _rope_tables
+from .attn_adapter import HEAD_DIM
 from .block_adapter import _block_classes
 from .transformer_adapter import dit_forward
+
+
+def _rotary_tables(rotary_emb: torch.Tensor):
+    """Complex ``[1, 1, S, 64]`` table -> fp32 cos / sin ``[S, 64]``, made on the current stream for each call: autograd keeps them
+    for the backward pass (512 bytes per token and layer), a captured graph makes them again at every replay."""
+    r = torch.view_as_real(rotary_emb.reshape(-1, rotary_emb.shape[-1]))
+    return r[..., 0].to(torch.float32).contiguous(), r[..., 1].to(torch.float32).contiguous()
 
 
 class DAXWanTrainingAttnProcessor:
@@ -46,7 +53,7 @@ class DAXWanTrainingAttnProcessor:
             raise ValueError(f"hidden size {D} != heads {attn.heads} x {HEAD_DIM}")
         cos = sin = None
         if rotary_emb is not None:
-            cos, sin = _rope_tables(rotary_emb)
+            cos, sin = _rotary_tables(rotary_emb)
 
         def heads(t):
             return t.unflatten(2, (attn.heads, HEAD_DIM)).transpose(1, 2)

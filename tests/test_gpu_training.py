@@ -257,3 +257,40 @@ def test_whole_model_trains(ag):
         if exact[n].numel() >= 4096:
             e_plain, e_own = ((r[n].double() - exact[n]).norm() / exact[n].norm() for r in (plain, own))
             assert e_own <= 1.5 * e_plain + 2 * 2.0 ** -9, (n, float(e_plain), float(e_own))
+
+
+def test_captured_step_follows_its_rotary_table(ag):
+    """The table is an input like the others: a graph captured after a warm-up step reads what it holds at the replay, and
+    nothing that other tables' steps put in its place."""
+    from dax_b200.adapters.wan import attn_adapter
+    from dax_b200.adapters.wan.modules import _Pipe, wan_rope_table
+    from dax_b200.adapters.wan.training import enable_training
+    net = _blocks(layers=1).bfloat16().to(DEV)
+    enable_training(_Pipe(net))
+    torch.manual_seed(6)
+    args = [torch.randn(s).bfloat16().to(DEV) for s in ((2, 256, 512), (2, 77, 512), (2, 6, 512))]
+    dy = torch.randn(2, 256, 512).bfloat16().to(DEV)
+    tables = [wan_rope_table((2, 8, 16), device=DEV).roll(i, 2) for i in range(6)]
+    rope = tables[0].clone()
+    cached = len(attn_adapter._ROPE_CACHE)
+
+    def step(r):
+        return _step(net, *args, r, dy)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(rope)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step(rope)
+    for t in tables[1:]:
+        want = step(t)
+        rope.copy_(t)
+        graph.replay()
+        torch.cuda.synchronize()
+        for n in want:
+            assert torch.equal(captured[n], want[n]), n
+    assert len(attn_adapter._ROPE_CACHE) == cached

@@ -139,3 +139,20 @@ def test_an_optimised_pipe_is_not_trained():
     replace_transformer(net)
     with pytest.raises(NotImplementedError, match="inference forward"):
         enable_training(_Pipe(net))
+
+
+@pytest.mark.parametrize("dtype", [torch.complex64, torch.complex128])
+def test_training_keeps_no_rotary_tables(dtype):
+    """Tables are made for each call, on the stream of the call: a cache knows neither streams nor captured graphs."""
+    from dax_b200.adapters.wan import attn_adapter, training
+    before = dict(attn_adapter._ROPE_CACHE)
+    ang = torch.rand(1, 1, 20, 64, dtype=torch.float64)
+    table = torch.polar(torch.ones_like(ang), ang).to(dtype)
+    for _ in range(2):
+        cos, sin = training._rotary_tables(table)
+        assert cos.dtype == sin.dtype == torch.float32 and cos.shape == sin.shape == (20, 64) and cos.is_contiguous() and sin.is_contiguous()
+        assert torch.equal(cos, table[0, 0].real.float()) and torch.equal(sin, table[0, 0].imag.float())
+        again = training._rotary_tables(table)
+        assert again[0].data_ptr() != cos.data_ptr() and again[1].data_ptr() != sin.data_ptr()
+        table.conj_physical_()
+    assert attn_adapter._ROPE_CACHE.keys() == before.keys()
