@@ -282,18 +282,20 @@ __global__ void __launch_bounds__(Shape<DT, ELEMS, false>::T, Shape<DT, ELEMS, f
     }
     cta_sum<N, W>(sum, red[parity]);
     float mean[R], rstd[R];
-    bool centre = false;
+    bool centre[R], any = false;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       mean[r] = LN ? sum[R + (LN ? r : 0)] * inv_d : 0.f;
       const float var = fmaf(-mean[r], mean[r], sum[r] * inv_d);
-      if (LN) centre = centre || !(var >= 4.f * mean[r] * mean[r]);
+      centre[r] = LN && !(var >= 4.f * mean[r] * mean[r]);
+      any = any || centre[r];
       rstd[r] = rsqrtf(var + p.eps);
     }
-    if (LN && centre) {
+    if (LN && any) {
       // E[x^2] - mean^2 loses digits where the mean is not small against the spread (every thread sees the same numbers, so
       // the branch is uniform): a second pass around the first estimate of the mean.  It takes the rounding of that
-      // estimate out as well, so that a constant row normalises to zero.
+      // estimate out as well, so that a constant row normalises to zero.  A row that does not need it keeps its first numbers:
+      // its bits do not depend on the row beside it.
 #pragma unroll
       for (int r = 0; r < R; ++r) {
         uint64_t q2 = f2_splat(0.f), s2 = f2_splat(0.f);
@@ -314,6 +316,7 @@ __global__ void __launch_bounds__(Shape<DT, ELEMS, false>::T, Shape<DT, ELEMS, f
       cta_sum<N, W>(sum, red_c[parity]);
 #pragma unroll
       for (int r = 0; r < R; ++r) {
+        if (!centre[r]) continue;
         const float dm = sum[R + (LN ? r : 0)] * inv_d;
         mean[r] += dm;
         rstd[r] = rsqrtf(fmaxf(fmaf(-dm, dm, sum[r] * inv_d), 0.f) + p.eps);
