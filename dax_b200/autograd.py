@@ -29,7 +29,8 @@ class _Attention(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dout):
         q, k, v, out, lse, q_lens, k_lens = ctx.saved_tensors
-        dq, dk, dv = ops.attention_backward(dout, q, k, v, out, lse, q_lens=q_lens, k_lens=k_lens, sm_scale=ctx.sm_scale)
+        dq, dk, dv = ops.attention_backward(dout, q, k, v, out, lse, q_lens=q_lens, k_lens=k_lens, sm_scale=ctx.sm_scale,
+                                            need_keys=any(ctx.needs_input_grad[1:3]))
         return dq, dk, dv, None, None, None
 
 

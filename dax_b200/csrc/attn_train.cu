@@ -1401,6 +1401,7 @@ int run_backward(const CUtensorMap& mq, const CUtensorMap& mdo, const CUtensorMa
     attn_bwd_join_kernel<BF16><<<dim3(static_cast<unsigned>(tiles_of(rows, 8)), 1), 256, 0, st>>>(t, t, s_q, rows, p.Sq, p.heads, p.Sk);
     DAX_CUDA(cudaGetLastError());
   }
+  if (p.dk.p == nullptr) return DAX_OK;  // neither dk nor dv is wanted
   p.splits = s_kv;
   p.part = part_kv;
   DAX_TRY((allow_smem<decltype(&attn_bwd_dkdv_kernel<BF16>), &attn_bwd_dkdv_kernel<BF16>>(KV_SMEM)));
@@ -1486,8 +1487,11 @@ int dax_attn_backward(const void* dout, const void* q, const void* k, const void
   DAX_TRY(check_rows(what, "v", v, v_strides));
   DAX_TRY(check_rows(what, "o", o, o_strides));
   DAX_TRY(check_rows(what, "dq", dq, dq_strides));
-  DAX_TRY(check_rows(what, "dk", dk, dk_strides));
-  DAX_TRY(check_rows(what, "dv", dv, dv_strides));
+  const bool keys = dk != nullptr || dv != nullptr;
+  if (keys) {
+    DAX_TRY(check_rows(what, "dk", dk, dk_strides));
+    DAX_TRY(check_rows(what, "dv", dv, dv_strides));
+  }
   DAX_REQUIRE(lse != nullptr, DAX_ERR_INVALID, "%s: lse is null", what);
   const BackwardLayout w = backward_layout(B * heads, Sq, Sk);
   DAX_REQUIRE(workspace != nullptr && workspace_bytes >= w.bytes, DAX_ERR_INVALID,
@@ -1502,8 +1506,10 @@ int dax_attn_backward(const void* dout, const void* q, const void* k, const void
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   TrainParams p{};
   p.dq = rows_of(dq, dq_strides);
-  p.dk = rows_of(dk, dk_strides);
-  p.dv = rows_of(dv, dv_strides);
+  if (keys) {
+    p.dk = rows_of(dk, dk_strides);
+    p.dv = rows_of(dv, dv_strides);
+  }
   p.lse = const_cast<float*>(lse);
   p.q_lens = q_lens;
   p.k_lens = k_lens;

@@ -709,10 +709,12 @@ def attention_lse(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, q_lens: 
 
 def attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor, lse: torch.Tensor, *,
                        q_lens: Optional[torch.Tensor] = None, k_lens: Optional[torch.Tensor] = None,
-                       sm_scale: Optional[float] = None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+                       sm_scale: Optional[float] = None,
+                       need_keys: bool = True) -> Tuple[torch.Tensor, Optional[torch.Tensor], Optional[torch.Tensor]]:
     """Gradients ``(dq, dk, dv)`` (token-major) of ``attention_lse`` for the output gradient ``dout``, from the same inputs
     and what it returned.  The probabilities are recomputed; sums are fp32 in a fixed order, so equal inputs give equal
-    bits.  Tokens that do not exist get zero gradients and contribute to none."""
+    bits.  Tokens that do not exist get zero gradients and contribute to none.  With ``need_keys=False`` dk and dv are None
+    and their kernel does not run."""
     what = "attention_backward"
     B, heads, Sq, Sk, sm_scale = _attention_inputs(what, q, k, v, q_lens, k_lens, sm_scale)
     for name, t in (("dout", dout), ("out", out)):
@@ -720,10 +722,13 @@ def attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: 
             raise ValueError(f"{what}: {name} must be {list(q.shape)} of {q.dtype}, got {list(t.shape)} of {t.dtype}")
     _vector(what, "lse", lse, (B, heads, Sq))
     dev = _on_one_device(what, dout, q, k, v, out, lse, q_lens, k_lens)
-    dq, dk = _token_major(q), _token_major(k)
-    dv = torch.empty_like(dk)
+    dq = _token_major(q)
+    dk = dv = None
+    if need_keys:
+        dk = _token_major(k)
+        dv = torch.empty_like(dk)
     if lse.numel() == 0 or Sk == 0:
-        return dq.zero_(), dk.zero_(), dv.zero_()
+        return tuple(g if g is None else g.zero_() for g in (dq, dk, dv))
     (dout, dos), (q, qs), (k, ks), (v, vs), (out, os_) = map(_heads_view, (dout, q, k, v, out))
     kv = _token_major_strides(heads, Sk)
     with _OnDevice(dev) as stream:
@@ -733,6 +738,6 @@ def attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: 
         tok = TRACE.begin(what)
         check(lib.dax_attn_backward(dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), _dt(q.dtype),
                                     B, heads, Sq, Sk, dos, qs, ks, vs, os_, sm_scale, _ptr(q_lens), _ptr(k_lens), dq.data_ptr(),
-                                    dk.data_ptr(), dv.data_ptr(), _token_major_strides(heads, Sq), kv, kv, ws.data_ptr(), n, stream))
+                                    _ptr(dk), _ptr(dv), _token_major_strides(heads, Sq), kv, kv, ws.data_ptr(), n, stream))
         TRACE.end(tok, (B, heads, Sq, Sk))
     return dq, dk, dv

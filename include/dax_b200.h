@@ -325,7 +325,8 @@ int dax_rmsnorm_rope_backward(const void* dy, const void* x, int dtype, int64_t 
  * q_lens, k_lens: int32 [B] on the device or NULL (all tokens): tokens from a sample's length on do not exist, whatever they
  * hold (values below 0 and above S count as 0 and S).  Outputs of queries that do not exist or see no key: o = 0,
  * lse = -inf, dq = 0; of keys that do not exist: dk = dv = 0.
- * dax_attn_backward needs o and lse as dax_attn_forward_lse wrote them for the same inputs.  Results do not depend on
+ * dax_attn_backward needs o and lse as dax_attn_forward_lse wrote them for the same inputs.  dk and dv may both be NULL: then
+ * their kernel does not run (dq's always does: it finds what the other needs).  Results do not depend on
  * timing (no atomics): equal inputs give equal bits.
  * Workspaces (16-byte aligned): dax_attn_lse_workspace_bytes may be 0 (then NULL will do).  With few query or key rows the
  * other axis is split over several CTAs, whose fp32 parts it holds; the split depends on the sizes alone.

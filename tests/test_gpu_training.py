@@ -294,3 +294,25 @@ def test_captured_step_follows_its_rotary_table(ag):
         for n in want:
             assert torch.equal(captured[n], want[n]), n
     assert len(attn_adapter._ROPE_CACHE) == cached
+
+
+@pytest.mark.parametrize("shape", [(2, 3, 300, 500), (1, 1, 5000, 60), (1, 1, 40, 4000)])
+def test_frozen_keys_and_values_cost_nothing(ag, monkeypatch, shape):
+    """LoRA on self-attention alone leaves the keys and values of cross-attention without a gradient: theirs is not computed,
+    that of the queries has the same bits."""
+    from dax_b200 import ops
+    B, H, Sq, Sk = shape
+    torch.manual_seed(7)
+    q, do = (torch.randn(B, H, Sq, 128, device=DEV).bfloat16() for _ in range(2))
+    k, v = (torch.randn(B, H, Sk, 128, device=DEV).bfloat16() for _ in range(2))
+    got = []
+    backward = ops.attention_backward
+    monkeypatch.setattr(ops, "attention_backward", lambda *a, **kw: got.append(backward(*a, **kw)) or got[-1])
+    for t in (q, k, v):
+        t.requires_grad_()
+    dq, dk, dv = torch.autograd.grad(ag.attention(q, k, v), (q, k, v), do)
+    only_q, = torch.autograd.grad(ag.attention(q, k.detach(), v.detach()), q, do)
+    only_v, = torch.autograd.grad(ag.attention(q.detach(), k.detach(), v), v, do)
+    assert torch.equal(only_q, dq) and torch.equal(only_v, dv)
+    assert [r[1] is None and r[2] is None for r in got] == [False, True, False]
+    assert ops.attention_backward(do[:, :, :0], q[:, :, :0], k, v, do[:, :, :0], torch.empty(B, H, 0, device=DEV), need_keys=False)[1:] == (None, None)

@@ -156,3 +156,17 @@ def test_training_keeps_no_rotary_tables(dtype):
         assert again[0].data_ptr() != cos.data_ptr() and again[1].data_ptr() != sin.data_ptr()
         table.conj_physical_()
     assert attn_adapter._ROPE_CACHE.keys() == before.keys()
+
+
+def test_attention_gradients_of_keys_and_values_come_together(lib):
+    s = I64x3(76800, 128, 256)
+    n = lib.dax_attn_backward_workspace_bytes(1, 2, 300, 300)
+
+    def call(dk, dv, ws):
+        return lib.dax_attn_backward(ONE, ONE, ONE, ONE, ONE, ONE, _lib.DAX_BF16, 1, 2, 300, 300, s, s, s, s, s, 0.1, None, None, ONE, dk, dv, s,
+                                     s, s, ws, n, None)
+
+    assert call(ONE, None, ONE) == _lib.DAX_ERR_INVALID and b"dv is null" in lib.dax_last_error()
+    assert call(None, ONE, ONE) == _lib.DAX_ERR_INVALID and b"dk is null" in lib.dax_last_error()
+    # neither is wanted: the next check is the workspace's
+    assert call(None, None, None) == _lib.DAX_ERR_INVALID and b"workspace" in lib.dax_last_error()
