@@ -66,6 +66,8 @@ SIGNATURES = {
     "dax_rmsnorm_rope_backward": (c_int, [c_void_p, c_void_p, c_int, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_size_t, c_void_p]),
     "dax_attn_lse_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int64, c_int64]),
     "dax_attn_forward_lse": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int64, c_int64, c_int64, c_int64, I64x3, I64x3, I64x3, c_float, c_void_p, c_void_p, c_void_p, I64x3, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "dax_attn_lse_kernels": (c_int, [c_int64, c_int64, c_int64, c_int64]),
+    "dax_attn_backward_kernels": (c_int, [c_int, c_int64, c_int64, c_int64, c_int64, c_int]),
     "dax_attn_backward_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int64, c_int64]),
     "dax_attn_backward": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int64, c_int64, c_int64, c_int64, I64x3, I64x3, I64x3, I64x3, I64x3, c_float, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, I64x3, I64x3, I64x3, c_void_p, c_size_t, c_void_p]),
 }

@@ -1468,6 +1468,17 @@ int dax_attn_forward_lse(const void* q, const void* k, const void* v, int dtype,
   return dtype == DAX_BF16 ? run_forward<true>(mq, mk, mv, p, st) : run_forward<false>(mq, mk, mv, p, st);
 }
 
+int dax_attn_lse_kernels(int64_t B, int64_t heads, int64_t Sq, int64_t Sk) {
+  if (B <= 0 || heads <= 0 || Sq <= 0 || Sk <= 0) return 0;
+  return dax::forward_splits(B * heads, Sq, Sk) > 1 ? 2 : 1;
+}
+
+int dax_attn_backward_kernels(int dtype, int64_t B, int64_t heads, int64_t Sq, int64_t Sk, int keys) {
+  using namespace dax;
+  if (B <= 0 || heads <= 0 || Sq <= 0 || Sk <= 0) return 0;
+  return (dtype == DAX_F16 ? 1 : 0) + (dq_splits(B * heads, Sq, Sk) > 1 ? 2 : 1) + (keys == 0 ? 0 : dkdv_splits(B * heads, Sq, Sk) > 1 ? 2 : 1);
+}
+
 size_t dax_attn_backward_workspace_bytes(int64_t B, int64_t heads, int64_t Sq, int64_t Sk) {
   if (B <= 0 || heads <= 0 || Sq <= 0 || Sk <= 0) return 0;
   return dax::backward_layout(B * heads, Sq, Sk).bytes;

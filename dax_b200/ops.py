@@ -29,9 +29,7 @@ class _Trace:
     """Optional launch accounting: number of library kernels launched and, when timing is on, CUDA
     events around each wrapper on the stream it launches on (used by the benchmark's roofline leg)."""
 
-    KERNELS_PER_CALL = {"layernorm_modulate_quant": 1, "linear_dynamic": 2, "quant_rowwise": 1, "gemm_dequant": 1, "rmsnorm_rope_pack": 1, "attn_prepare": 5, "attn_forward": 1,
-                        "layernorm_modulate": 1, "layernorm_modulate_backward": 2, "rmsnorm_rope": 1, "rmsnorm_rope_backward": 2,
-                        "attention_lse": 1, "attention_backward": 2}
+    KERNELS_PER_CALL = {"layernorm_modulate_quant": 1, "linear_dynamic": 2, "quant_rowwise": 1, "gemm_dequant": 1, "rmsnorm_rope_pack": 1, "attn_prepare": 5, "attn_forward": 1}
 
     def __init__(self):
         self.launches = 0
@@ -41,8 +39,9 @@ class _Trace:
     def reset(self, timing: bool = False):
         self.launches, self.timing, self.events = 0, timing, []
 
-    def begin(self, name):
-        self.launches += self.KERNELS_PER_CALL[name]
+    def begin(self, name, kernels=None):
+        """``kernels``: how many this call launches, where that goes by its arguments."""
+        self.launches += self.KERNELS_PER_CALL[name] if kernels is None else kernels
         if not self.timing:
             return None
         e0 = torch.cuda.Event(enable_timing=True)
@@ -494,9 +493,16 @@ def _norm_workspace_bytes(device: int, B: int, S: int, D: int) -> int:
 
 
 @functools.lru_cache(maxsize=256)
-def _attention_workspace_bytes(device: int, backward: bool, B: int, heads: int, Sq: int, Sk: int) -> int:
+def _attention_plan(device: int, B: int, heads: int, Sq: int, Sk: int) -> Tuple[int, int]:
+    """Workspace bytes and kernels of the forward pass on the current device, which is ``device``."""
     lib = load()
-    return (lib.dax_attn_backward_workspace_bytes if backward else lib.dax_attn_lse_workspace_bytes)(B, heads, Sq, Sk)
+    return lib.dax_attn_lse_workspace_bytes(B, heads, Sq, Sk), lib.dax_attn_lse_kernels(B, heads, Sq, Sk)
+
+
+@functools.lru_cache(maxsize=256)
+def _attention_backward_plan(device: int, dtype: int, B: int, heads: int, Sq: int, Sk: int, keys: bool) -> Tuple[int, int]:
+    lib = load()
+    return lib.dax_attn_backward_workspace_bytes(B, heads, Sq, Sk), lib.dax_attn_backward_kernels(dtype, B, heads, Sq, Sk, keys)
 
 
 @functools.lru_cache(maxsize=1024)
@@ -532,7 +538,7 @@ def layernorm_modulate(x: torch.Tensor, *, eps: float = 1e-6, ln_weight: Optiona
     mean = _row_statistics(x, B, S)
     rstd = torch.empty_like(mean)
     with _OnDevice(dev) as stream:
-        tok = TRACE.begin(what)
+        tok = TRACE.begin(what, int(rows.numel() > 0))
         check(load().dax_layernorm_modulate(rows.data_ptr(), _dt(x.dtype), B, S, D, sb, ss, _ptr(ln_weight),
                                             _ptr(ln_bias), _ptr(shift), _ptr(scale), float(eps), y.data_ptr(), S * D, D,
                                             mean.data_ptr(), rstd.data_ptr(), stream))
@@ -563,9 +569,10 @@ def layernorm_modulate_backward(dy: torch.Tensor, x: torch.Tensor, mean: torch.T
     dshift, dscale = (torch.empty_like(scale), torch.empty_like(scale)) if need_params and scale is not None else (None, None)
     with _OnDevice(dev) as stream:
         lib, dt = load(), _dt(x.dtype)
-        n = _norm_workspace_bytes(dev, B, S, D) if dweight is not None or dscale is not None else 0
+        sums = dweight is not None or dscale is not None
+        n = _norm_workspace_bytes(dev, B, S, D) if sums else 0
         ws = _workspace(n, x.device)
-        tok = TRACE.begin(what)
+        tok = TRACE.begin(what, (rows.numel() > 0) + sums)
         check(lib.dax_layernorm_modulate_backward(grads.data_ptr(), rows.data_ptr(), dt, B, S, D, gb, gs, sb, ss,
                                                   mean.data_ptr(), rstd.data_ptr(), _ptr(ln_weight), _ptr(ln_bias), _ptr(scale),
                                                   dx.data_ptr(), S * D, D, _ptr(dweight), _ptr(dbias), _ptr(dshift), _ptr(dscale),
@@ -598,7 +605,7 @@ def rmsnorm_rope(x: torch.Tensor, norm_weight: Optional[torch.Tensor] = None, *,
     y = _dense_like(x)
     rstd = _row_statistics(x, B, S)
     with _OnDevice(dev) as stream:
-        tok = TRACE.begin(what)
+        tok = TRACE.begin(what, int(rows.numel() > 0))
         check(load().dax_rmsnorm_rope(rows.data_ptr(), _dt(x.dtype), B, S, D, sb, ss, _ptr(norm_weight), _ptr(rope_cos),
                                       _ptr(rope_sin), float(eps), y.data_ptr(), S * D, D, rstd.data_ptr(), stream))
         TRACE.end(tok, (B, S, D))
@@ -624,7 +631,7 @@ def rmsnorm_rope_backward(dy: torch.Tensor, x: torch.Tensor, rstd: torch.Tensor,
         lib, dt = load(), _dt(x.dtype)
         n = _norm_workspace_bytes(dev, B, S, D) if dweight is not None else 0
         ws = _workspace(n, x.device)
-        tok = TRACE.begin(what)
+        tok = TRACE.begin(what, (rows.numel() > 0) + (dweight is not None))
         check(lib.dax_rmsnorm_rope_backward(grads.data_ptr(), rows.data_ptr(), dt, B, S, D, gb, gs, sb, ss,
                                             rstd.data_ptr(), _ptr(norm_weight), _ptr(rope_cos), _ptr(rope_sin), dx.data_ptr(), S * D, D,
                                             _ptr(dweight), _ptr(ws), n, stream))
@@ -697,9 +704,9 @@ def attention_lse(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, q_lens: 
     (q, qs), (k, ks), (v, vs) = _heads_view(q), _heads_view(k), _heads_view(v)
     with _OnDevice(dev) as stream:
         lib = load()
-        n = _attention_workspace_bytes(dev, False, B, heads, Sq, Sk)
+        n, kernels = _attention_plan(dev, B, heads, Sq, Sk)
         ws = _workspace(n, q.device)
-        tok = TRACE.begin(what)
+        tok = TRACE.begin(what, kernels)
         check(lib.dax_attn_forward_lse(q.data_ptr(), k.data_ptr(), v.data_ptr(), _dt(q.dtype), B, heads, Sq, Sk, qs, ks, vs, sm_scale,
                                        _ptr(q_lens), _ptr(k_lens), out.data_ptr(), _token_major_strides(heads, Sq), lse.data_ptr(),
                                        _ptr(ws), n, stream))
@@ -733,10 +740,11 @@ def attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: 
     kv = _token_major_strides(heads, Sk)
     with _OnDevice(dev) as stream:
         lib = load()
-        n = _attention_workspace_bytes(dev, True, B, heads, Sq, Sk)
+        dt = _dt(q.dtype)
+        n, kernels = _attention_backward_plan(dev, dt, B, heads, Sq, Sk, need_keys)
         ws = _workspace(n, q.device)
-        tok = TRACE.begin(what)
-        check(lib.dax_attn_backward(dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), _dt(q.dtype),
+        tok = TRACE.begin(what, kernels)
+        check(lib.dax_attn_backward(dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), dt,
                                     B, heads, Sq, Sk, dos, qs, ks, vs, os_, sm_scale, _ptr(q_lens), _ptr(k_lens), dq.data_ptr(),
                                     _ptr(dk), _ptr(dv), _token_major_strides(heads, Sq), kv, kv, ws.data_ptr(), n, stream))
         TRACE.end(tok, (B, heads, Sq, Sk))

@@ -330,6 +330,7 @@ int dax_rmsnorm_rope_backward(const void* dy, const void* x, int dtype, int64_t 
  * timing (no atomics): equal inputs give equal bits.
  * Workspaces (16-byte aligned): dax_attn_lse_workspace_bytes may be 0 (then NULL will do).  With few query or key rows the
  * other axis is split over several CTAs, whose fp32 parts it holds; the split depends on the sizes alone.
+ * dax_attn_lse_kernels, dax_attn_backward_kernels: how many kernels a call launches (`keys`: dk and dv are wanted).
  * ------------------------------------------------------------------------------------------- */
 size_t dax_attn_lse_workspace_bytes(int64_t B, int64_t heads, int64_t Sq, int64_t Sk);
 
@@ -338,7 +339,11 @@ int dax_attn_forward_lse(const void* q, const void* k, const void* v, int dtype,
                          const int32_t* k_lens, void* o, int64_t o_strides[3], float* lse, void* workspace, size_t workspace_bytes,
                          void* stream);
 
+int dax_attn_lse_kernels(int64_t B, int64_t heads, int64_t Sq, int64_t Sk);
+
 size_t dax_attn_backward_workspace_bytes(int64_t B, int64_t heads, int64_t Sq, int64_t Sk);
+
+int dax_attn_backward_kernels(int dtype, int64_t B, int64_t heads, int64_t Sq, int64_t Sk, int keys);
 
 int dax_attn_backward(const void* dout, const void* q, const void* k, const void* v, const void* o, const float* lse, int dtype,
                       int64_t B, int64_t heads, int64_t Sq, int64_t Sk, int64_t do_strides[3], int64_t q_strides[3],
