@@ -7,7 +7,7 @@ import logging
 from ...parallel.initialize import initialize
 from .attn_adapter import replace_wan_attention
 from .block_adapter import replace_wan_blocks
-from .transformer_adapter import quantize_transformer, replace_transformer
+from .transformer_adapter import quantize_transformer, refuse_training, replace_transformer
 
 log = logging.getLogger("dax_b200")
 
@@ -20,7 +20,9 @@ def optimize_pipe(pipe, sequence_parallel=True, compile=True, overlap_comm=True,
     "int8_bf16".  ``fp8_linear`` (not in the
     reference's signature, where FP8 is reachable only through ``quantize_dynamic``) selects e4m3
     activations x e4m3 weights; ``fuse_blocks`` binds the fused CUDA forward on every Wan block (LayerNorm /
-    modulation / GELU / gated residuals ride in the quantiser and GEMM kernels)."""
+    modulation / GELU / gated residuals ride in the quantiser and GEMM kernels).  A pipe in training (``enable_training``)
+    is refused."""
+    refuse_training(pipe.transformer)
     sp_size = 1
     if sequence_parallel:
         sp_size = initialize()

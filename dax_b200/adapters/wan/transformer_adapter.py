@@ -19,11 +19,22 @@ from ...quant.quantization import (
 )
 
 
+def refuse_training(transformer) -> None:
+    """Quantised linears and the inference processors and forwards have no gradient: they do not replace those that
+    ``enable_training`` has bound."""
+    from .training import training_block_forward  # which imports this module
+    for name, m in transformer.named_modules():
+        if getattr(getattr(m, "forward", None), "__func__", None) is training_block_forward:
+            raise NotImplementedError(f"{name} is set up for training (enable_training): optimise or quantise a pipe of its own, "
+                                      "with the trained weights loaded")
+
+
 def quantize_transformer(transformer, dtype: str = "int8"):
     """Swap every ``nn.Linear`` of the transformer for the dynamic quantised Linear, except the
     condition embedder and the output projection (``transformer_adapter.py:227-234``).
     ``dtype``: "int8" (the reference's choice), "fp8_e4m3" or "fp8_e5m2" (activation format; FP8
-    weights are e4m3)."""
+    weights are e4m3).  A transformer in training is refused."""
+    refuse_training(transformer)
     if dtype == "int8":
         cfg = get_dynamic_int8_per_token_act_per_channel_weight_qconfig()
     elif dtype in ("fp8", "fp8_e4m3"):

@@ -170,3 +170,20 @@ def test_attention_gradients_of_keys_and_values_come_together(lib):
     assert call(None, ONE, ONE) == _lib.DAX_ERR_INVALID and b"dk is null" in lib.dax_last_error()
     # neither is wanted: the next check is the workspace's
     assert call(None, None, None) == _lib.DAX_ERR_INVALID and b"workspace" in lib.dax_last_error()
+
+
+@pytest.mark.parametrize("kw", [{}, {"int8_linear": True}, {"fuse_blocks": False}])
+def test_a_pipe_in_training_is_not_optimised(kw):
+    """The inference processors and forwards would replace the differentiable ones without a word; nothing is changed."""
+    from dax_b200.adapters.wan import enable_training, optimize_pipe, quantize_transformer
+    from dax_b200.adapters.wan.modules import WanDiT, _Pipe
+    net = WanDiT(layers=1, dim=128, ffn_dim=128, heads=1, text_dim=32, freq_dim=32)
+    pipe = _Pipe(net)
+    assert enable_training(pipe) == 1
+    before = (net.forward.__func__, net.blocks[0].forward.__func__, type(net.blocks[0].attn1.processor), type(net.blocks[0].ffn.net[2]))
+    with pytest.raises(NotImplementedError, match="training"):
+        optimize_pipe(pipe, sequence_parallel=False, overlap_comm=False, compile=False, **kw)
+    with pytest.raises(NotImplementedError, match="training"):
+        quantize_transformer(net, "int8")
+    assert before == (net.forward.__func__, net.blocks[0].forward.__func__, type(net.blocks[0].attn1.processor), type(net.blocks[0].ffn.net[2]))
+    assert enable_training(pipe) == 1  # again is fine
