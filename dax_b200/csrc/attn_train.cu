@@ -69,6 +69,7 @@ struct TrainParams {
   float* range;        // backward, fp16: [2][BH][kRangeChunks]: largest |v_j|^2, then largest |do_i|^2, of each chunk of the head's tokens
   float* part;         // split runs: fp32 partial sums
   float* part_lse;     // split forward runs: [splits, BH, Sq] log2 of each part's sum of exponentials
+  float* part_e;       // split dq runs: [splits, BH, Sq_pad] sums of ds, as row_stats has D
   int* status;
   int B, heads, Sq, Sk, Sq_pad, splits;
   float sm_scale;
@@ -258,6 +259,12 @@ __device__ __forceinline__ float range_max(const float* range, int S) {
   const float v = lane * range_rows(S) < S ? range[lane] : 0.f;
   return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(v)));
 }
+__device__ __forceinline__ float range_of_v(const TrainParams& p, int bh) { return range_max(p.range + static_cast<int64_t>(bh) * kRangeChunks, p.Sk); }
+// A head's factor in dk, over that of p beside it: what -D is kept times for the dk/dv kernel.
+__device__ __forceinline__ float stat_factor(const TrainParams& p, int bh) {
+  const float do_top = range_max(p.range + (static_cast<int64_t>(p.B) * p.heads + bh) * kRangeChunks, p.Sq);
+  return range_factor(do_top * range_of_v(p, bh)) * P_UNSHIFT<false>;
+}
 
 // Largest |v_j|^2 (blockIdx.z 0) and |do_i|^2 (1) of each chunk of tokens that exist: half a warp per token.  A NaN is passed
 // over: what it touches is NaN anyway.  The backward pass of 12 heads x
@@ -316,10 +323,13 @@ __global__ void __launch_bounds__(256) attn_range_kernel(const Rows v, const Row
 // rounded ds of each row, e_i, and subtracts e_i m for an m near the mean key (the first tile's), which is what rounding
 // left of it.
 //
-// D is taken from the rounded o.  What that rounding leaves in ds, p_ij times one number per row, is well below the rounding
-// of ds as long as a row spreads over many keys (from 64 keys on the error of dk does not show it), but with two keys it
-// made dk 2.3 times as inexact as a single rounding.  Where all keys lie in one tile the kernel has sum_j p_ij dp_ij, which is
-// D, at hand, and takes that.
+// D is taken from the rounded o.  What that rounding leaves in ds is p_ij times one number per row, and that number is e_i (the
+// exact ds of a row add up to zero): nothing beside the rounding of ds where a row spreads over many keys, more than it
+// where p_ij is near one.  Where all keys lie in one tile the kernel has e_i before it rounds ds, and takes it out of D.  With
+// more keys e_i is known at the end: the dk/dv kernel gets D + e_i, but dq keeps e_i times (the row's own mean of k - m), for
+// which the sum of p_ij k_j would be needed, one product more.  Error of the norms of dq / dk, bf16, 1,000 x 2,000, in brackets one
+// rounding of the exact result (1.7e-3): scores of unit spread 2.4e-3 / 2.3e-3, of spread 10 (largest p 0.74 on average) 5.2e-3 /
+// 2.7e-3 (dk 5.0e-3 with D alone), of 30 (0.91) 6.4e-3 / 2.6e-3 (6.1e-3); fp16 an eighth of all.
 constexpr int DQ_SLOTS = 6;
 constexpr int DQ_OFF_Q = DQ_SLOTS * TILE_BYTES;
 constexpr int DQ_OFF_MEAN = DQ_OFF_Q;               // [16][128] floats: sums of keys, in the end m in the first row; over q
@@ -355,6 +365,7 @@ attn_bwd_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
   // a split run leaves fp32 sums [split][BH][Sq][128] that are joined afterwards
   float* part = p.part + ((static_cast<int64_t>(split) * p.B * p.heads + bh) * p.Sq + q0) * 128;
   float* stat = p.row_stats + static_cast<int64_t>(bh) * p.Sq_pad + q0;
+  float* part_e = p.part_e + (static_cast<int64_t>(split) * p.B * p.heads + bh) * p.Sq_pad + q0;
   const int64_t stats = static_cast<int64_t>(p.B) * p.heads * p.Sq_pad;
   const int rows_in = min(128, p.Sq - q0);  // rows of the CTA
 
@@ -363,6 +374,7 @@ attn_bwd_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
       stat[threadIdx.x] = -INFINITY;
       stat[stats + threadIdx.x] = 0.f;
     }
+    if (p.splits > 1 && threadIdx.x < 128) part_e[threadIdx.x] = 0.f;
     if (p.splits > 1) zero_rows(part, 512, rows_in, 512);
     else zero_rows(out_ptr(p.dq, b, h, q0), p.dq.st * 2, rows_in, 256);
     return;
@@ -495,11 +507,8 @@ attn_bwd_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
     const bool live = q_row < q_len;
     float* s_mean = reinterpret_cast<float*>(smem + DQ_OFF_MEAN);
     const float l = live ? p.lse[static_cast<int64_t>(bh) * p.Sq + q_row] : -INFINITY;
-    float v_top = 0.f, do_top = 0.f;
-    if constexpr (!BF16) {
-      v_top = range_max(p.range + static_cast<int64_t>(bh) * kRangeChunks, p.Sk);
-      do_top = range_max(p.range + (static_cast<int64_t>(p.B) * p.heads + bh) * kRangeChunks, p.Sq);
-    }
+    float v_top = 0.f;
+    if constexpr (!BF16) v_top = range_of_v(p, bh);
     bool ok = mbar_wait(rows_full, 0, abort_flag);
     {  // a quarter of a row of do to tensor memory, and its part of D to where dq will be
       uint32_t w[16];
@@ -538,7 +547,7 @@ attn_bwd_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
     if constexpr (!BF16) {
       factor = range_factor(sum_of_groups(tm + lanes + T_DQ + 1) * v_top);
       nd *= factor;
-      to_stat = range_factor(do_top * v_top) * P_UNSHIFT<BF16> * power_inverse(factor);
+      to_stat = stat_factor(p, bh) * power_inverse(factor);
     }
     if (cg == 0 && split == 0) {
       stat[r] = nl + P_SHIFT<BF16>;
@@ -675,6 +684,12 @@ attn_bwd_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
       // the softmax over one key is constant: its gradient is zero, not the rounding of dp - D
       const float unscale = BF16 ? 1.f : power_inverse(factor), mul = k_len == 1 ? 0.f : p.sm_scale * unscale;
       const float neg_e = -sum_of_groups(tm + lanes + T_S);
+      if (cg == 0) {  // D + e for the dk/dv kernel (one tile of keys: e is in D already)
+        float off = live && n_all > 1 ? neg_e : 0.f;
+        if constexpr (!BF16) off *= stat_factor(p, bh) * unscale;
+        if (p.splits > 1) part_e[r] = off;
+        else if (n_all > 1) stat[stats + r] += off;  // this thread's own
+      }
       const int rows = max(0, min(32, rows_in - (warp & 3) * 32));
       uint8_t* st = smem + warp * 4096;  // every product and every copy is complete: the ring stages the results
       uint32_t v[32];
@@ -886,11 +901,8 @@ attn_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
     // fp16: 2^P_SHIFT p is at hand and the head's factor times ds is wanted (-D comes with both in it)
     float unscale = 1.f, factor = 1.f;
     if constexpr (!BF16) {
-      const float v_top = range_max(p.range + static_cast<int64_t>(bh) * kRangeChunks, p.Sk);
-      const float do_top = range_max(p.range + (static_cast<int64_t>(p.B) * p.heads + bh) * kRangeChunks, p.Sq);
-      factor = range_factor(do_top * v_top);
-      unscale = power_inverse(factor);
-      factor *= P_UNSHIFT<BF16>;
+      factor = stat_factor(p, bh);
+      unscale = P_UNSHIFT<BF16> * power_inverse(factor);
     }
     const uint64_t factor2 = f2_splat(factor);
     const auto minus_d = [factor2](uint32_t y0, uint32_t y1, uint64_t nd) {
@@ -1259,6 +1271,9 @@ struct JoinTarget {
   const int* k_lens;
   float mul;
   bool scores;  // dq, dk: a gradient through the scores, zero where there is one key only
+  const float* part_e;  // dq: its parts of the rows' e ...
+  float* stat;          // ... and -D, which takes their sum: [BH, Sq_pad]
+  int S_pad;
 };
 template <bool BF16>
 __global__ void __launch_bounds__(256) attn_bwd_join_kernel(const JoinTarget t0, const JoinTarget t1, int splits, int64_t rows,
@@ -1277,6 +1292,12 @@ __global__ void __launch_bounds__(256) attn_bwd_join_kernel(const JoinTarget t0,
   }
   const float mul = t.scores && valid_len(t.k_lens, b, Sk) == 1 ? 0.f : t.mul;
   store4<BF16>(out_ptr(t.out, b, bh % heads, s) + c, acc, mul);
+  if (t.stat != nullptr && c == 0) {
+    const int64_t at = static_cast<int64_t>(bh) * t.S_pad + s, stride = rows / S * t.S_pad;
+    float off = 0.f;
+    for (int k = 0; k < splits; ++k) off += t.part_e[k * stride + at];
+    t.stat[at] += off;
+  }
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------------
@@ -1308,13 +1329,14 @@ inline int dkdv_splits(int64_t BH, int64_t Sq, int64_t Sk) { return choose_split
 inline int64_t pad128(int64_t S) { return tiles_of(S, 128) * 128; }
 inline size_t round256(size_t n) { return (n + 255) / 256 * 256; }
 
-struct BackwardLayout { size_t stats, range, dq, dkdv, bytes; };
+struct BackwardLayout { size_t stats, range, e, dq, dkdv, bytes; };
 inline BackwardLayout backward_layout(int64_t BH, int64_t Sq, int64_t Sk) {
   BackwardLayout w{};
   const int s_q = dq_splits(BH, Sq, Sk), s_kv = dkdv_splits(BH, Sq, Sk);
   w.stats = 0;
   w.range = round256(static_cast<size_t>(BH) * pad128(Sq) * 8);
-  w.dq = w.range + round256(static_cast<size_t>(BH) * kRangeChunks * 8);
+  w.e = w.range + round256(static_cast<size_t>(BH) * kRangeChunks * 8);
+  w.dq = w.e + (s_q > 1 ? round256(static_cast<size_t>(s_q) * BH * pad128(Sq) * 4) : 0);
   w.dkdv = w.dq + (s_q > 1 ? round256(static_cast<size_t>(s_q) * BH * Sq * 512) : 0);
   w.bytes = w.dkdv + (s_kv > 1 ? round256(static_cast<size_t>(s_kv) * BH * Sk * 1024) : 0);
   return w;
@@ -1397,7 +1419,7 @@ int run_backward(const CUtensorMap& mq, const CUtensorMap& mdo, const CUtensorMa
   DAX_CUDA(cudaGetLastError());
   if (s_q > 1) {
     const int64_t rows = static_cast<int64_t>(BH) * p.Sq;
-    const JoinTarget t = {p.dq, part_q, p.k_lens, p.sm_scale, true};
+    const JoinTarget t = {p.dq, part_q, p.k_lens, p.sm_scale, true, p.part_e, p.row_stats + static_cast<int64_t>(BH) * p.Sq_pad, p.Sq_pad};
     attn_bwd_join_kernel<BF16><<<dim3(static_cast<unsigned>(tiles_of(rows, 8)), 1), 256, 0, st>>>(t, t, s_q, rows, p.Sq, p.heads, p.Sk);
     DAX_CUDA(cudaGetLastError());
   }
@@ -1409,8 +1431,8 @@ int run_backward(const CUtensorMap& mq, const CUtensorMap& mdo, const CUtensorMa
   DAX_CUDA(cudaGetLastError());
   if (s_kv > 1) {
     const int64_t rows = static_cast<int64_t>(BH) * p.Sk;
-    const JoinTarget tk = {p.dk, part_kv, p.k_lens, p.sm_scale, true},
-                     tv = {p.dv, part_kv + s_kv * rows * 128, p.k_lens, 1.f, false};
+    const JoinTarget tk = {p.dk, part_kv, p.k_lens, p.sm_scale, true, nullptr, nullptr, 0},
+                     tv = {p.dv, part_kv + s_kv * rows * 128, p.k_lens, 1.f, false, nullptr, nullptr, 0};
     attn_bwd_join_kernel<BF16><<<dim3(static_cast<unsigned>(tiles_of(rows, 8)), 2), 256, 0, st>>>(tk, tv, s_kv, rows, p.Sk, p.heads, p.Sk);
     DAX_CUDA(cudaGetLastError());
   }
@@ -1526,6 +1548,7 @@ int dax_attn_backward(const void* dout, const void* q, const void* k, const void
   p.k_lens = k_lens;
   p.row_stats = reinterpret_cast<float*>(ws + w.stats);
   p.range = reinterpret_cast<float*>(ws + w.range);
+  p.part_e = reinterpret_cast<float*>(ws + w.e);
   p.status = device_status_ptr();
   DAX_REQUIRE(p.status != nullptr, DAX_ERR_CUDA, "%s: cannot resolve the device status word", what);
   p.B = static_cast<int>(B);
