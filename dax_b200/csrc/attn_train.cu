@@ -365,7 +365,7 @@ attn_bwd_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
   // a split run leaves fp32 sums [split][BH][Sq][128] that are joined afterwards
   float* part = p.part + ((static_cast<int64_t>(split) * p.B * p.heads + bh) * p.Sq + q0) * 128;
   float* stat = p.row_stats + static_cast<int64_t>(bh) * p.Sq_pad + q0;
-  float* part_e = p.part_e + (static_cast<int64_t>(split) * p.B * p.heads + bh) * p.Sq_pad + q0;
+  const auto part_e = [&] { return p.part_e + (static_cast<int64_t>(split) * p.B * p.heads + bh) * p.Sq_pad + q0; };
   const int64_t stats = static_cast<int64_t>(p.B) * p.heads * p.Sq_pad;
   const int rows_in = min(128, p.Sq - q0);  // rows of the CTA
 
@@ -374,7 +374,7 @@ attn_bwd_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
       stat[threadIdx.x] = -INFINITY;
       stat[stats + threadIdx.x] = 0.f;
     }
-    if (p.splits > 1 && threadIdx.x < 128) part_e[threadIdx.x] = 0.f;
+    if (p.splits > 1 && threadIdx.x < 128) part_e()[threadIdx.x] = 0.f;
     if (p.splits > 1) zero_rows(part, 512, rows_in, 512);
     else zero_rows(out_ptr(p.dq, b, h, q0), p.dq.st * 2, rows_in, 256);
     return;
@@ -639,6 +639,9 @@ attn_bwd_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
     if (n_all == 1) ok = ok && tile(0, std::true_type{});
     else
       for (int j = 0; ok && j < n; ++j) ok = tile(j, std::false_type{});
+    // for the end; read again instead of kept in registers over the loop
+    const float minus_d_stat = cg == 0 && p.splits == 1 ? stat[stats + r] : 0.f;  // this thread's own
+    if constexpr (!BF16) to_stat = stat_factor(p, bh) * power_inverse(factor);
     // m: the mean of the first tile's keys; a thread adds eight channels of four keys
     if (ok) ok = mbar_wait(&full[(2 * n) % DQ_SLOTS], ((2 * n) / DQ_SLOTS) & 1u, abort_flag);
     {
@@ -685,10 +688,9 @@ attn_bwd_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
       const float unscale = BF16 ? 1.f : power_inverse(factor), mul = k_len == 1 ? 0.f : p.sm_scale * unscale;
       const float neg_e = -sum_of_groups(tm + lanes + T_S);
       if (cg == 0) {  // D + e for the dk/dv kernel (one tile of keys: e is in D already)
-        float off = live && n_all > 1 ? neg_e : 0.f;
-        if constexpr (!BF16) off *= stat_factor(p, bh) * unscale;
-        if (p.splits > 1) part_e[r] = off;
-        else if (n_all > 1) stat[stats + r] += off;  // this thread's own
+        const float off = live && n_all > 1 ? neg_e : 0.f;
+        if (p.splits > 1) part_e()[r] = off * to_stat;
+        else stat[stats + r] = fmaf(off, to_stat, minus_d_stat);
       }
       const int rows = max(0, min(32, rows_in - (warp & 3) * 32));
       uint8_t* st = smem + warp * 4096;  // every product and every copy is complete: the ring stages the results
