@@ -11,9 +11,9 @@
 // order of addition that changes from run to run) and, with a 128-wide tile of one SM, its operand reads need more
 // shared-memory bandwidth than the seven products here, four of which take their A operand from tensor memory.
 //
-// Bound by the tensor cores and, in long runs, by power (the SM clock falls to 1.65 GHz).  Measured, bf16: forward 1,200
-// TFLOP/s at 5 heads x 16,384 tokens (573 us), 1,240 at 40 x 4,096; backward 941 and 908 TFLOP/s of its own ten operations per
-// pair and channel, 1,318 and 1,271 of the fourteen that the seven products do (1,826 and 946 us).  A library product
+// Bound by the tensor cores and, in long runs, by power (the SM clock falls to 1.65 GHz).  Measured, bf16: forward 1,215
+// TFLOP/s at 5 heads x 16,384 tokens (566 us), 1,240 at 40 x 4,096; backward 943 and 900 TFLOP/s of its own ten operations per
+// pair and channel, 1,320 and 1,260 of the fourteen that the seven products do (1,821 and 955 us; fp16 1,945 and 1,035).  A library product
 // of 16-bit matrices reaches 1,615 for a moment and 1,373 for seconds.
 //
 // q_lens / k_lens (per sample, optional) bound the tokens that exist: rows behind a length take no part in anything (not
@@ -267,8 +267,8 @@ __device__ __forceinline__ float stat_factor(const TrainParams& p, int bh) {
 }
 
 // Largest |v_j|^2 (blockIdx.z 0) and |do_i|^2 (1) of each chunk of tokens that exist: half a warp per token.  A NaN is passed
-// over: what it touches is NaN anyway.  The backward pass of 12 heads x
-// 4,095 x 4,095 takes 316 us with it and the factors, 307 without.
+// over: what it touches is NaN anyway.  12 heads x 4,095 x 4,095: 10 us for 25 MB from DRAM (most of it latency; eight loads in
+// flight instead of four change nothing), the backward pass takes 316 us with it and the factors, 307 without.
 __global__ void __launch_bounds__(256) attn_range_kernel(const Rows v, const Rows dout, const TrainParams p) {
   const bool keys = blockIdx.z == 0;
   const Rows& t = keys ? v : dout;
@@ -311,7 +311,7 @@ __global__ void __launch_bounds__(256) attn_range_kernel(const Rows v, const Row
 //                for the multiply-add pipe and for tensor memory, fall into each other
 //   producer     q, and do and o in the ring's last two slots; then k_0, v_0, k_1, ... through the ring, at last k's first tile
 //   issuer 0     s = q.k_j^T and dp = do.v_j^T        issuer 1     dq += ds.k_j
-// 8 heads x 4,096 x 4,096 bf16: 96 us, 1.3 us per tile of keys and CTA and about 6 us around them; tensor pipe 66 % of the
+// 8 heads x 4,096 x 4,096 bf16: 97 us, 1.3 us per tile of keys and CTA and about 6 us around them; tensor pipe 66 % of the
 // time, unit of the exponentials 45 %.
 // Tensor memory: s [0,128)  dp [128,256)  dq [256,384)  do [384,448)  ds [448,512).  do and ds are A operands in tensor
 // memory, so of the three products only s reads both operands from shared memory, whose bandwidth would otherwise be the
@@ -639,8 +639,11 @@ attn_bwd_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
     if (n_all == 1) ok = ok && tile(0, std::true_type{});
     else
       for (int j = 0; ok && j < n; ++j) ok = tile(j, std::false_type{});
-    // for the end; read again instead of kept in registers over the loop
-    const float minus_d_stat = cg == 0 && p.splits == 1 ? stat[stats + r] : 0.f;  // this thread's own
+    // for the end; read (and its address computed) again instead of kept in registers over the loop
+    int q_end = q0 + r;
+    asm volatile("" : "+r"(q_end));
+    float* stat_d = p.row_stats + (static_cast<int64_t>(p.B) * p.heads + bh) * p.Sq_pad + q_end;
+    const float minus_d_stat = cg == 0 && p.splits == 1 ? *stat_d : 0.f;  // this thread's own
     if constexpr (!BF16) to_stat = stat_factor(p, bh) * power_inverse(factor);
     // m: the mean of the first tile's keys; a thread adds eight channels of four keys
     if (ok) ok = mbar_wait(&full[(2 * n) % DQ_SLOTS], ((2 * n) / DQ_SLOTS) & 1u, abort_flag);
@@ -688,9 +691,9 @@ attn_bwd_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
       const float unscale = BF16 ? 1.f : power_inverse(factor), mul = k_len == 1 ? 0.f : p.sm_scale * unscale;
       const float neg_e = -sum_of_groups(tm + lanes + T_S);
       if (cg == 0) {  // D + e for the dk/dv kernel (one tile of keys: e is in D already)
-        const float off = live && n_all > 1 ? neg_e : 0.f;
+        const float off = live && k_len > 128 ? neg_e : 0.f;
         if (p.splits > 1) part_e()[r] = off * to_stat;
-        else stat[stats + r] = fmaf(off, to_stat, minus_d_stat);
+        else *stat_d = fmaf(off, to_stat, minus_d_stat);
       }
       const int rows = max(0, min(32, rows_in - (warp & 3) * 32));
       uint8_t* st = smem + warp * 4096;  // every product and every copy is complete: the ring stages the results
