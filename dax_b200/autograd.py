@@ -2,7 +2,8 @@
 
 Thin ``torch.autograd.Function`` wrappers over the forward / backward pairs of ``dax_b200.ops``.  The forward passes keep
 their inputs and the row statistics, the backward passes recompute the rest; gradients of inputs that do not need one are
-not computed where that saves work.  Gradients of gradients are not available.
+not computed where that saves work (dk and dv of attention together, the parameters of the norms together).  Gradients of
+gradients, forward-mode derivatives and ``vmap`` are not available: PyTorch raises.
 
 All of them can be captured into a CUDA graph.  A captured backward pass must not meet an eager autograd graph of the same
 leaves that is still alive (PyTorch ties a leaf's accumulation to the stream it was first used on): drop the results of

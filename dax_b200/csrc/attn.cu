@@ -101,9 +101,8 @@ __device__ __forceinline__ void mma_tile(uint32_t d_tmem, uint32_t a_addr, uint3
   }
 }
 
-// Two fp32 values -> bf16x2 by keeping the upper halves (one byte-permute for two elements; the
-// rounding conversion instructions run on the 16-per-clock unit the exponentials already saturate).
-// Truncation lowers every P by 2^-9 on average; the epilogue multiplies O by (1 + 2^-9) to centre it.
+// Two fp32 values -> bf16x2 by keeping the upper halves: one byte-permute for two elements (as many per clock as
+// rounding conversions).  Truncation lowers every P by 2^-9 on average; the epilogue multiplies O by (1 + 2^-9) to centre it.
 __device__ __forceinline__ uint32_t pack_bf16x2_trunc(float a, float b) {
   uint32_t r;
   asm("prmt.b32 %0, %1, %2, 0x7632;" : "=r"(r) : "r"(__float_as_uint(a)), "r"(__float_as_uint(b)));

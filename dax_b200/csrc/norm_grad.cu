@@ -21,9 +21,10 @@
 // shared memory allow, and two to four CTAs per SM fill each other's waits.
 // Statistics, coefficients and sums are fp32; y and dx are rounded once, when they are stored.
 //
-// Measured (x and y, or x, dy and dx, once each; a plain copy reaches 6.5 TB/s): 32,760 x 5,120 bf16 LayerNorm + modulation
-// 117 us (5.7 TB/s) forward, 191 (5.3) backward with its sums, RMSNorm + rotation 111 (6.0) and 211 (4.8); 6,240 x 5,120 fp32
-// 53 (4.9) and 89 (4.3).  What is left beside the bytes is issue slots (58 % used in the backward pass, two rounds over a row
+// Measured (x and y, or x, dy and dx, once each, each pass on its own, replayed from a graph; a plain copy reaches 6.5 TB/s),
+// us forward and backward with its sums: 32,760 x 5,120 bf16 LayerNorm + modulation 118 (5.7 TB/s) and 183 (5.5), RMSNorm +
+// rotation 109 (6.2) and 204 (4.9), fp16 118 and 207, 109 and 211; 16,380 x 5,120 fp32 124 (5.4) and 183 (5.5), 120 (5.6) and 189 (5.3);
+// 2 x 4,095 x 1,536 fp16 affine LayerNorm 12 and 27.  What is left beside the bytes is issue slots (58 % used in the backward pass, two rounds over a row
 // that lives in shared memory) and the waits for a row's sums.
 #include <algorithm>
 #include <atomic>
@@ -600,7 +601,10 @@ __global__ void __launch_bounds__(512, 2) norm_join_kernel(const JoinArgs p) {
 // Elements of a row per thread: few while the rows are narrow, so that there are threads; at most 320 threads.  Between
 // 2,560 and 5,120 channels 16 and 32 both fit; which is faster goes by the registers that the pass needs beside the row
 // (32,760 x 5,120 bf16, us, 16 / 32: LayerNorm forward 117 / 124, backward 205 / 193, RMSNorm 118 / 112 and 211 / 225;
-// fp32 6,240 rows, LayerNorm: 52 / 54 and 89 / 104).
+// fp32 6,240 rows, LayerNorm: 52 / 54 and 89 / 104).  Between (2,688, 3,584, 4,096 and 4,608
+// channels, tensors of 210 MB, us, smallest and largest time with 16 / with 32): bf16 LayerNorm forward 69-75 / 69-71, backward 134-142 /
+// 112-129, RMSNorm forward 78-84 / 71-78, backward 138-150 / 132-149 (with 32 5 and 7 % faster at 3,584 and 4,096, slower at the
+// others); fp32 LayerNorm 78-80 / 78-79 and 100-107 / 127-141, RMSNorm 77-81 / 70-76 (16 costs 6 to 12 % there) and 120-128 / 128-138.
 inline int row_elems(int64_t D, int dtype, bool ln, bool backward) {
   return D <= 1024 ? 8 : (D <= (dtype != DAX_F32 && ln == backward ? 2560 : 5120) ? 16 : 32);
 }
