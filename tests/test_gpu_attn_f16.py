@@ -187,3 +187,62 @@ def test_maxima_that_rise_tile_by_tile(ops, step):
     err = U + 2.0 ** -19 + 2.0 ** -23 * 7 * step + S * W
     assert bool(((out[0, 0].double() - want).abs() <= (err * (1 + U) + U) * want).all())
     assert bool(((lse.double() - torch.logsumexp(s, 0)).abs() <= 2.0 ** -18 + 2.0 ** -22 * 7 * step).all())
+
+
+def test_layouts_and_far_offsets(ops):
+    """The largest norms are found through the tensors' own strides: heads inside a wider projection, every second token, tokens
+    more than 2^32 bytes apart."""
+    B, H, S, far = 2, 3, 300, 1 << 22
+    g = torch.Generator(device=DEV).manual_seed(7)
+    q, k, v, do = ((torch.randn(B, S, H, 128, generator=g, device=DEV) * s).half().transpose(1, 2) for s in (1.0, 1.0, 1.0, 1e-3))
+    v[1, 2, 250] *= 30
+    want = run(ops, q, k, v, do)
+    for f in (lambda t: t.contiguous(), lambda t: torch.cat([1000 * t, t], 1)[:, H:], lambda t: torch.stack([t, 1000 * t], 3).flatten(2, 3)[:, :, ::2]):
+        assert all(torch.equal(a, b) for a, b in zip(run(ops, f(q), f(k), f(v), f(do)), want))
+    if torch.cuda.mem_get_info()[0] < 24 << 30:
+        pytest.skip("needs 24 GB")
+    buf = torch.full((2 * S * far,), 1000.0, dtype=torch.float16, device=DEV)
+    views = [torch.as_strided(buf, (B, H, S, 128), (S * far, 512, far, 1), 128 * i) for i in range(4)]
+    for t, x in zip(views, (q, k, v, do)):
+        t.copy_(x)
+    assert all(torch.equal(a, b) for a, b in zip(run(ops, *views), want))
+
+
+@pytest.mark.parametrize("shape", [(2, 2, 200, 700), (1, 1, 40, 4000), (1, 1, 4000, 40)])
+def test_captured_factors_follow_the_inputs(ops, shape):
+    """Two graphs replayed in turn on inputs a thousand times larger and smaller than those of the capture: the bits of eager calls."""
+    B, H, Sq, Sk = shape
+    g = torch.Generator(device=DEV).manual_seed(8)
+    make = lambda s: [(torch.randn(B, H, S, 128, generator=g, device=DEV) * f).half() for S, f in ((Sq, 1.0), (Sk, 1.0), (Sk, s), (Sq, s))]  # noqa: E731
+    static, graphs, outs = [make(0.1), make(3.0)], [], []
+    for st in static:
+        run(ops, *st)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(run(ops, *st))
+        graphs.append(graph)
+    for s in (1e-3, 100.0):
+        fresh = [make(s), make(s)]
+        for st, new in zip(static, fresh):
+            for a, b in zip(st, new):
+                a.copy_(b)
+        for graph in graphs + graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        for o, new in zip(outs, fresh):
+            assert all(torch.equal(a, b) for a, b in zip(o, run(ops, *new)))
+
+
+def test_equal_inputs_give_equal_bits_on_any_stream(ops):
+    for shape in ((300, 500), (100, 4000), (4000, 100)):
+        q, k, v, do = draw(*shape, 1.0, 1e-2, seed=9)
+        want = run(ops, q, k, v, do)
+        torch.cuda.synchronize()
+        streams, got = [torch.cuda.Stream() for _ in range(2)], []
+        for _ in range(3):
+            for s in streams:
+                with torch.cuda.stream(s):
+                    got.append(run(ops, q, k, v, do))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for r in got for a, b in zip(r, want))
